@@ -461,6 +461,60 @@ B200ASR_API int b200asr_conv3x3s2_gelu(const void *x, int32_t n, int32_t h, int3
                                        int64_t y_stride_x, int32_t *error_flag,
                                        b200asr_stream_t stream);
 
+/* ------------------------------------------------------ 4-bit paged KV cache ----
+ * A cached head row of D values (D = 64 or 128) is D / 2 bytes of codes (value 2j in the
+ * low half of byte j) plus a bf16 scale and a bf16 zero: value = zero + code * scale.
+ * zero is the row's minimum, scale the smallest bf16 with 15 * scale >= maximum - minimum
+ * (0 for a row narrower than 2^-100); a row with an infinity or a NaN reads as NaN.
+ * No reference counterpart (its cache is bf16, engine/model_runner.py:116-131).
+ *   k_codes, v_codes  uint8 [num_blocks, block_size, num_kv_heads, D / 2]
+ *   params            bf16 [num_blocks, block_size, num_kv_heads, 4]: K scale, K zero,
+ *                     V scale, V zero
+ *   code_stride       bytes between blocks, slots, heads of k_codes and of v_codes
+ *                     (multiples of 16; rows are contiguous, bases 16-byte aligned)
+ *   param_stride      the same of params, in elements (multiples of 4; base 8-byte aligned) */
+typedef struct {
+  void *k_codes, *v_codes, *params;
+  int64_t code_stride[3], param_stride[3];
+  int32_t num_blocks, block_size, num_kv_heads, head_dim;
+} b200asr_kv4;
+
+/* key/value bf16 [num_tokens, num_kv_heads, D] (token and head strides in elements,
+ * multiples of 8) quantised into their slots; slot -1 is skipped (store_kvcache,
+ * layers/attention.py:52-67). No slot may occur twice. Rows of other slots are untouched. */
+B200ASR_API int b200asr_store_kvcache4(const void *key, int64_t key_token_stride,
+                                       int64_t key_head_stride, const void *value,
+                                       int64_t value_token_stride, int64_t value_head_stride,
+                                       const b200asr_kv4 *cache, const int32_t *slot_mapping,
+                                       int32_t num_tokens, int32_t *error_flag,
+                                       b200asr_stream_t stream);
+/* The rows of `slots` as bf16 key/value (the inverse); slot -1 reads as zeros. */
+B200ASR_API int b200asr_load_kvcache4(const b200asr_kv4 *cache, const int32_t *slots,
+                                      int32_t num_tokens, void *key, int64_t key_token_stride,
+                                      int64_t key_head_stride, void *value,
+                                      int64_t value_token_stride, int64_t value_head_stride,
+                                      int32_t *error_flag, b200asr_stream_t stream);
+
+/* paged_decode over the 4-bit cache (layers/attention.py:96-107 with max_seqlen_q = 1):
+ * q/out bf16 [>= batch, num_heads, D] with row and head strides in elements (multiples of
+ * 8), any num_heads that is a multiple of the cache's num_kv_heads. cu_seqlens_k int32
+ * [batch + 1]; block_tables int32 [batch, bt_width], row stride bt_stride. A row without a
+ * cached token gives zeros; rows of out past `batch` are left alone. A length beyond
+ * bt_width blocks is cut there (B200ASR_DEVERR_LENGTH); every length must be <=
+ * max_seqlen_k. The workspace needs no initial value and keeps nothing between calls; it is
+ * b200asr_paged_decode4_workspace_size bytes (0 for max_seqlen_k <= 512), 16-byte aligned,
+ * and serves one call at a time. */
+B200ASR_API size_t b200asr_paged_decode4_workspace_size(int32_t max_seqlen_k, int32_t num_heads,
+                                                        int32_t num_kv_heads, int32_t head_dim);
+B200ASR_API int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
+                                      const b200asr_kv4 *cache, int32_t num_heads,
+                                      const int32_t *cu_seqlens_k, const int32_t *block_tables,
+                                      int64_t bt_stride, int32_t bt_width, int32_t batch,
+                                      int32_t max_seqlen_k, float scale, void *out,
+                                      int64_t out_row_stride, int64_t out_head_stride,
+                                      void *workspace, size_t workspace_bytes,
+                                      int32_t *error_flag, b200asr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

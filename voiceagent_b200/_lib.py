@@ -87,6 +87,14 @@ SIGNATURES: dict[str, tuple] = {
     "b200asr_conv_pack_weight": (c_int32, [P, c_int32, c_int32, P, P]),
     "b200asr_conv3x3s2_gelu": (c_int32, [P, c_int32, c_int32, c_int32, c_int32, P, P, c_int32,
                                          P, c_int64, c_int64, c_int64, P, P]),
+    "b200asr_store_kvcache4": (c_int32, [P, c_int64, c_int64, P, c_int64, c_int64, P, P, c_int32,
+                                         P, P]),
+    "b200asr_load_kvcache4": (c_int32, [P, P, c_int32, P, c_int64, c_int64, P, c_int64, c_int64,
+                                        P, P]),
+    "b200asr_paged_decode4_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    "b200asr_paged_decode4": (c_int32, [P, c_int64, c_int64, P, c_int32, P, P, c_int64, c_int32,
+                                        c_int32, c_int32, c_float, P, c_int64, c_int64, P,
+                                        c_size_t, P, P]),
 }
 
 
@@ -97,6 +105,15 @@ class L2Prefetch(ctypes.Structure):
                 ("batch", c_int32), ("block_size", c_int32), ("num_kv_heads", c_int32),
                 ("head_dim", c_int32), ("k_cache", c_void_p), ("v_cache", c_void_p),
                 ("num_slots", c_int64), ("range", c_void_p * 2), ("range_bytes", c_int64 * 2)]
+
+
+class Kv4(ctypes.Structure):
+    """``b200asr_kv4`` (include/b200asr.h), passed by pointer."""
+
+    _fields_ = [("k_codes", c_void_p), ("v_codes", c_void_p), ("params", c_void_p),
+                ("code_stride", c_int64 * 3), ("param_stride", c_int64 * 3),
+                ("num_blocks", c_int32), ("block_size", c_int32), ("num_kv_heads", c_int32),
+                ("head_dim", c_int32)]
 
 
 class B200AsrError(RuntimeError):

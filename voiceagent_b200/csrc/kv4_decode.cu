@@ -1,0 +1,746 @@
+// One-token attention over the 4-bit paged KV cache (kv4.cuh has the format).
+//
+// The 4-bit form of paged_decode (layers/attention.py:96-107 with max_seqlen_q = 1):
+//   out[b, h] = softmax(q[b, h] K_b^T * scale) V_b,
+// with a row's codes c and parameters (scale, zero):
+//   score_t = ks_t (q . c_t) + kz_t sum(q),     out = (sum_t (p_t vs_t) c'_t + sum_t p_t vz_t) / sum_t p_t.
+// Codes go through the tensor cores as bf16 whole numbers, exact in bf16: q . c needs no
+// dequantised K, and the V scale goes into the probability before its rounding to bf16
+// (which the bf16 form of this kernel rounds as well). Everything else is held in 32 bits.
+//
+// What bounds it: at 136 bytes per cached (token, KV head) of D = 128 the bytes are a quarter
+// of the bf16 cache's, and turning codes into MMA operands costs ~240 instructions per 16
+// tokens, ~65 % of the SM's issue slots at the copy rate of HBM; so instructions are counted:
+//  * MMA m16n8k16 with cached tokens (scores) or dims (output) as its 16 rows and the group's
+//    query heads as its 8 columns. A word of 8 codes becomes four bf16 pairs by
+//    (w >> 4 i) & 0x000f000f | 0x43004300, each 128 + code. For K the 128 is taken off by
+//    the accumulator's start value -128 sum(q); for V, whose accumulator runs over the whole
+//    context, the pair is lowered by 136 to code - 8, small and centred, and the zero moves up
+//    by 8 steps.
+//  * The rows' dims are assigned to lanes so that a lane's codes are contiguous bytes: 16 of a
+//    K row, 8 of a V row.
+//  * A warp keeps its own ring of cp.async stages (32 tokens each) and its own softmax state:
+//    no barrier inside a segment. The running maximum moves only when a score passes it by 8
+//    (base 2), so most stages need one vote instead of reductions and rescales.
+// Work split: (sequence, KV head) pairs are cut into rounds of 128 tokens (4 warps x 32), laid
+// end to end and divided evenly among the CTAs whatever the length mix. A pair that several
+// CTAs share leaves fp32 partials in the workspace, and a second kernel joins them in token
+// order (the result does not depend on timing). Nothing in the workspace outlives the call.
+#include "kv4.cuh"
+
+namespace b200asr {
+
+constexpr int kD4Warps = 4;
+constexpr int kD4Tile = 32;                      // tokens of a warp's stage
+constexpr int kD4Round = kD4Warps * kD4Tile;     // tokens of a CTA's round
+constexpr int kD4Stages = 3;
+constexpr int kD4CtasPerSm = 3;
+constexpr float kD4Lazy = 8.f;                   // base-2 slack of the running maximum
+
+struct Decode4Args {
+  const __nv_bfloat16 *q;
+  int64_t q_row, q_head;
+  b200asr_kv4 c;
+  const int32_t *cu_seqlens_k;
+  const int32_t *block_tables;
+  int64_t bt_stride;
+  int bt_width;
+  int batch;
+  int group;      // query heads of a KV head
+  int subs;       // column groups of 8 * NT query heads per KV head
+  int bs_shift;   // log2(block_size), or -1
+  int whole;      // a CTA per (sequence, head) pair: nothing is split
+  float scale_log2;
+  __nv_bfloat16 *out;
+  int64_t out_row, out_head;
+  float *ws;      // partials: [2 * ctas][8 * NT][D + 2]
+  int32_t *error_flag;
+};
+
+// The sequence's cached tokens, held to what its table row can address.
+__device__ __forceinline__ int decode4_len(const Decode4Args &a, int b) {
+  const int len = max(0, a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b]);
+  return static_cast<int>(min(static_cast<int64_t>(len),
+                              static_cast<int64_t>(a.bt_width) * a.c.block_size));
+}
+
+__device__ __forceinline__ int rounds_of(int len) { return (len + kD4Round - 1) / kD4Round; }
+
+// Rounds of all pairs, and of the pairs of sequences before `upto` (block-wide; 128 threads).
+__device__ __forceinline__ int64_t decode4_rounds(const Decode4Args &a, int pairs, int upto,
+                                                  int64_t &before) {
+  __shared__ int64_t part[2][kD4Warps];
+  int64_t all = 0, some = 0;
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+    const int r = rounds_of(decode4_len(a, b));
+    all += r;
+    if (b < upto) some += r;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    some += __shfl_xor_sync(0xffffffffu, some, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    part[0][threadIdx.x >> 5] = all;
+    part[1][threadIdx.x >> 5] = some;
+  }
+  __syncthreads();
+  all = some = 0;
+#pragma unroll
+  for (int w = 0; w < kD4Warps; ++w) {
+    all += part[0][w];
+    some += part[1][w];
+  }
+  before = some * pairs;
+  __syncthreads();
+  return all * pairs;
+}
+
+// CTA c's first unit of `units` dealt evenly to `ctas`, and the CTA of unit u.
+__device__ __forceinline__ int64_t first_unit(int64_t units, int ctas, int c) {
+  return units / ctas * c + min(static_cast<int64_t>(c), units % ctas);
+}
+__device__ __forceinline__ int cta_of_unit(int64_t units, int ctas, int64_t u) {
+  const int64_t base = units / ctas, more = units % ctas;
+  return static_cast<int>(u < more * (base + 1) ? u / (base + 1) : more + (u - more * (base + 1)) / base);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 8 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movm_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Codes i and i + 4 of a word (or i of two words' halves) as the bf16 pair 128 + code.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
+  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+}
+// 128 + code -> code - 8, exact in bf16.
+__device__ __forceinline__ uint32_t centre_pair(uint32_t p) {
+  __nv_bfloat162 x = *reinterpret_cast<__nv_bfloat162 *>(&p);
+  const uint32_t k = 0xc308c308u;  // -136, -136
+  x = __hadd2(x, *reinterpret_cast<const __nv_bfloat162 *>(&k));
+  return *reinterpret_cast<uint32_t *>(&x);
+}
+
+template <int D, int NT>
+struct Dec4 {
+  static constexpr int ROW = D / 2;                        // bytes of a row's codes
+  static constexpr int CHUNKS = ROW / 16;                  // 16-byte pieces of a row
+  static constexpr int STAGE = kD4Tile * (2 * ROW + 8);    // K, V, parameters
+  static constexpr int RING = kD4Stages * STAGE;
+  static constexpr int STATE = NT * (4 * (D / 16) + 4) * 32 * 4;  // one warp's softmax state
+  static constexpr int SMEM = kD4Warps * RING + 3 * STATE;
+};
+
+// Where row `r` of a V stage lies: the lanes of one shared-memory phase read rows 2t of four
+// consecutive t, and this order of rows (for D = 128 with the row's 16-byte pieces exchanged
+// in every second group of four) puts them into different banks.
+template <int D>
+__device__ __forceinline__ int v_place(int r) {
+  return D == 128 ? (r & ~3) | ((r & 1) << 1) | ((r >> 1) & 1) : (r & ~7) | ((r & 1) << 2) | ((r >> 1) & 3);
+}
+template <int D>
+__device__ __forceinline__ int v_swap(int r) {
+  return D == 128 ? ((r >> 2) & 1) << 1 : 0;
+}
+
+// A position in the flattened (sequence, pair, round) list.
+struct Cursor4 {
+  int b, p, r, rounds, len;
+  __device__ __forceinline__ void load(const Decode4Args &a) {
+    len = decode4_len(a, b);
+    rounds = rounds_of(len);
+  }
+  __device__ __forceinline__ void next(const Decode4Args &a, int pairs) {
+    if (++r < rounds) return;
+    r = 0;
+    if (++p < pairs) return;
+    p = 0;
+    do {
+      ++b;
+      if (b >= a.batch) return;
+      load(a);
+    } while (rounds == 0);
+  }
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
+    paged_decode4_kernel(const Decode4Args a) {
+  using C = Dec4<D, NT>;
+  constexpr int KS = D / 16;        // k-steps of a score, and 16-dim row tiles of the output
+  constexpr int KW = D / 32;        // code words a lane reads of a K row
+  constexpr int VW = D / 64;        // code words a lane reads of a V row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t *ring = smem + warp * C::RING;
+  float *state = reinterpret_cast<float *>(smem + kD4Warps * C::RING);
+  const uint32_t ring_s = smem_addr(ring);
+  const int pairs = a.c.num_kv_heads * a.subs;
+
+  pdl_trigger();
+  pdl_wait();
+
+  // rows without a key
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b] > static_cast<int64_t>(a.bt_width) * a.c.block_size &&
+        tid == 0)
+      raise_flag(a.error_flag, B200ASR_DEVERR_LENGTH);
+    if (decode4_len(a, b) == 0)
+      for (int i = tid; i < a.c.num_kv_heads * a.group * D; i += blockDim.x)
+        a.out[b * a.out_row + i / D * a.out_head + i % D] = f2bf(0.f);
+  }
+
+  // this CTA's units, and where they begin
+  int64_t u0, u1;
+  Cursor4 ld;
+  if (a.whole) {
+    ld.b = blockIdx.x / pairs;
+    ld.p = blockIdx.x - ld.b * pairs;
+    ld.r = 0;
+    ld.load(a);
+    u0 = 0;
+    u1 = ld.rounds;
+  } else {
+    int64_t unused;
+    const int64_t units = decode4_rounds(a, pairs, 0, unused);
+    u0 = first_unit(units, gridDim.x, blockIdx.x);
+    u1 = first_unit(units, gridDim.x, blockIdx.x + 1);
+    if (u0 < u1) {  // find the sequence: a warp scan, the same in every warp
+      int64_t carry = 0;
+      for (int base = 0;; base += 32) {
+        const int b = base + lane;
+        const int n = b < a.batch ? rounds_of(decode4_len(a, b)) * pairs : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, u0 < carry + incl);
+        if (here) {
+          const int src = __ffs(here) - 1;
+          const int64_t begin = carry + __shfl_sync(0xffffffffu, incl - n, src);
+          ld.b = base + src;
+          ld.load(a);
+          const int64_t off = u0 - begin;
+          ld.p = static_cast<int>(off / ld.rounds);
+          ld.r = static_cast<int>(off - static_cast<int64_t>(ld.p) * ld.rounds);
+          break;
+        }
+        carry += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+  }
+  if (u0 >= u1) return;
+  const int total = static_cast<int>(u1 - u0);
+  Cursor4 cur = ld;
+
+  // ------------------------------------------------------------------ loads of a stage
+  auto token_of = [&](const Cursor4 &c) { return c.r * kD4Round + warp * kD4Tile + lane; };
+  // the block of this lane's token (its table entry is read one stage ahead of its use)
+  auto block_of = [&](const Cursor4 &c) -> int {
+    const int tok = token_of(c);
+    if (tok >= c.len) return 0;
+    const int j = a.bs_shift >= 0 ? tok >> a.bs_shift : tok / a.c.block_size;
+    return a.block_tables[c.b * a.bt_stride + j];
+  };
+  auto issue = [&](const Cursor4 &c, int block, int stage) {
+    const int tok = token_of(c);
+    const int valid = tok < c.len;
+    const int at = a.bs_shift >= 0 ? tok & (a.c.block_size - 1) : tok % a.c.block_size;
+    if (valid && (block < 0 || block >= a.c.num_blocks)) {
+      raise_flag(a.error_flag, B200ASR_DEVERR_BLOCK);
+      block = 0;
+    }
+    if (!valid) block = 0;
+    const int h = c.p / a.subs;
+    const int64_t off = block * a.c.code_stride[0] + (valid ? at : 0) * a.c.code_stride[1] +
+                        h * a.c.code_stride[2];
+    const int64_t poff = block * a.c.param_stride[0] + (valid ? at : 0) * a.c.param_stride[1] +
+                         h * a.c.param_stride[2];
+    const uint32_t ks = ring_s + stage * C::STAGE, vs = ks + kD4Tile * C::ROW, ps = vs + kD4Tile * C::ROW;
+    cp_async8(ps + lane * 8, static_cast<const __nv_bfloat16 *>(a.c.params) + poff, valid);
+#pragma unroll
+    for (int i = 0; i < C::CHUNKS; ++i) {
+      const int id = i * 32 + lane, row = id / C::CHUNKS, ch = id % C::CHUNKS;
+      const int64_t o = __shfl_sync(0xffffffffu, off, row) + ch * 16;
+      const bool ok = __shfl_sync(0xffffffffu, valid, row) != 0;
+      cp_async16(ks + row * C::ROW + ch * 16, static_cast<const uint8_t *>(a.c.k_codes) + o, ok);
+      cp_async16(vs + v_place<D>(row) * C::ROW + (ch ^ v_swap<D>(row)) * 16,
+                 static_cast<const uint8_t *>(a.c.v_codes) + o, ok);
+    }
+  };
+
+  int issued = 0, next_block = block_of(ld);
+  auto issue_next = [&]() {
+    if (issued < total) {
+      const Cursor4 c = ld;
+      const int block = next_block;
+      if (++issued < total) {
+        ld.next(a, pairs);
+        next_block = block_of(ld);
+      }
+      issue(c, block, (issued - 1) % kD4Stages);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kD4Stages - 1; ++s) issue_next();
+
+  // ------------------------------------------------------------------ segments
+  int done = 0;
+  while (done < total) {
+    const int b = cur.b, p = cur.p, r_first = cur.r;
+    const int r_last = min(cur.rounds, cur.r + (total - done));  // one past
+    const int h = p / a.subs, col0 = (p - h * a.subs) * 8 * NT;
+    const int cols = min(8 * NT, a.group - col0);
+    const __nv_bfloat16 *qp = a.q + b * a.q_row + (static_cast<int64_t>(h) * a.group + col0) * a.q_head;
+    // q as the MMA's column operand, in the lane order of the codes: word j of a lane holds
+    // dims 32 t + 8 j (D = 128) or 16 t + 8 j (D = 64) and up
+    uint32_t qf[NT][KS][2];
+    float qs0[NT], qs1[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (n * 8 + g < cols)
+          u = *reinterpret_cast<const uint4 *>(qp + (n * 8 + g) * a.q_head + t * (D / 4) + j * 8);
+        float f[8];
+        unpack8(u, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += f[e];
+        qf[n][2 * j][0] = __byte_perm(u.x, u.z, 0x5410);
+        qf[n][2 * j][1] = __byte_perm(u.x, u.z, 0x7632);
+        qf[n][2 * j + 1][0] = __byte_perm(u.y, u.w, 0x5410);
+        qf[n][2 * j + 1][1] = __byte_perm(u.y, u.w, 0x7632);
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      qs0[n] = __shfl_sync(0xffffffffu, sum, 8 * t);      // column 2t: lanes with g = 2t
+      qs1[n] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);  // column 2t + 1
+    }
+    float o[NT][KS][4], m0[NT], m1[NT], l0[NT], l1[NT], z0[NT], z1[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m0[n] = m1[n] = -INFINITY;
+      l0[n] = l1[n] = z0[n] = z1[n] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KS; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][j][e] = 0.f;
+    }
+
+    for (int r = r_first; r < r_last; ++r, ++done) {
+      cp_wait<kD4Stages - 2>();
+      __syncwarp();
+      const int stage = done % kD4Stages;
+      const uint8_t *kst = ring + stage * C::STAGE, *vst = kst + kD4Tile * C::ROW;
+      const uint8_t *pst = vst + kD4Tile * C::ROW;
+      const int left = cur.len - (r * kD4Round + warp * kD4Tile);  // tokens of this stage and on
+      float s[NT][2][4];
+      uint32_t vpar[2][2];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const uint2 pa = *reinterpret_cast<const uint2 *>(pst + (mt * 16 + g) * 8);
+        const uint2 pb = *reinterpret_cast<const uint2 *>(pst + (mt * 16 + g + 8) * 8);
+        vpar[mt][0] = pa.y;
+        vpar[mt][1] = pb.y;
+        uint32_t ka[KW], kb[KW];
+        const uint8_t *ra = kst + (mt * 16 + g) * C::ROW + t * (C::ROW / 4), *rb = ra + 8 * C::ROW;
+        if constexpr (KW == 4) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(ra), y = *reinterpret_cast<const uint4 *>(rb);
+          ka[0] = x.x; ka[1] = x.y; ka[2] = x.z; ka[3] = x.w;
+          kb[0] = y.x; kb[1] = y.y; kb[2] = y.z; kb[3] = y.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2 *>(ra), y = *reinterpret_cast<const uint2 *>(rb);
+          ka[0] = x.x; ka[1] = x.y;
+          kb[0] = y.x; kb[1] = y.y;
+        }
+        float acc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][0] = acc[n][2] = -128.f * qs0[n];
+          acc[n][1] = acc[n][3] = -128.f * qs1[n];
+        }
+#pragma unroll
+        for (int j = 0; j < KW; ++j)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t a0 = code_pair(ka[j], 2 * half), a2 = code_pair(ka[j], 2 * half + 1);
+            const uint32_t a1 = code_pair(kb[j], 2 * half), a3 = code_pair(kb[j], 2 * half + 1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma_bf16(acc[n], a0, a1, a2, a3, qf[n][2 * j + half][0], qf[n][2 * j + half][1]);
+          }
+        const float2 kpa = unpack2(pa.x), kpb = unpack2(pb.x);
+        const float sa = kpa.x * a.scale_log2, za = kpa.y * a.scale_log2;
+        const float sb = kpb.x * a.scale_log2, zb = kpb.y * a.scale_log2;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          s[n][mt][0] = fmaf(sa, acc[n][0], za * qs0[n]);
+          s[n][mt][1] = fmaf(sa, acc[n][1], za * qs1[n]);
+          s[n][mt][2] = fmaf(sb, acc[n][2], zb * qs0[n]);
+          s[n][mt][3] = fmaf(sb, acc[n][3], zb * qs1[n]);
+        }
+      }
+      if (left < kD4Tile) {  // the sequence ends in this stage
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (mt * 16 + g >= left) s[n][mt][0] = s[n][mt][1] = -INFINITY;
+            if (mt * 16 + g + 8 >= left) s[n][mt][2] = s[n][mt][3] = -INFINITY;
+          }
+      }
+      bool move = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float x0 = fmaxf(fmaxf(s[n][0][0], s[n][0][2]), fmaxf(s[n][1][0], s[n][1][2]));
+        const float x1 = fmaxf(fmaxf(s[n][0][1], s[n][0][3]), fmaxf(s[n][1][1], s[n][1][3]));
+        move = move || x0 > m0[n] + kD4Lazy || x1 > m1[n] + kD4Lazy;
+      }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float x0 = fmaxf(fmaxf(s[n][0][0], s[n][0][2]), fmaxf(s[n][1][0], s[n][1][2]));
+          float x1 = fmaxf(fmaxf(s[n][0][1], s[n][0][3]), fmaxf(s[n][1][1], s[n][1][3]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+          }
+          x0 = fmaxf(x0, m0[n]);
+          x1 = fmaxf(x1, m1[n]);
+          const float f0 = x0 == -INFINITY ? 1.f : exp2f(m0[n] - x0);
+          const float f1 = x1 == -INFINITY ? 1.f : exp2f(m1[n] - x1);
+          m0[n] = x0;
+          m1[n] = x1;
+          l0[n] *= f0;
+          z0[n] *= f0;
+          l1[n] *= f1;
+          z1[n] *= f1;
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
+            o[n][j][0] *= f0;
+            o[n][j][2] *= f0;
+            o[n][j][1] *= f1;
+            o[n][j][3] *= f1;
+          }
+        }
+      }
+      uint32_t pf[NT][2][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        // a column without a key so far keeps p = 0 (its scores are -inf)
+        const float r0 = m0[n] == -INFINITY ? 0.f : m0[n], r1 = m1[n] == -INFINITY ? 0.f : m1[n];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const float2 va = unpack2(vpar[mt][0]), vb = unpack2(vpar[mt][1]);
+          const float ca = fmaf(8.f, va.x, va.y), cb = fmaf(8.f, vb.x, vb.y);  // zero of code - 8
+          const float p0 = exp2f(s[n][mt][0] - r0), p1 = exp2f(s[n][mt][1] - r1);
+          const float p2 = exp2f(s[n][mt][2] - r0), p3 = exp2f(s[n][mt][3] - r1);
+          l0[n] += p0 + p2;
+          l1[n] += p1 + p3;
+          z0[n] = fmaf(p0, ca, fmaf(p2, cb, z0[n]));
+          z1[n] = fmaf(p1, ca, fmaf(p3, cb, z1[n]));
+          pf[n][mt][0] = movm_trans(pack2(p0 * va.x, p1 * va.x));
+          pf[n][mt][1] = movm_trans(pack2(p2 * vb.x, p3 * vb.x));
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        // this lane's codes (dims of g) of tokens 2t, 2t + 1, 2t + 8, 2t + 9
+        uint32_t w[4][VW];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = mt * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (VW == 2) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(
+                vst + v_place<D>(row) * C::ROW + (((g >> 1) ^ v_swap<D>(row)) << 4) + (g & 1) * 8);
+            w[i][0] = x.x;
+            w[i][1] = x.y;
+          } else {
+            w[i][0] = *reinterpret_cast<const uint32_t *>(vst + v_place<D>(row) * C::ROW + g * 4);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VW; ++j)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7632 : 0x5410;
+            const uint32_t x = __byte_perm(w[0][j], w[1][j], sel);  // tokens 2t, 2t + 1
+            const uint32_t y = __byte_perm(w[2][j], w[3][j], sel);  // tokens 2t + 8, 2t + 9
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const uint32_t a0 = centre_pair(code_pair(x, i)), a1 = centre_pair(code_pair(x, i + 1));
+              const uint32_t a2 = centre_pair(code_pair(y, i)), a3 = centre_pair(code_pair(y, i + 1));
+              // output rows of this tile: dims (D / 8) g + e and e + 1, e = 8 j + 4 half + i
+              const int tile = 4 * j + 2 * half + i / 2;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_bf16(o[n][tile], a0, a1, a2, a3, pf[n][mt][0], pf[n][mt][1]);
+            }
+          }
+      }
+      __syncwarp();  // the stage's last reads are done: its slot may be refilled
+      issue_next();
+    }
+
+    // -------------------------------------------------------- end of the segment
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l0[n] += __shfl_xor_sync(0xffffffffu, l0[n], d);
+        l1[n] += __shfl_xor_sync(0xffffffffu, l1[n], d);
+        z0[n] += __shfl_xor_sync(0xffffffffu, z0[n], d);
+        z1[n] += __shfl_xor_sync(0xffffffffu, z1[n], d);
+      }
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        o[n][j][0] += z0[n];
+        o[n][j][2] += z0[n];
+        o[n][j][1] += z1[n];
+        o[n][j][3] += z1[n];
+      }
+    }
+    // the four warps' states: 2 and 3 into 0 and 1, then 1 into 0
+    auto put = [&](float *to) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float *q = to + n * (4 * KS + 4) * 32 + lane;
+        q[0] = m0[n];
+        q[32] = m1[n];
+        q[64] = l0[n];
+        q[96] = l1[n];
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[(4 + 4 * j + e) * 32] = o[n][j][e];
+      }
+    };
+    auto join = [&](const float *from) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float *q = from + n * (4 * KS + 4) * 32 + lane;
+        const float x0 = fmaxf(m0[n], q[0]), x1 = fmaxf(m1[n], q[32]);
+        const float u0f = m0[n] == -INFINITY && x0 == -INFINITY ? 1.f : exp2f(m0[n] - x0);
+        const float u1f = m1[n] == -INFINITY && x1 == -INFINITY ? 1.f : exp2f(m1[n] - x1);
+        const float w0 = q[0] == -INFINITY && x0 == -INFINITY ? 1.f : exp2f(q[0] - x0);
+        const float w1 = q[32] == -INFINITY && x1 == -INFINITY ? 1.f : exp2f(q[32] - x1);
+        m0[n] = x0;
+        m1[n] = x1;
+        l0[n] = l0[n] * u0f + q[64] * w0;
+        l1[n] = l1[n] * u1f + q[96] * w1;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          o[n][j][0] = o[n][j][0] * u0f + q[(4 + 4 * j) * 32] * w0;
+          o[n][j][1] = o[n][j][1] * u1f + q[(5 + 4 * j) * 32] * w1;
+          o[n][j][2] = o[n][j][2] * u0f + q[(6 + 4 * j) * 32] * w0;
+          o[n][j][3] = o[n][j][3] * u1f + q[(7 + 4 * j) * 32] * w1;
+        }
+      }
+    };
+    constexpr int SF = C::STATE / 4;
+    if (warp >= 2) put(state + (warp - 2) * SF);
+    __syncthreads();
+    if (warp < 2) join(state + warp * SF);
+    if (warp == 1) put(state + 2 * SF);
+    __syncthreads();
+    if (warp == 0) {
+      join(state + 2 * SF);
+      const bool full = r_first == 0 && r_last == cur.rounds;
+      const int slot = 2 * blockIdx.x + (r_first > 0 ? 0 : 1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = n * 8 + 2 * t + e;
+          if (col >= cols) continue;
+          const float l = e ? l1[n] : l0[n];
+          if (full) {
+            const float inv = 1.f / l;
+            __nv_bfloat16 *dst = a.out + b * a.out_row +
+                                 (static_cast<int64_t>(h) * a.group + col0 + col) * a.out_head + g * (D / 8);
+#pragma unroll
+            for (int j = 0; j < KS; j += 4)
+              *reinterpret_cast<uint4 *>(dst + 2 * j) =
+                  make_uint4(pack2(o[n][j][e] * inv, o[n][j][e + 2] * inv),
+                             pack2(o[n][j + 1][e] * inv, o[n][j + 1][e + 2] * inv),
+                             pack2(o[n][j + 2][e] * inv, o[n][j + 2][e + 2] * inv),
+                             pack2(o[n][j + 3][e] * inv, o[n][j + 3][e + 2] * inv));
+          } else {
+            float *w = a.ws + (static_cast<int64_t>(slot) * 8 * NT + col) * (D + 4);
+            if (g == 0) {
+              w[0] = e ? m1[n] : m0[n];
+              w[1] = l;
+            }
+#pragma unroll
+            for (int j = 0; j < KS; j += 2)
+              *reinterpret_cast<float4 *>(w + 4 + g * (D / 8) + 2 * j) =
+                  make_float4(o[n][j][e], o[n][j][e + 2], o[n][j + 1][e], o[n][j + 1][e + 2]);
+          }
+        }
+    }
+    // the compute cursor follows the rounds just done
+    cur.r = r_last - 1;
+    cur.next(a, pairs);
+  }
+  cp_wait<0>();
+}
+
+// Joins the partials of the pairs that several CTAs shared: one CTA per (sequence, pair).
+template <int D, int NT>
+__global__ void __launch_bounds__(kD4Warps * 32) paged_decode4_join_kernel(const Decode4Args a, int ctas) {
+  pdl_trigger();
+  pdl_wait();
+  const int pairs = a.c.num_kv_heads * a.subs;
+  const int b = blockIdx.x / pairs, p = blockIdx.x - b * pairs;
+  const int rounds = rounds_of(decode4_len(a, b));
+  int64_t first;
+  const int64_t units = decode4_rounds(a, pairs, b, first);
+  if (rounds == 0) return;
+  first += static_cast<int64_t>(p) * rounds;
+  const int c0 = cta_of_unit(units, ctas, first), c1 = cta_of_unit(units, ctas, first + rounds - 1);
+  if (c0 == c1) return;
+  const int h = p / a.subs, col0 = (p - h * a.subs) * 8 * NT;
+  const int cols = min(8 * NT, a.group - col0);
+  for (int i = threadIdx.x; i < cols * D; i += blockDim.x) {
+    const int col = i / D, d = i - col * D;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+      // a CTA's share begins inside the pair (slot 0) unless it holds the pair's first round
+      const float *w = a.ws + (static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * 8 * NT + col) * (D + 4);
+      const float wm = w[0], x = fmaxf(m, wm);
+      const float fo = m == -INFINITY ? 0.f : exp2f(m - x);
+      const float fw = wm == -INFINITY && x == -INFINITY ? 1.f : exp2f(wm - x);
+      l = l * fo + w[1] * fw;
+      o = o * fo + w[4 + d] * fw;
+      m = x;
+    }
+    a.out[b * a.out_row + (static_cast<int64_t>(h) * a.group + col0 + col) * a.out_head + d] = f2bf(o / l);
+  }
+}
+
+constexpr int kD4WholeMax = 512;  // longest context whose pairs are not split
+
+template <int D, int NT>
+int launch_decode4(Decode4Args a, int max_seqlen_k, size_t ws_bytes, cudaStream_t stream) {
+  using C = Dec4<D, NT>;
+  a.subs = (a.group + 8 * NT - 1) / (8 * NT);
+  const int64_t pairs = static_cast<int64_t>(a.c.num_kv_heads) * a.subs * a.batch;
+  const int64_t most = pairs * ((max_seqlen_k + kD4Round - 1) / kD4Round);
+  const int per_sm = NT == 1 ? kD4CtasPerSm : 2;
+  a.whole = max_seqlen_k <= kD4WholeMax;
+  const int64_t grid = a.whole ? pairs : std::min<int64_t>(std::max<int64_t>(most, 1), per_sm * num_sms());
+  B200_REQUIRE(grid <= 0x7fffffff && pairs <= 0x7fffffff, "paged_decode4: too many rows");
+  if (!a.whole) {
+    const size_t need = static_cast<size_t>(per_sm) * num_sms() * 2 * 8 * NT * (D + 4) * 4;
+    if (a.ws == nullptr || ws_bytes < need) {
+      set_error("paged_decode4: workspace of %zu bytes, %zu needed", ws_bytes, need);
+      return B200ASR_ERR_WORKSPACE;
+    }
+  }
+  auto kfn = paged_decode4_kernel<D, NT>;
+  const cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  B200_LAUNCH_CHECK_ERR(e, "paged_decode4 (configuration)");
+  B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(static_cast<unsigned>(grid)), dim3(kD4Warps * 32),
+                                      C::SMEM, stream, true, 1, a),
+                        "paged_decode4");
+  if (!a.whole)
+    B200_LAUNCH_CHECK_ERR(launch_kernel(paged_decode4_join_kernel<D, NT>, dim3(static_cast<unsigned>(pairs)),
+                                        dim3(kD4Warps * 32), 0, stream, true, 1, a, static_cast<int>(grid)),
+                          "paged_decode4 (join)");
+  return B200ASR_OK;
+}
+
+}  // namespace b200asr
+
+using namespace b200asr;
+
+extern "C" size_t b200asr_paged_decode4_workspace_size(int32_t max_seqlen_k, int32_t num_heads,
+                                                       int32_t num_kv_heads, int32_t head_dim) {
+  if (max_seqlen_k <= kD4WholeMax || num_heads < 1 || num_kv_heads < 1 || head_dim < 1) return 0;
+  const int nt = num_heads / num_kv_heads > 8 ? 2 : 1;
+  const int per_sm = nt == 1 ? kD4CtasPerSm : 2;
+  return static_cast<size_t>(per_sm) * num_sms() * 2 * 8 * nt * (head_dim + 4) * 4;
+}
+
+extern "C" int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
+                                     const b200asr_kv4 *cache, int32_t num_heads,
+                                     const int32_t *cu_seqlens_k, const int32_t *block_tables,
+                                     int64_t bt_stride, int32_t bt_width, int32_t batch,
+                                     int32_t max_seqlen_k, float scale, void *out,
+                                     int64_t out_row_stride, int64_t out_head_stride,
+                                     void *workspace, size_t workspace_bytes, int32_t *error_flag,
+                                     b200asr_stream_t stream) {
+  B200_REQUIRE(cache != nullptr, "paged_decode4: null cache");
+  const int D = cache->head_dim;
+  B200_REQUIRE(D == 64 || D == 128, "paged_decode4: head_dim %d unsupported (64 or 128)", D);
+  B200_REQUIRE(batch >= 0 && num_heads >= 1 && max_seqlen_k >= 0 && bt_width >= 0,
+               "paged_decode4: bad sizes");
+  B200_REQUIRE(cache->num_kv_heads >= 1 && num_heads % cache->num_kv_heads == 0,
+               "paged_decode4: num_heads %d not a multiple of num_kv_heads %d", num_heads,
+               cache->num_kv_heads);
+  if (batch == 0) return B200ASR_OK;
+  B200_REQUIRE(q && out && cu_seqlens_k && (block_tables || bt_width == 0) && cache->k_codes &&
+                   cache->v_codes && cache->params,
+               "paged_decode4: null pointer");
+  B200_REQUIRE(kv4_cache_ok(*cache), "paged_decode4: cache sizes, or rows not 16-byte (codes) and "
+               "8-byte (parameters) aligned");
+  B200_REQUIRE(aligned16(q) && aligned16(out) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0 &&
+                   out_row_stride % 8 == 0 && out_head_stride % 8 == 0,
+               "paged_decode4: q and out rows must be 16-byte aligned");
+  B200_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "paged_decode4: workspace alignment");
+  Decode4Args a{};
+  a.q = static_cast<const __nv_bfloat16 *>(q);
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.c = *cache;
+  a.cu_seqlens_k = cu_seqlens_k;
+  a.block_tables = block_tables;
+  a.bt_stride = bt_stride;
+  a.bt_width = bt_width;
+  a.batch = batch;
+  a.group = num_heads / cache->num_kv_heads;
+  const int bs = cache->block_size;
+  a.bs_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<__nv_bfloat16 *>(out);
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  a.ws = static_cast<float *>(workspace);
+  a.error_flag = error_flag;
+  // Up to 8 query heads of a KV head are one column tile; more take two per pass over the cache.
+  auto fn = D == 128 ? (a.group <= 8 ? launch_decode4<128, 1> : launch_decode4<128, 2>)
+                     : (a.group <= 8 ? launch_decode4<64, 1> : launch_decode4<64, 2>);
+  return fn(a, max_seqlen_k, workspace_bytes, stream);
+}

@@ -12,7 +12,7 @@ import ctypes
 
 import torch
 
-from voiceagent_b200._lib import check, lib
+from voiceagent_b200._lib import Kv4, check, lib
 
 BF16 = torch.bfloat16
 
@@ -351,6 +351,138 @@ def varlen_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=Non
         _p(q), q.stride(0), _p(k), k.stride(0), _p(v), v.stride(0), _p(cu_seqlens),
         cu_seqlens.numel() - 1, total, int(max_seqlen), num_heads, head_dim, float(scale), _p(out),
         out.stride(0), _p(error_flag), _stream()), "varlen_attention")
+    return out
+
+
+# ------------------------------------------------------------ 4-bit paged KV cache
+# A cached head row is head_dim / 2 bytes of codes plus a bf16 scale and zero (value = zero +
+# code * scale), a quarter of the bf16 cache's bytes. No reference counterpart: the reference
+# caches bf16 (engine/model_runner.py:116-131). The calls mirror the bf16 cache's.
+
+
+def kv4_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, device="cuda"):
+    """A zeroed 4-bit cache of one layer: ``(k_codes, v_codes, kv_params)``, uint8
+    ``[num_blocks, block_size, num_kv_heads, head_dim / 2]`` twice and bf16 ``[..., 4]``
+    (K scale, K zero, V scale, V zero)."""
+    _need(head_dim in (64, 128), "kv4_cache: head_dim 64 or 128")
+    shape = (num_blocks, block_size, num_kv_heads)
+    return (torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device),
+            torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device),
+            torch.zeros(*shape, 4, dtype=BF16, device=device))
+
+
+def _here(what: str, *tensors: torch.Tensor | None) -> None:
+    """Every tensor on the current CUDA device: the launch goes to that device's stream."""
+    here = None
+    for t in tensors:
+        if t is None:
+            continue
+        _need(t.is_cuda, f"{what}: b200asr kernels need CUDA tensors")
+        if here is None:
+            here = torch.cuda.current_device()
+        _need(t.get_device() == here, f"{what}: tensors on another device than the current one")
+
+
+def _kv4(what: str, k_codes, v_codes, kv_params) -> Kv4:
+    """The cache as the C ABI takes it (strides of the first three axes are free)."""
+    _need(k_codes.dtype == torch.uint8 and v_codes.dtype == torch.uint8
+          and kv_params.dtype == BF16, f"{what}: uint8 codes and bf16 parameters")
+    _need(k_codes.dim() == 4 and k_codes.shape == v_codes.shape
+          and k_codes.stride() == v_codes.stride() and k_codes.stride(3) == 1,
+          f"{what}: codes [num_blocks, block_size, num_kv_heads, head_dim / 2], alike for K and V")
+    blocks, size, heads, row = k_codes.shape
+    _need(tuple(kv_params.shape) == (blocks, size, heads, 4) and kv_params.stride(3) == 1,
+          f"{what}: parameters [num_blocks, block_size, num_kv_heads, 4]")
+    _here(what, k_codes, v_codes, kv_params)
+    cs, ps = k_codes.stride(), kv_params.stride()
+    return Kv4(k_codes.data_ptr(), v_codes.data_ptr(), kv_params.data_ptr(), cs[:3], ps[:3], blocks,
+               size, heads, 2 * row)
+
+
+def store_kvcache4(key, value, k_codes, v_codes, kv_params, slot_mapping, error_flag=None) -> None:
+    """:func:`store_kvcache` into a 4-bit cache: key/value bf16 [T, H_kv, D] (free token and
+    head strides), slot_mapping int32 [T], -1 skips; no slot twice."""
+    what = "store_kvcache4"
+    cache = _kv4(what, k_codes, v_codes, kv_params)
+    _need(key.dtype == BF16 and value.dtype == BF16 and key.dim() == 3
+          and key.shape[1:] == (cache.num_kv_heads, cache.head_dim) and value.shape == key.shape
+          and key.stride(2) == 1 and value.stride(2) == 1,
+          f"{what}: key/value bf16 [T, num_kv_heads, head_dim] with contiguous rows")
+    _need(slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous()
+          and slot_mapping.shape == key.shape[:1], f"{what}: int32 slots, one per token")
+    _here(what, key, value, slot_mapping, error_flag)
+    _count()
+    check(lib.b200asr_store_kvcache4(
+        _p(key), key.stride(0), key.stride(1), _p(value), value.stride(0), value.stride(1),
+        ctypes.byref(cache), _p(slot_mapping), key.shape[0], _p(error_flag), _stream()), what)
+
+
+def load_kvcache4(k_codes, v_codes, kv_params, slots, key=None, value=None, error_flag=None):
+    """Rows of a 4-bit cache as bf16 ``(key, value)`` [T, H_kv, D]; slot -1 reads as zeros."""
+    what = "load_kvcache4"
+    cache = _kv4(what, k_codes, v_codes, kv_params)
+    _need(slots.dtype == torch.int32 and slots.dim() == 1 and slots.is_contiguous(),
+          f"{what}: int32 slots [T]")
+    shape = (slots.shape[0], cache.num_kv_heads, cache.head_dim)
+    key = torch.empty(shape, dtype=BF16, device=slots.device) if key is None else key
+    value = torch.empty(shape, dtype=BF16, device=slots.device) if value is None else value
+    for x in (key, value):
+        _need(x.dtype == BF16 and tuple(x.shape) == shape and x.stride(2) == 1,
+              f"{what}: key/value bf16 [T, num_kv_heads, head_dim] with contiguous rows")
+    _here(what, slots, key, value, error_flag)
+    _count()
+    check(lib.b200asr_load_kvcache4(
+        ctypes.byref(cache), _p(slots), shape[0], _p(key), key.stride(0), key.stride(1), _p(value),
+        value.stride(0), value.stride(1), _p(error_flag), _stream()), what)
+    return key, value
+
+
+def _attention4_args(what: str, q, out, cu_seqlens_k, block_tables, cache: Kv4) -> None:
+    _need(q.dtype == BF16 and q.dim() == 3 and q.shape[2] == cache.head_dim and q.stride(2) == 1
+          and q.shape[1] % cache.num_kv_heads == 0,
+          f"{what}: q bf16 [rows, num_heads, head_dim] with contiguous rows, num_heads a multiple "
+          "of num_kv_heads")
+    _need(out.dtype == BF16 and out.shape == q.shape and out.stride(2) == 1,
+          f"{what}: out like q")
+    _need(block_tables.dtype == torch.int32 and cu_seqlens_k.dtype == torch.int32,
+          f"{what}: int32 metadata")
+    _need(cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous() and cu_seqlens_k.shape[0] >= 1,
+          f"{what}: cu_seqlens_k [batch + 1]")
+    _need(block_tables.dim() == 2 and block_tables.shape[0] >= cu_seqlens_k.shape[0] - 1
+          and (block_tables.stride(1) == 1 or block_tables.shape[1] <= 1),
+          f"{what}: block_tables [batch, blocks] with contiguous rows")
+
+
+def paged_decode4_workspace_size(max_seqlen_k: int, num_heads: int, num_kv_heads: int,
+                                 head_dim: int = 128) -> int:
+    return int(lib.b200asr_paged_decode4_workspace_size(max_seqlen_k, num_heads, num_kv_heads,
+                                                        head_dim))
+
+
+def paged_decode4(q, k_codes, v_codes, kv_params, cu_seqlens_k, block_tables, *,
+                  max_seqlen_k: int, scale: float, out, workspace=None,
+                  error_flag=None) -> torch.Tensor:
+    """:func:`paged_decode` over a 4-bit cache. q/out [>= B, H, D], H any multiple of H_kv,
+    D 64 or 128; a row without a cached token gives zeros, rows past B are left alone.
+    ``workspace`` (uint8, :func:`paged_decode4_workspace_size` bytes, any contents, one call at
+    a time) is taken from the caching allocator when not given."""
+    what = "paged_decode4"
+    cache = _kv4(what, k_codes, v_codes, kv_params)
+    _attention4_args(what, q, out, cu_seqlens_k, block_tables, cache)
+    batch = cu_seqlens_k.shape[0] - 1
+    _need(batch <= q.shape[0], f"{what}: cu_seqlens_k longer than the batch")
+    if workspace is None:
+        need = paged_decode4_workspace_size(max_seqlen_k, q.shape[1], cache.num_kv_heads,
+                                            cache.head_dim)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _here(what, q, out, cu_seqlens_k, block_tables, workspace, error_flag)
+    _count(1 if max_seqlen_k <= DECODE_SHORT_CTX else 2)  # + the join of split contexts
+    check(lib.b200asr_paged_decode4(
+        _p(q), q.stride(0), q.stride(1), ctypes.byref(cache), q.shape[1], _p(cu_seqlens_k),
+        _p(block_tables), block_tables.stride(0), block_tables.shape[1], batch, max_seqlen_k,
+        float(scale), _p(out), out.stride(0), out.stride(1), _p(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _p(error_flag),
+        _stream()), what)
     return out
 
 

@@ -515,6 +515,24 @@ B200ASR_API int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64
                                       void *workspace, size_t workspace_bytes,
                                       int32_t *error_flag, b200asr_stream_t stream);
 
+/* ------------------------------------------- rotary positions with several axes ----
+ * qk_norm_rope_store (models/qwen3.py:43-48) for positions int64 [axes, num_tokens] (row
+ * stride position_stride): frequency j of the head_dim / 2 turns by the position of axis
+ * freq_axis[j] (the upstream model's time / height / width rows and their sections). qkv
+ * bf16 rows hold num_heads query, num_kv_heads key and num_kv_heads value heads; q_out bf16
+ * [num_tokens, num_heads, head_dim]. Everything is computed in 32 bits and rounded to bf16
+ * once. With slot_mapping (-1 skips), K and V go to a contiguous bf16 cache (k_cache,
+ * v_cache, num_slots; cache4 NULL) or, quantised from the bf16 K and V, to a 4-bit one
+ * (cache4; k_cache and v_cache NULL). A position or an axis out of range reads as position
+ * 0 (B200ASR_DEVERR_POSITION). */
+B200ASR_API int b200asr_qk_norm_mrope_store(
+    const void *qkv, int64_t qkv_row_stride, const int64_t *positions, int64_t position_stride,
+    int32_t axes, const int32_t *freq_axis, int32_t num_tokens, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, const void *q_norm_weight, const void *k_norm_weight,
+    float eps, const float *cos_sin_cache, int32_t max_position, void *q_out,
+    int64_t q_out_row_stride, const int32_t *slot_mapping, void *k_cache, void *v_cache,
+    int64_t num_slots, const b200asr_kv4 *cache4, int32_t *error_flag, b200asr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -95,6 +95,9 @@ SIGNATURES: dict[str, tuple] = {
     "b200asr_paged_decode4": (c_int32, [P, c_int64, c_int64, P, c_int32, P, P, c_int64, c_int32,
                                         c_int32, c_int32, c_float, P, c_int64, c_int64, P,
                                         c_size_t, P, P]),
+    "b200asr_qk_norm_mrope_store": (c_int32, [P, c_int64, P, c_int64, c_int32, P, c_int32, c_int32,
+                                              c_int32, c_int32, P, P, c_float, P, c_int32, P,
+                                              c_int64, P, P, P, c_int64, P, P, P]),
 }
 
 

@@ -486,6 +486,80 @@ def paged_decode4(q, k_codes, v_codes, kv_params, cu_seqlens_k, block_tables, *,
     return out
 
 
+# ------------------------------------------------- rotary positions with several axes
+
+
+def mrope_freq_axis(sections, *, interleaved: bool, device="cuda") -> torch.Tensor:
+    """The axis of each of the ``sum(sections)`` = head_dim / 2 frequencies, int32, for
+    :func:`qk_norm_mrope_store`: one run of frequencies per axis, or (``interleaved``) axis
+    ``a`` > 0 at every frequency ``a`` modulo the axes below ``axes * sections[a]``, axis 0
+    at the others."""
+    axes, half = len(sections), sum(sections)
+    _need(axes >= 1 and min(sections) >= 0, "mrope_freq_axis: sections of frequencies, one per axis")
+    if interleaved:
+        _need(all(n == 0 or a + axes * (n - 1) < half for a, n in enumerate(sections) if a),
+              "mrope_freq_axis: interleaved sections reach past the frequencies")
+        axis = [j % axes if j < axes * sections[j % axes] else 0 for j in range(half)]
+    else:
+        axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(axis, dtype=torch.int32, device=device)
+
+
+def qk_norm_mrope_store(qkv, positions, freq_axis, *, num_heads: int, num_kv_heads: int,
+                        head_dim: int, q_weight, k_weight, eps: float, cos_sin_cache, q_out,
+                        k_cache=None, v_cache=None, k_codes=None, v_codes=None, kv_params=None,
+                        slot_mapping=None, error_flag=None) -> torch.Tensor:
+    """:func:`qk_norm_rope_store` for positions with several axes (time, height, width):
+    positions int64 [axes, T], ``freq_axis`` int32 [head_dim / 2] the axis each frequency
+    turns by (:func:`mrope_freq_axis`). K and V go to a bf16 cache (``k_cache``,
+    ``v_cache``) or a 4-bit one (``k_codes``, ``v_codes``, ``kv_params``); returns q_out
+    [T, num_heads, head_dim]."""
+    what = "qk_norm_mrope_store"
+    tokens = qkv.shape[0]
+    _need(qkv.dtype == BF16 and qkv.dim() == 2 and qkv.stride(1) == 1
+          and qkv.shape[1] == (num_heads + 2 * num_kv_heads) * head_dim,
+          f"{what}: qkv bf16 [T, (num_heads + 2 num_kv_heads) head_dim] with contiguous rows")
+    _need(positions.dtype == torch.int64 and positions.dim() == 2 and positions.shape[1] == tokens
+          and (positions.stride(1) == 1 or tokens <= 1), f"{what}: positions int64 [axes, T]")
+    _need(freq_axis.dtype == torch.int32 and freq_axis.is_contiguous()
+          and freq_axis.numel() == head_dim // 2, f"{what}: freq_axis int32 [head_dim / 2]")
+    _need(q_weight.dtype == BF16 and k_weight.dtype == BF16 and q_weight.is_contiguous()
+          and k_weight.is_contiguous() and q_weight.numel() == k_weight.numel() == head_dim,
+          f"{what}: norm weights bf16 [head_dim]")
+    _need(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.is_contiguous()
+          and cos_sin_cache.shape[-1] == head_dim, f"{what}: fp32 rope table [positions, head_dim]")
+    _need(q_out.dtype == BF16 and tuple(q_out.shape) == (tokens, num_heads, head_dim)
+          and q_out.stride(2) == 1 and (q_out.stride(1) == head_dim or num_heads == 1),
+          f"{what}: q_out bf16 [T, num_heads, head_dim]")
+    num_slots, cache4 = 0, None
+    if slot_mapping is not None:
+        _need(slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous()
+              and slot_mapping.numel() == tokens, f"{what}: int32 slots, one per token")
+        _need((k_cache is None) != (k_codes is None),
+              f"{what}: slot_mapping needs a bf16 cache or a 4-bit one")
+        if k_codes is not None:
+            cache4 = _kv4(what, k_codes, v_codes, kv_params)
+            _need(cache4.num_kv_heads == num_kv_heads and cache4.head_dim == head_dim,
+                  f"{what}: the 4-bit cache has other heads")
+        else:
+            for c in (k_cache, v_cache):
+                _need(c is not None and c.dtype == BF16 and c.is_contiguous()
+                      and tuple(c.shape[-2:]) == (num_kv_heads, head_dim)
+                      and c.numel() == k_cache.numel(),
+                      f"{what}: contiguous bf16 caches [..., num_kv_heads, head_dim]")
+            num_slots = k_cache.numel() // (num_kv_heads * head_dim)
+    _here(what, qkv, positions, freq_axis, q_weight, k_weight, cos_sin_cache, q_out, slot_mapping,
+          k_cache, v_cache, error_flag)
+    _count()
+    check(lib.b200asr_qk_norm_mrope_store(
+        _p(qkv), qkv.stride(0), _p(positions), positions.stride(0), positions.shape[0], _p(freq_axis),
+        tokens, num_heads, num_kv_heads, head_dim, _p(q_weight), _p(k_weight), float(eps),
+        _p(cos_sin_cache), cos_sin_cache.shape[0], _p(q_out), q_out.stride(0), _p(slot_mapping),
+        _p(k_cache) if cache4 is None else None, _p(v_cache) if cache4 is None else None, num_slots,
+        None if cache4 is None else ctypes.byref(cache4), _p(error_flag), _stream()), what)
+    return q_out
+
+
 # --------------------------------------------------------------------- sampler
 
 

@@ -13,7 +13,8 @@
  * declared bounds (a KV slot or block id outside the pool, a position outside the
  * RoPE table) it skips that access and ORs a bit into *error_flag (when non-NULL):
  *   B200ASR_DEVERR_SLOT 1, B200ASR_DEVERR_BLOCK 2, B200ASR_DEVERR_POSITION 4,
- *   B200ASR_DEVERR_LENGTH 8. The host reads the word after the step.
+ *   B200ASR_DEVERR_LENGTH 8, B200ASR_DEVERR_ADAPTER 32. The host reads the word after the
+ *   step.
  *
  * Reference locations are paths inside the qwen-asr-vllm project.
  */
@@ -47,7 +48,8 @@ enum {
   B200ASR_DEVERR_SLOT = 1,
   B200ASR_DEVERR_BLOCK = 2,
   B200ASR_DEVERR_POSITION = 4,
-  B200ASR_DEVERR_LENGTH = 8
+  B200ASR_DEVERR_LENGTH = 8,
+  B200ASR_DEVERR_ADAPTER = 32 /* a row's adapter index is neither -1 nor an adapter */
 };
 
 /* Library version (major*10000 + minor*100 + patch) and last error message. */
@@ -532,6 +534,36 @@ B200ASR_API int b200asr_qk_norm_mrope_store(
     float eps, const float *cos_sin_cache, int32_t max_position, void *q_out,
     int64_t q_out_row_stride, const int32_t *slot_mapping, void *k_cache, void *v_cache,
     int64_t num_slots, const b200asr_kv4 *cache4, int32_t *error_flag, b200asr_stream_t stream);
+
+/* ------------------------------------- low-rank adapters of many requests at once ----
+ * y[t] = x[t] W^T + scales[a] (x[t] A_a^T) B_a^T with a = row_adapter[t] (-1: none; another
+ * index outside [0, num_adapters) counts as none and raises B200ASR_DEVERR_ADAPTER), beside
+ * the projections of models/qwen3.py:20-69. lora_a bf16 [num_adapters, rank, k], lora_b bf16
+ * [num_adapters, n, rank], both contiguous; scales fp32; row_adapter int32; rank a multiple
+ * of 8, at most 128 (smaller adapters are padded with zeros). x rows 16-byte aligned.
+ * lora_down: t fp32 [rows, rank] = scales[a] x A_a^T; rows without an adapter are not written.
+ * linear_small_lora: linear_small (no SiLU) whose epilogue adds t B_a^T before the one
+ *   rounding to bf16, from lora_down's t; m <= 64.
+ * lora_rows: y bf16 [rows, n], both products in one accumulator, t rounded to bf16; k and n
+ *   multiples of 8. The workspace (b200asr_lora_rows_workspace_size bytes, 16-byte aligned)
+ *   needs no initial value, keeps nothing between calls and serves one call at a time. */
+B200ASR_API int b200asr_lora_down(const void *x, int64_t x_row_stride, int32_t rows, int32_t k,
+                                  const void *lora_a, int32_t num_adapters, int32_t rank,
+                                  const float *scales, const int32_t *row_adapter, float *t,
+                                  int32_t *error_flag, b200asr_stream_t stream);
+B200ASR_API int b200asr_linear_small_lora(const void *x, int64_t x_row_stride, int32_t m, int32_t k,
+                                          const void *w, int32_t n, const float *t,
+                                          const void *lora_b, int32_t num_adapters, int32_t rank,
+                                          const int32_t *row_adapter, void *y,
+                                          int64_t y_row_stride, int32_t *error_flag,
+                                          b200asr_stream_t stream);
+B200ASR_API size_t b200asr_lora_rows_workspace_size(int32_t rows, int32_t rank);
+B200ASR_API int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t rows, int32_t k,
+                                  const void *w, int32_t n, const void *lora_a,
+                                  const void *lora_b, int32_t num_adapters, int32_t rank,
+                                  const float *scales, const int32_t *row_adapter, void *y,
+                                  int64_t y_row_stride, void *workspace, size_t workspace_bytes,
+                                  int32_t *error_flag, b200asr_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -34,6 +34,9 @@
 //        per-head RMSNorm, the rotation (partner dims in lane ^ 16) and the paged-cache
 //        store of K and V happen on the reduced tile, with the rounding of the unfused
 //        kernels (bf16 projection, bf16 after the norm, after the weight, after RoPE).
+//      - low-rank adapter epilogue: a column's row belongs to one request, whose adapter's
+//        up-projection of lora_down's t (lora.cu) is added to the reduced sums in fp32, before
+//        their one rounding; the split columns spread the adapters' rows over the CTAs.
 //    A decode layer is then qkv (norm + rope + store) -> attention -> o_proj (+residual)
 //    -> gate_up (norm, SiLU*mul) -> down (+residual): five launches instead of eight.
 //
@@ -76,7 +79,7 @@ struct LinearArgs {
   int32_t *error_flag;
 };
 
-enum : int { kEpiPlain = 0, kEpiSilu = 1, kEpiAdd = 2, kEpiQkRope = 3 };
+enum : int { kEpiPlain = 0, kEpiSilu = 1, kEpiAdd = 2, kEpiQkRope = 3, kEpiLora = 4 };
 
 struct LinearFuse {
   // RMSNorm prologue: x[r, k] = bf16(bf16(h[r, k] * rsqrt(sum_t ss[t][r] / K + eps)) * w[k])
@@ -105,6 +108,11 @@ struct LinearFuse {
   __nv_bfloat16 *k_cache, *v_cache;
   const int32_t *slot_mapping;
   int64_t num_slots;
+  // low-rank adapter epilogue: y[c, n] += sum_r lora_t[c][r] lora_b[row_adapter[c]][n][r]
+  const float *lora_t;
+  const __nv_bfloat16 *lora_b;
+  const int32_t *row_adapter;
+  int num_adapters, rank, lora_n;
   // optional L2 prefetch, issued before the wait (b200asr_l2_prefetch): a layer's cached
   // K/V rows of the listed sequences, and up to two contiguous byte ranges
   const int32_t *pf_cu_seqlens_k;  // null: no K/V prefetch
@@ -381,6 +389,24 @@ __device__ __forceinline__ void qk_rope_store4(const LinearFuse &f, const Linear
                              lane * 4) = packed;
 }
 
+// Four neighbouring outputs of row c: += t[c] . B_ad[n .. n + 3] (B's rows are contiguous).
+__device__ __forceinline__ void lora_up4(float (&y)[4], const LinearFuse &f, int c, int ad, int n) {
+  const float *t = f.lora_t + static_cast<int64_t>(c) * f.rank;
+  const __nv_bfloat16 *b = f.lora_b + (static_cast<int64_t>(ad) * f.lora_n + n) * f.rank;
+#pragma unroll 2
+  for (int r = 0; r < f.rank; r += 8) {
+    const float4 t0 = *reinterpret_cast<const float4 *>(t + r);
+    const float4 t1 = *reinterpret_cast<const float4 *>(t + r + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v[8];
+      unpack8(*reinterpret_cast<const uint4 *>(b + e * f.rank + r), v);
+      y[e] = fmaf(t0.x, v[0], fmaf(t0.y, v[1], fmaf(t0.z, v[2], fmaf(t0.w, v[3], y[e]))));
+      y[e] = fmaf(t1.x, v[4], fmaf(t1.y, v[5], fmaf(t1.z, v[6], fmaf(t1.w, v[7], y[e]))));
+    }
+  }
+}
+
 template <int MP, bool NORM_IN, int EPI>
 __global__ void __launch_bounds__(kLnThreads)
     linear_small_kernel(const __grid_constant__ CUtensorMap tm_w,
@@ -626,6 +652,12 @@ __global__ void __launch_bounds__(kLnThreads)
       else if (i == 1) cur = pre[1];
       else epi_fetch<EPI>(cur, f, a, c, tile, lane);
       qk_rope_store4(f, a, c, tile, lane, v4, cur, qk_nw);
+    } else if (EPI == kEpiLora) {
+      float y[4] = {acc.x, acc.y, acc.z, acc.w};
+      const int ad = f.row_adapter[c];
+      if (ad >= 0 && ad < f.num_adapters) lora_up4(y, f, c, ad, tile * kLnRows + lane * 4);
+      __nv_bfloat16 *dst = a.y + c * a.y_stride + tile * kLnRows + lane * 4;
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
     } else {
       __nv_bfloat16 *dst = a.y + c * a.y_stride + tile * kLnRows + lane * 4;
       *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc.x, acc.y), pack2(acc.z, acc.w));
@@ -1110,6 +1142,34 @@ extern "C" int b200asr_linear_small(const void *x, int64_t x_row_stride, int32_t
                                               error_flag, st);
   return silu_inner ? dispatch_linear<false, kEpiSilu>(x, x_row_stride, m, k, w, n, a, f, tiles, st)
                     : dispatch_linear<false, kEpiPlain>(x, x_row_stride, m, k, w, n, a, f, tiles, st);
+}
+
+extern "C" int b200asr_linear_small_lora(const void *x, int64_t x_row_stride, int32_t m, int32_t k,
+                                         const void *w, int32_t n, const float *t,
+                                         const void *lora_b, int32_t num_adapters, int32_t rank,
+                                         const int32_t *row_adapter, void *y, int64_t y_row_stride,
+                                         int32_t *error_flag, b200asr_stream_t stream) {
+  B200_REQUIRE(m >= 0 && m <= 64, "linear_small_lora: %d rows (at most 64)", m);
+  if (m == 0) return B200ASR_OK;
+  B200_REQUIRE(k > 0 && k % kLnBK == 0, "linear_small_lora: K %d must be a multiple of %d", k, kLnBK);
+  B200_REQUIRE(n > 0 && n % kLnRows == 0, "linear_small_lora: N %d must be a multiple of %d", n, kLnRows);
+  B200_REQUIRE(rank >= 8 && rank % 8 == 0 && num_adapters >= 1,
+               "linear_small_lora: rank %d must be a multiple of 8", rank);
+  B200_REQUIRE(x && w && t && lora_b && row_adapter && y, "linear_small_lora: null pointer");
+  B200_REQUIRE(aligned16(x) && aligned16(w) && aligned16(t) && aligned16(lora_b) && aligned16(y) &&
+                   x_row_stride >= k && x_row_stride % 8 == 0 && y_row_stride >= n && y_row_stride % 4 == 0,
+               "linear_small_lora: misaligned tensor");
+  const int tiles = n / kLnRows;
+  const LinearArgs a = make_args(m, linear_split(tiles, k / kLnBK), 0, y, y_row_stride, error_flag);
+  LinearFuse f = {};
+  f.lora_t = t;
+  f.lora_b = static_cast<const __nv_bfloat16 *>(lora_b);
+  f.row_adapter = row_adapter;
+  f.num_adapters = num_adapters;
+  f.rank = rank;
+  f.lora_n = n;
+  return dispatch_linear<false, kEpiLora>(x, x_row_stride, m, k, w, n, a, f, tiles,
+                                          static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int b200asr_linear_small_add(const void *x, int64_t x_row_stride, int32_t m, int32_t k,

@@ -1,0 +1,617 @@
+// Low-rank adapters of many requests beside a shared projection (models/qwen3.py:20-69 has
+// the projections; the reference serves one set of weights):
+//   y[t] = x[t] W^T + s_a (x[t] A_a^T) B_a^T,   a = row_adapter[t], none for a = -1.
+//
+// lora_down   rows of a decode step: t = s_a x A_a^T in 32 bits, which the projection's own
+//             epilogue expands (linear.cu, b200asr_linear_small_lora).
+// lora_rows   any number of rows: t as bf16, then x W^T and t B^T in one accumulator.
+#include "common.cuh"
+
+namespace b200asr {
+
+// The row's adapter, or -1 (flagged when the index is neither -1 nor an adapter).
+__device__ __forceinline__ int row_adapter_of(const int32_t *rows, int64_t t, int num, int32_t *flag) {
+  const int a = rows[t];
+  if (a >= 0 && a < num) return a;
+  if (a != -1) raise_flag(flag, B200ASR_DEVERR_ADAPTER);
+  return -1;
+}
+
+// ------------------------------------------------------------------ down, few rows
+// One warp per (row, 4 ranks): every lane holds 8 consecutive k of x and of the four rows of A,
+// 16-byte loads all independent of each other. At decode sizes this is latency: enough warps
+// that each streams a few KB, no shared memory, no second pass.
+constexpr int kLdRanks = 4;
+
+__global__ void __launch_bounds__(128) lora_down_kernel(
+    const __nv_bfloat16 *__restrict__ x, int64_t x_stride, int rows, int k,
+    const __nv_bfloat16 *__restrict__ a, int num_adapters, int rank, const float *__restrict__ scales,
+    const int32_t *__restrict__ row_adapter, float *__restrict__ t, int32_t *error_flag) {
+  pdl_trigger();
+  pdl_wait();
+  const int per_row = rank / kLdRanks;
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = w / per_row, r0 = (w - row * per_row) * kLdRanks;
+  if (row >= rows) return;
+  const int ad = row_adapter_of(row_adapter, row, num_adapters, lane == 0 ? error_flag : nullptr);
+  if (ad < 0) return;  // the expansion does not read this row
+  const __nv_bfloat16 *xr = x + row * x_stride;
+  const __nv_bfloat16 *ar = a + (static_cast<int64_t>(ad) * rank + r0) * k;
+  float acc[kLdRanks] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = lane * 8; i < k; i += 256) {
+    float xv[8], av[8];
+    unpack8(*reinterpret_cast<const uint4 *>(xr + i), xv);
+#pragma unroll
+    for (int r = 0; r < kLdRanks; ++r) {
+      unpack8(*reinterpret_cast<const uint4 *>(ar + static_cast<int64_t>(r) * k + i), av);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r] = fmaf(xv[e], av[e], acc[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kLdRanks; ++r) acc[r] = warp_sum(acc[r]);
+  if (lane == 0) {
+    const float s = scales[ad];
+    *reinterpret_cast<float4 *>(t + static_cast<int64_t>(row) * rank + r0) =
+        make_float4(acc[0] * s, acc[1] * s, acc[2] * s, acc[3] * s);
+  }
+}
+
+// ------------------------------------------------------------------ down, any rows
+// A CTA takes 32 rows; its four warps split K, mma m16n8k16 straight from global memory (a
+// lane's 8 consecutive k are its operands of two k-steps, so x and A are read in 64-byte
+// runs), and their sums are joined in shared memory. The distinct adapters of the 32 rows are
+// taken in turn: a prefill batch's rows follow one another by request, so there are one or
+// two. t is rounded to bf16 once, as activations between projections are: it is the operand
+// of the second product. The last CTAs of the launch list each 256-row tile's distinct
+// adapters for that product.
+constexpr int kLtRows = 32;
+constexpr int kLoraMaxRank = 128;
+constexpr int kLgTile = 256;            // rows and columns of a CTA pair's tile
+constexpr int kLgPlan = 1 + kLgTile;    // plan entry of a row tile: count, adapters ascending
+
+struct LoraDownArgs {
+  const __nv_bfloat16 *x;
+  int64_t x_stride;
+  int rows, k, rank, num_adapters;
+  const __nv_bfloat16 *a;
+  const float *scales;
+  const int32_t *row_adapter;
+  __nv_bfloat16 *t;   // [rows, rank]
+  int32_t *plan;      // [row tiles][kLgPlan]
+  int32_t *error_flag;
+};
+
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t a0, const uint32_t a1,
+                                               const uint32_t a2, const uint32_t a3,
+                                               const uint32_t b0, const uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Distinct adapters of rows [256 tile, +256), ascending (128 threads, two rows each).
+__device__ __forceinline__ void lora_plan(const LoraDownArgs &p, int tile) {
+  __shared__ int ids[kLgTile], first[kLgTile];
+  int count = 0;
+  for (int i = threadIdx.x; i < kLgTile; i += 128) {
+    const int64_t r = static_cast<int64_t>(tile) * kLgTile + i;
+    ids[i] = r < p.rows ? row_adapter_of(p.row_adapter, r, p.num_adapters, nullptr) : -1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kLgTile; i += 128) {
+    bool is_first = ids[i] >= 0;
+    for (int j = 0; j < i && is_first; ++j) is_first = ids[j] != ids[i];
+    first[i] = is_first;
+  }
+  __syncthreads();
+  int32_t *out = p.plan + static_cast<int64_t>(tile) * kLgPlan;
+  for (int i = threadIdx.x; i < kLgTile; i += 128) {
+    if (!first[i]) continue;
+    int place = 0;
+    for (int j = 0; j < kLgTile; ++j) place += first[j] && ids[j] < ids[i];
+    out[1 + place] = ids[i];
+    ++count;
+  }
+  count = __syncthreads_count(count & 1) + 2 * __syncthreads_count(count >> 1);
+  if (threadIdx.x == 0) out[0] = count;
+}
+
+// NT: rank tiles of 8 per pass over x.
+template <int NT>
+__global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs p) {
+  __shared__ float part[2][kLtRows][8 * NT + 1];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int tiles = (p.rows + kLtRows - 1) / kLtRows;
+  if (static_cast<int>(blockIdx.x) >= tiles) {
+    lora_plan(p, blockIdx.x - tiles);
+    return;
+  }
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kLtRows;
+  const int mine = row0 + lane < p.rows ? row_adapter_of(p.row_adapter, row0 + lane, p.num_adapters,
+                                                         warp == 0 ? p.error_flag : nullptr)
+                                        : -1;
+  for (unsigned left = __ballot_sync(0xffffffffu, mine >= 0); left;) {
+    const int ad = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
+    const unsigned rows = __ballot_sync(0xffffffffu, mine == ad);
+    left &= ~rows;
+    const __nv_bfloat16 *am = p.a + static_cast<int64_t>(ad) * p.rank * p.k;
+    for (int r0 = 0; r0 < p.rank; r0 += 8 * NT) {
+      float acc[2][NT][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
+#pragma unroll 2
+      for (int k0 = warp * 32; k0 < p.k; k0 += 128) {
+        const int kk = k0 + q * 8;
+        uint4 xv[2][2], av[NT];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const int r = m * 16 + hh * 8 + g;
+            xv[m][hh] = make_uint4(0, 0, 0, 0);
+            if (kk < p.k && (rows >> r & 1))
+              xv[m][hh] = *reinterpret_cast<const uint4 *>(p.x + (row0 + r) * p.x_stride + kk);
+          }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          av[j] = make_uint4(0, 0, 0, 0);
+          if (kk < p.k && r0 + j * 8 + g < p.rank)
+            av[j] = *reinterpret_cast<const uint4 *>(am + static_cast<int64_t>(r0 + j * 8 + g) * p.k + kk);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            mma_bf16_16816(acc[m][j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av[j].x, av[j].y);
+            mma_bf16_16816(acc[m][j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av[j].z, av[j].w);
+          }
+      }
+      // warps 0 and 1 lay their sums down, 2 and 3 add theirs
+#pragma unroll
+      for (int turn = 0; turn < 2; ++turn) {
+        if (warp >> 1 == turn) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float &to = part[warp & 1][m * 16 + g + (e >> 1) * 8][j * 8 + q * 2 + (e & 1)];
+                to = turn ? to + acc[m][j][e] : acc[m][j][e];
+              }
+        }
+        __syncthreads();
+      }
+      const float s = p.scales[ad];
+      for (int i = tid; i < kLtRows * 4 * NT; i += 128) {
+        const int r = i / (4 * NT), c = 2 * (i - r * (4 * NT));
+        if ((rows >> r & 1) && r0 + c < p.rank)
+          *reinterpret_cast<uint32_t *>(p.t + (row0 + r) * p.rank + r0 + c) =
+              pack2((part[0][r][c] + part[1][r][c]) * s, (part[0][r][c + 1] + part[1][r][c + 1]) * s);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// --------------------------------------------------------- projection + up, any rows
+// y = x W^T + t B^T in one accumulator, rounded once. A pair of CTAs (cta_group::2) takes tiles
+// of 256 rows x 256 columns: each CTA loads its 128 rows of x and 128 of the 256 weight rows,
+// 32 KB per 64 of K, so an SM reads 64 bytes per cycle of MMA where one CTA alone on a 128 x
+// 256 tile would read 96. Persistent: the two halves of TMEM hold two accumulators, and a tile
+// is written out while the next one's products run.
+// The adapters are more K steps at the end of a tile, one per distinct adapter of its 256 rows
+// (and 64 ranks): the weight side is 256 rows of B_a, the row side t with zeros in the rows of
+// other adapters, which four warps write in the layout the MMA reads. They have a buffer and
+// barriers of their own, so the ring of x and W runs on.
+//   warps 0-3 epilogue | 4-7 t rows | 8 TMA | 9 TMEM and MMA (of the pair's first CTA)
+constexpr int kLgThreads = 320;
+constexpr int kLgBK = 64;
+constexpr int kLgStages = 6;
+constexpr int kLgHalf = 128 * kLgBK * 2;          // 16 KB: 128 rows of x or of W
+constexpr int kLgStage = 2 * kLgHalf;
+constexpr int kLgSmem = 1024 + (kLgStages + 1) * kLgStage + 256;
+static_assert(kLgSmem <= 232448, "shared memory of a CTA");
+
+struct LoraGemmArgs {
+  int rows, n, k_steps, rank;
+  int tiles_m, tiles_n;
+  const __nv_bfloat16 *t;
+  const int32_t *row_adapter;
+  const int32_t *plan;
+  __nv_bfloat16 *y;
+  int64_t y_stride;
+  int32_t *error_flag;
+};
+
+__device__ __forceinline__ uint32_t lg_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void lg_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same shared-memory address in the pair's first CTA.
+__device__ __forceinline__ uint32_t lg_first(uint32_t saddr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(saddr));
+  return r;
+}
+__device__ __forceinline__ void lg_arrive_first(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lg_first(smem_addr(bar)))
+               : "memory");
+}
+// As mbar_wait, acquiring what the other CTA of the pair released.
+__device__ __forceinline__ bool lg_wait(uint64_t *bar, uint32_t parity, int32_t *err, volatile int *abort) {
+  const uint64_t start = globaltimer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (globaltimer_ns() - start > kWaitLimitNs) {
+      *abort = 1;
+      raise_flag(err, B200ASR_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+// Loads into this CTA's shared memory, counted on the first CTA's barrier.
+__device__ __forceinline__ void lg_load_2d(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void lg_load_3d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void lg_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the barrier at this address in both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void lg_commit(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
+    lora_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_b, const LoraGemmArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *ring = smem;                                   // [stage] x half | W half
+  uint8_t *lora = smem + kLgStages * kLgStage;            // t half | B half
+  uint64_t *bars = reinterpret_cast<uint64_t *>(lora + kLgStage);
+  uint64_t *full = bars;                       // first CTA's: both CTAs' loads of the stage
+  uint64_t *empty = full + kLgStages;          // each CTA's: the stage's MMAs are done
+  uint64_t *acc_full = empty + kLgStages;      // [2] each CTA's: the tile's MMAs are done
+  uint64_t *acc_empty = acc_full + 2;          // [2] first CTA's: both CTAs' warps have read it
+  uint64_t *l_full = acc_empty + 2;            // first CTA's: B of both CTAs and every t row
+  uint64_t *l_empty = l_full + 1;              // each CTA's
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(l_empty + 1);
+  __shared__ int abort_flag;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = lg_rank();
+  pdl_trigger();
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kLgStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 8);
+    }
+    mbar_init(l_full, 1 + 8);
+    mbar_init(l_empty, 1);
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  lg_cluster_sync();  // both CTAs' barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int chunks = (a.rank + kLgBK - 1) / kLgBK;
+  auto tile_m = [&](int t) { return t / a.tiles_n; };
+  auto tile_n = [&](int t) { return t % a.tiles_n; };
+  auto lora_steps = [&](int t) { return a.plan[static_cast<int64_t>(tile_m(t)) * kLgPlan] * chunks; };
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------------- loads
+    if (lane == 0) {
+      uint32_t it = 0, lt = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const int m0 = tile_m(t) * kLgTile + rank * 128, n0 = tile_n(t) * kLgTile + rank * 128;
+        for (int s = 0; s < a.k_steps && ok; ++s, ++it) {
+          const int st = it % kLgStages;
+          ok = lg_wait(&empty[st], ((it / kLgStages) & 1) ^ 1, a.error_flag, &abort_flag);
+          if (!ok) break;
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * kLgStage);
+          const uint32_t bar = lg_first(smem_addr(&full[st]));
+          lg_load_2d(ring + st * kLgStage, &tm_x, s * kLgBK, m0, bar);
+          lg_load_2d(ring + st * kLgStage + kLgHalf, &tm_w, s * kLgBK, n0, bar);
+        }
+        const int steps = lora_steps(t);
+        for (int s = 0; s < steps && ok; ++s, ++lt) {
+          ok = lg_wait(l_empty, (lt & 1) ^ 1, a.error_flag, &abort_flag);
+          if (!ok) break;
+          if (rank == 0) mbar_arrive_expect_tx(l_full, 2 * kLgHalf);
+          const int ad = a.plan[static_cast<int64_t>(tile_m(t)) * kLgPlan + 1 + s / chunks];
+          lg_load_3d(lora + kLgHalf, &tm_b, (s % chunks) * kLgBK, n0, ad, lg_first(smem_addr(l_full)));
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------------- MMAs
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_bf16_f32(256, 256, false, false);
+      uint32_t it = 0, lt = 0;
+      int j = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs, ++j) {
+        const int acc = j & 1;
+        ok = lg_wait(&acc_empty[acc], ((j >> 1) & 1) ^ 1, a.error_flag, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * 256;
+        for (int s = 0; s < a.k_steps; ++s, ++it) {
+          const int st = it % kLgStages;
+          ok = lg_wait(&full[st], (it / kLgStages) & 1, a.error_flag, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t xb = smem_addr(ring + st * kLgStage), wb = xb + kLgHalf;
+#pragma unroll
+          for (int kk = 0; kk < kLgBK / 16; ++kk)
+            lg_mma(d, smem_desc_sw128(xb + kk * 32, 16, 1024), smem_desc_sw128(wb + kk * 32, 16, 1024), idesc,
+                   (s > 0 || kk > 0) ? 1u : 0u);
+          lg_commit(&empty[st]);
+        }
+        const int steps = ok ? lora_steps(t) : 0;
+        for (int s = 0; s < steps; ++s, ++lt) {
+          ok = lg_wait(l_full, lt & 1, a.error_flag, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tb = smem_addr(lora), bb = tb + kLgHalf;
+          const int kmax = (min(kLgBK, a.rank - (s % chunks) * kLgBK) + 15) / 16;
+          for (int kk = 0; kk < kmax; ++kk)
+            lg_mma(d, smem_desc_sw128(tb + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024), idesc, 1u);
+          lg_commit(l_empty);
+        }
+        if (ok) lg_commit(&acc_full[acc]);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------- t rows of the adapters
+    const int r = tid - 128;  // row of this CTA's half
+    uint8_t *dst = lora + (r >> 3) * 1024 + (r & 7) * 128;
+    uint32_t lt = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      const int64_t row = static_cast<int64_t>(tile_m(t)) * kLgTile + rank * 128 + r;
+      const int mine = row < a.rows ? a.row_adapter[row] : -1;
+      const int32_t *plan = a.plan + static_cast<int64_t>(tile_m(t)) * kLgPlan;
+      const int steps = plan[0] * chunks;
+      for (int s = 0; s < steps; ++s, ++lt) {
+        const int c0 = (s % chunks) * kLgBK;
+        const bool own_row = mine == plan[1 + s / chunks];
+        uint4 v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          v[c] = make_uint4(0, 0, 0, 0);
+          if (own_row && c0 + c * 8 < a.rank)
+            v[c] = *reinterpret_cast<const uint4 *>(a.t + row * a.rank + c0 + c * 8);
+        }
+        ok = __all_sync(0xffffffffu, lg_wait(l_empty, (lt & 1) ^ 1, a.error_flag, &abort_flag));
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4 *>(dst + ((c ^ (r & 7)) << 4)) = v[c];
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) lg_arrive_first(l_full);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------- epilogue
+    int j = 0;
+    for (int t = pair; t < tiles; t += pairs, ++j) {
+      const int acc = j & 1;
+      if (!__all_sync(0xffffffffu, lg_wait(&acc_full[acc], (j >> 1) & 1, a.error_flag, &abort_flag))) break;
+      tc_fence_after();
+      const int64_t row = static_cast<int64_t>(tile_m(t)) * kLgTile + rank * 128 + tid;
+      const int n0 = tile_n(t) * kLgTile;
+      const uint32_t base = tmem + acc * 256 + (static_cast<uint32_t>(warp * 32) << 16);
+      __nv_bfloat16 *dst = a.y + row * a.y_stride + n0;
+#pragma unroll 1
+      for (int c = 0; c < 256; c += 32) {
+        if (n0 + c >= a.n) break;
+        float v[32];
+        tmem_ld32(base + c, v);
+        tmem_wait_ld();
+        if (row < a.rows) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n0 + c + i * 8 < a.n)
+              *reinterpret_cast<uint4 *>(dst + c + i * 8) =
+                  make_uint4(pack2(v[8 * i], v[8 * i + 1]), pack2(v[8 * i + 2], v[8 * i + 3]),
+                             pack2(v[8 * i + 4], v[8 * i + 5]), pack2(v[8 * i + 6], v[8 * i + 7]));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) lg_arrive_first(&acc_empty[acc]);
+    }
+  }
+  // No CTA leaves while the other may still read its shared memory, its TMEM or its barriers,
+  // nor, after a timed-out wait, while copies may still be landing in it.
+  __syncwarp();
+  if (abort_flag) {
+    const uint64_t start = globaltimer_ns();
+    while (globaltimer_ns() - start < 2000000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  lg_cluster_sync();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+}  // namespace b200asr
+
+using namespace b200asr;
+
+namespace {
+
+int lora_shapes(const char *what, int rows, int k, int rank, int num_adapters) {
+  B200_REQUIRE(rows >= 0 && k >= 8 && k % 8 == 0 && num_adapters >= 1, "%s: bad sizes (K %d must be a "
+               "multiple of 8)", what, k);
+  B200_REQUIRE(rank >= 8 && rank % 8 == 0 && rank <= kLoraMaxRank,
+               "%s: rank %d must be a multiple of 8 in [8, %d]", what, rank, kLoraMaxRank);
+  return B200ASR_OK;
+}
+
+}  // namespace
+
+extern "C" int b200asr_lora_down(const void *x, int64_t x_row_stride, int32_t rows, int32_t k,
+                                 const void *lora_a, int32_t num_adapters, int32_t rank,
+                                 const float *scales, const int32_t *row_adapter, float *t,
+                                 int32_t *error_flag, b200asr_stream_t stream) {
+  const int rc = lora_shapes("lora_down", rows, k, rank, num_adapters);
+  if (rc != B200ASR_OK) return rc;
+  if (rows == 0) return B200ASR_OK;
+  B200_REQUIRE(x && lora_a && scales && row_adapter && t, "lora_down: null pointer");
+  B200_REQUIRE(aligned16(x) && x_row_stride % 8 == 0 && aligned16(lora_a) && aligned16(t),
+               "lora_down: rows must be 16-byte aligned");
+  const int64_t warps = static_cast<int64_t>(rows) * (rank / kLdRanks);
+  B200_REQUIRE(warps <= 0x7fffffff, "lora_down: too many rows");
+  B200_LAUNCH_CHECK_ERR(
+      launch_kernel(lora_down_kernel, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, stream,
+                    true, 1, static_cast<const __nv_bfloat16 *>(x), x_row_stride, static_cast<int>(rows),
+                    static_cast<int>(k), static_cast<const __nv_bfloat16 *>(lora_a),
+                    static_cast<int>(num_adapters), static_cast<int>(rank), scales, row_adapter, t, error_flag),
+      "lora_down");
+  return B200ASR_OK;
+}
+
+extern "C" size_t b200asr_lora_rows_workspace_size(int32_t rows, int32_t rank) {
+  if (rows < 0 || rank < 0) return 0;
+  const size_t tiles = (static_cast<size_t>(rows) + kLgTile - 1) / kLgTile;
+  return (static_cast<size_t>(rows) * rank * 2 + 15) / 16 * 16 + tiles * kLgPlan * 4;
+}
+
+extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t rows, int32_t k,
+                                 const void *w, int32_t n, const void *lora_a, const void *lora_b,
+                                 int32_t num_adapters, int32_t rank, const float *scales,
+                                 const int32_t *row_adapter, void *y, int64_t y_row_stride,
+                                 void *workspace, size_t workspace_bytes, int32_t *error_flag,
+                                 b200asr_stream_t stream) {
+  const int rc = lora_shapes("lora_rows", rows, k, rank, num_adapters);
+  if (rc != B200ASR_OK) return rc;
+  B200_REQUIRE(n >= 8 && n % 8 == 0, "lora_rows: N %d must be a multiple of 8", n);
+  if (rows == 0) return B200ASR_OK;
+  B200_REQUIRE(x && w && lora_a && lora_b && scales && row_adapter && y && workspace, "lora_rows: null pointer");
+  B200_REQUIRE(aligned16(x) && x_row_stride >= k && x_row_stride % 8 == 0 && aligned16(w) && aligned16(lora_a) &&
+                   aligned16(lora_b) && aligned16(y) && y_row_stride % 8 == 0 && aligned16(workspace),
+               "lora_rows: rows must be 16-byte aligned");
+  const size_t need = b200asr_lora_rows_workspace_size(rows, rank);
+  if (workspace_bytes < need) {
+    set_error("lora_rows: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    return B200ASR_ERR_WORKSPACE;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  LoraGemmArgs g{};
+  g.rows = rows;
+  g.n = n;
+  g.k_steps = (k + kLgBK - 1) / kLgBK;
+  g.rank = rank;
+  g.tiles_m = (rows + kLgTile - 1) / kLgTile;
+  g.tiles_n = (n + kLgTile - 1) / kLgTile;
+  B200_REQUIRE(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 2, "lora_rows: too many tiles");
+  LoraDownArgs p{};
+  p.x = static_cast<const __nv_bfloat16 *>(x);
+  p.x_stride = x_row_stride;
+  p.rows = rows;
+  p.k = k;
+  p.rank = rank;
+  p.num_adapters = num_adapters;
+  p.a = static_cast<const __nv_bfloat16 *>(lora_a);
+  p.scales = scales;
+  p.row_adapter = row_adapter;
+  p.t = static_cast<__nv_bfloat16 *>(workspace);
+  p.plan = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(workspace) +
+                                       (static_cast<size_t>(rows) * rank * 2 + 15) / 16 * 16);
+  p.error_flag = error_flag;
+  g.t = p.t;
+  g.plan = p.plan;
+  g.row_adapter = row_adapter;
+  g.y = static_cast<__nv_bfloat16 *>(y);
+  g.y_stride = y_row_stride;
+  g.error_flag = error_flag;
+  CUtensorMap tx, tw, tb;
+  const uint32_t box[3] = {kLgBK, 128, 1};
+  const uint64_t xd[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows)};
+  const uint64_t xs[1] = {static_cast<uint64_t>(x_row_stride) * 2};
+  const uint64_t wd[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n)};
+  const uint64_t ws[1] = {static_cast<uint64_t>(k) * 2};
+  const uint64_t bd[3] = {static_cast<uint64_t>(rank), static_cast<uint64_t>(n), static_cast<uint64_t>(num_adapters)};
+  const uint64_t bs[2] = {static_cast<uint64_t>(rank) * 2, static_cast<uint64_t>(rank) * n * 2};
+  if (!make_tmap_bf16(&tx, x, 2, xd, xs, box) || !make_tmap_bf16(&tw, w, 2, wd, ws, box) ||
+      !make_tmap_bf16(&tb, lora_b, 3, bd, bs, box))
+    return B200ASR_ERR_CUDA;
+  B200_LAUNCH_CHECK_ERR(
+      cudaFuncSetAttribute(lora_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmem),
+      "lora_rows (configuration)");
+  const int down = (rows + kLtRows - 1) / kLtRows;
+  auto kfn = rank <= 32 ? lora_down_rows_kernel<4> : lora_down_rows_kernel<8>;
+  B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(down + g.tiles_m), dim3(128), 0, st, true, 1, p), "lora_rows (down)");
+  const int pairs = std::min(g.tiles_m * g.tiles_n, num_sms() / 2);
+  B200_LAUNCH_CHECK_ERR(launch_kernel(lora_gemm_kernel, dim3(2 * pairs), dim3(kLgThreads), kLgSmem, st, true, 1, tx,
+                                      tw, tb, g),
+                        "lora_rows");
+  return B200ASR_OK;
+}

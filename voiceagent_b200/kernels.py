@@ -638,6 +638,64 @@ def linear_small(x, weight, *, silu: bool = False, out=None, error_flag=None) ->
     return out
 
 
+# -------------------------------------------------- low-rank adapters of many requests
+
+LORA_MAX_RANK = 128
+
+
+def lora_linear(x, weight, lora_a, lora_b, scales, row_adapter, *, out=None,
+                error_flag=None) -> torch.Tensor:
+    """``x @ weight.T`` plus each row's own low-rank adapter:
+    ``scales[a] * (x @ lora_a[a].T) @ lora_b[a].T`` with ``a = row_adapter[row]`` (-1: none).
+
+    x bf16 [T, K] (rows may be strided), weight bf16 [N, K], lora_a bf16 [adapters, rank, K],
+    lora_b bf16 [adapters, N, rank] (rank a multiple of 8 up to 128; pad smaller adapters
+    with zeros), scales fp32 [adapters], row_adapter int32 [T]. Both products share one fp32
+    accumulator and one rounding; decode-size batches run on :func:`linear_small`'s kernel
+    with the adapters in its epilogue."""
+    what = "lora_linear"
+    _need(x.dtype == BF16 and x.dim() == 2 and x.stride(1) == 1, f"{what}: x bf16 [T, K] with contiguous rows")
+    _need(weight.dtype == BF16 and weight.dim() == 2 and weight.is_contiguous()
+          and weight.shape[1] == x.shape[1], f"{what}: weight bf16 [N, K]")
+    (m, k), n = x.shape, weight.shape[0]
+    _need(lora_a.dtype == BF16 and lora_a.dim() == 3 and lora_a.is_contiguous() and lora_a.shape[2] == k,
+          f"{what}: lora_a bf16 [adapters, rank, K]")
+    adapters, rank = lora_a.shape[:2]
+    _need(lora_b.dtype == BF16 and lora_b.is_contiguous() and tuple(lora_b.shape) == (adapters, n, rank),
+          f"{what}: lora_b bf16 [adapters, N, rank]")
+    _need(adapters >= 1 and 8 <= rank <= LORA_MAX_RANK and rank % 8 == 0,
+          f"{what}: rank a multiple of 8, at most {LORA_MAX_RANK}")
+    _need(k % 8 == 0 and n % 8 == 0 and k > 0 and n > 0 and x.stride(0) % 8 == 0,
+          f"{what}: K, N and the row stride of x multiples of 8")
+    _need(scales.dtype == torch.float32 and scales.is_contiguous() and scales.numel() == adapters,
+          f"{what}: fp32 scales, one per adapter")
+    _need(row_adapter.dtype == torch.int32 and row_adapter.is_contiguous() and row_adapter.numel() == m,
+          f"{what}: int32 row_adapter, one per row")
+    if out is None:
+        out = torch.empty(m, n, dtype=BF16, device=x.device)
+    _need(out.dtype == BF16 and tuple(out.shape) == (m, n) and out.stride(1) == 1
+          and out.stride(0) % 8 == 0, f"{what}: out bf16 [T, N] with contiguous rows")
+    _here(what, x, weight, lora_a, lora_b, scales, row_adapter, out, error_flag)
+    if m == 0:
+        return out
+    if linear_small_ok(x, weight):
+        t = torch.empty(m, rank, dtype=torch.float32, device=x.device)
+        _count(2)
+        check(lib.b200asr_lora_down(_p(x), x.stride(0), m, k, _p(lora_a), adapters, rank, _p(scales),
+                                    _p(row_adapter), _p(t), _p(error_flag), _stream()), what)
+        check(lib.b200asr_linear_small_lora(_p(x), x.stride(0), m, k, _p(weight), n, _p(t), _p(lora_b),
+                                            adapters, rank, _p(row_adapter), _p(out), out.stride(0),
+                                            _p(error_flag), _stream()), what)
+        return out
+    size = lib.b200asr_lora_rows_workspace_size(m, rank)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _count(2)
+    check(lib.b200asr_lora_rows(_p(x), x.stride(0), m, k, _p(weight), n, _p(lora_a), _p(lora_b), adapters,
+                                rank, _p(scales), _p(row_adapter), _p(out), out.stride(0), _p(workspace),
+                                size, _p(error_flag), _stream()), what)
+    return out
+
+
 # ---------------------------------------------------------------- decode-step fusions
 # A decoder row between the projections of a decode step is carried as ``h`` (fp32
 # [m, hidden], the pre-norm residual sum) and ``ss`` (fp32 [m, hidden / 128], per

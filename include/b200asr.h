@@ -517,6 +517,20 @@ B200ASR_API int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64
                                       void *workspace, size_t workspace_bytes,
                                       int32_t *error_flag, b200asr_stream_t stream);
 
+/* paged_prefill over the 4-bit cache (layers/attention.py:87-107): q/out bf16 [total_q,
+ * num_heads, D], rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] of sequence b attending its
+ * cu_seqlens_k[b + 1] - cu_seqlens_k[b] cached tokens, causal with the mask aligned
+ * bottom-right; strides, tables, flags and group sizes as for paged_decode4. A row that sees
+ * no key (no cached token, or more query than cached tokens) gives zeros. */
+B200ASR_API int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
+                                       const b200asr_kv4 *cache, int32_t num_heads,
+                                       const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                       const int32_t *block_tables, int64_t bt_stride,
+                                       int32_t bt_width, int32_t batch, int32_t total_q,
+                                       float scale, void *out, int64_t out_row_stride,
+                                       int64_t out_head_stride, int32_t *error_flag,
+                                       b200asr_stream_t stream);
+
 /* ------------------------------------------- rotary positions with several axes ----
  * qk_norm_rope_store (models/qwen3.py:43-48) for positions int64 [axes, num_tokens] (row
  * stride position_stride): frequency j of the head_dim / 2 turns by the position of axis

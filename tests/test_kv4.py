@@ -9,6 +9,9 @@ Tolerances of the attention outputs are element by element, from the roundings t
   D / 16 + 1 additions of 2^-23 each: an absolute error e of the score (base e) changes each
   probability by the factor exp(+-e), so the output by at most 2 e sum_t p_t |v_t - out|
   <= 2 e (sum_t p_t |v_t| + |out|);
+* prefill rounds the cache's values to bf16 as a bf16 cache would hold them: a score (base e)
+  then moves by at most e = 2^-8 |scale| sum_i |q_i k_i| + (the 32-bit part, terms |q_i k_i|),
+  and V by 2^-8 of |v|; its probability alone is rounded, 2^-8 of sum_t p_t |v_t|;
 * 2^-16 of sum_t p_t (|v_t| + |zero_t|) for the other 32-bit sums, exp2 and the division (up to a
   few hundred additions of 2^-24 each and exp2 within 2^-22).
 """
@@ -69,7 +72,7 @@ def sequence_rows(cache, table, n):
     return k, unpack_codes(vc).astype(np.float64), par[..., 2:3], par[..., 3:4], par[..., 0:1]
 
 
-def plain_attention(q, cache, table, n, scale, q_len=1):
+def plain_attention(q, cache, table, n, scale, prefill=False):
     """out [q_len, H, D] and its tolerance, causal with the mask aligned bottom-right."""
     q = q.double().cpu().numpy()
     m, heads, d = q.shape
@@ -89,11 +92,18 @@ def plain_attention(q, cache, table, n, scale, q_len=1):
             p = np.exp(s - s.max())
             p /= p.sum()
             o = p @ v[:seen, g]
-            e = abs(scale) * ks[:seen, g].max() * 143 * np.abs(q[i, h]).sum() * (d / 16 + 1) * 2.0 ** -23
             mass = p @ np.abs(v[:seen, g])
+            if prefill:  # a key's e weighs with its probability
+                e = (2.0 ** -8 + (d / 16 + 1) * 2.0 ** -23) * abs(scale) * (np.abs(k[:seen, g]) @ np.abs(q[i, h]))
+                rounded = 2 * 2.0 ** -8 * mass
+                moved = (p * e) @ np.abs(v[:seen, g]) + (p @ e) * np.abs(o)  # exp(x) - 1 <= x exp(x)
+                moved = moved * np.exp(e.max())
+            else:
+                e = abs(scale) * ks[:seen, g].max() * 143 * np.abs(q[i, h]).sum() * (d / 16 + 1) * 2.0 ** -23
+                rounded = 2.0 ** -8 * (p @ (vs[:seen, g] * np.abs(vcode[:seen, g] - 8)))
+                moved = 2 * e * (mass + np.abs(o))
             out[i, h] = o
-            tol[i, h] = (2.0 ** -8 * np.abs(o) + 2.0 ** -8 * (p @ (vs[:seen, g] * np.abs(vcode[:seen, g] - 8)))
-                         + 2 * e * (mass + np.abs(o))
+            tol[i, h] = (2.0 ** -8 * np.abs(o) + rounded + moved
                          + 2.0 ** -16 * (mass + p @ np.abs(vz[:seen, g] * np.ones(d))))
     return out, tol
 
@@ -206,6 +216,13 @@ def test_c_entries_refuse_bad_calls():
     assert dec(qs=2044) == 1 and "aligned" in err()
     assert dec(longest=-1) == 1 and "sizes" in err()
     assert dec(batch=0) == 0
+    pre = lambda **k: lib.b200asr_paged_prefill4(  # noqa: E731
+        p, 2048, 128, c, k.get("heads", 16), p, p, p, 4, 4, k.get("batch", 2), k.get("rows", 9), 1.0, p,
+        k.get("os", 2048), 128, None, None)
+    assert pre(heads=12) == 1 and "multiple" in err()
+    assert pre(os=2044) == 1 and "aligned" in err()
+    assert pre(rows=-1) == 1 and "sizes" in err()
+    assert pre(batch=0) == 0 and pre(rows=0) == 0
 
 
 def test_wrappers_refuse_cpu_tensors_and_wrong_types(kx):
@@ -418,3 +435,119 @@ def test_decode_not_finite_rows_reach_only_their_sequence(kx):
     out = torch.empty_like(q)
     kx.paged_decode4(q, *cache, starts(lens), table, max_seqlen_k=100, scale=0.1, out=out)
     assert out[1].isnan().all() and torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2])
+
+
+# ------------------------------------------------------------------------------ prefill
+
+
+def check_prefill(kx, q_lens, k_lens, heads, hkv, d, bs, layout="slots", q_scale=1.5, seed=0, scale=None):
+    table, blocks = paged(seed, k_lens, bs)
+    cache = filled(seed + 1, blocks, bs, hkv, d, layout)
+    poison_unused(cache, table, k_lens)
+    gen = torch.Generator().manual_seed(seed + 2)
+    total = sum(q_lens)
+    q = (torch.randn(total + 3, heads, d, generator=gen) * q_scale).bfloat16().cuda()
+    scale = d ** -0.5 if scale is None else scale
+    out = torch.full_like(q, float("nan"))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kx.paged_prefill4(q, *cache, starts(q_lens), starts(k_lens), table, max_seqlen_q=max(q_lens),
+                      max_seqlen_k=max(k_lens), scale=scale, out=out, error_flag=err)
+    torch.cuda.synchronize()
+    assert err.item() == 0 and out[total:].isnan().all()
+    at = 0
+    for b, (m, n) in enumerate(zip(q_lens, k_lens)):
+        want, tol = plain_attention(q[at:at + m], cache, table[b], n, scale, prefill=True)
+        check_close(out[at:at + m], want, tol, f"sequence {b}: {m} rows, {n} keys")
+        at += m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,hkv,d,bs,layout", [
+    (16, 8, 128, 256, "slots"), (4, 2, 128, 16, "heads"), (7, 1, 128, 48, "slots"), (14, 2, 64, 32, "heads"),
+    (3, 3, 64, 1, "slots"), (9, 1, 64, 16, "slots"), (34, 2, 128, 256, "slots")])
+def test_prefill_against_64_bits(kx, heads, hkv, d, bs, layout):
+    check_prefill(kx, [1, 5, 0, 64, 33, 1, 2], [1, 5, 17, 64, 300, 129, 140], heads, hkv, d, bs, layout)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,k_lens", [
+    ([200], [200]), ([128], [128]), ([129], [1000]), ([1], [0]), ([3, 4], [0, 2]), ([300, 7], [290, 3]), ([1], [2500])])
+def test_prefill_lengths(kx, q_lens, k_lens):
+    check_prefill(kx, q_lens, k_lens, 4, 2, 128, 16, seed=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+def test_prefill_scales(kx, scale):
+    check_prefill(kx, [70, 1], [200, 140], 4, 2, 128, 256, seed=5, scale=scale)
+
+
+@pytest.mark.gpu
+def test_prefill_more_items_than_ctas(kx):
+    rng = np.random.default_rng(1)
+    q = [int(n) for n in rng.integers(0, 6, size=200)]
+    check_prefill(kx, q, [n + int(rng.integers(0, 20)) for n in q], 4, 2, 64, 16, seed=6)
+
+
+@pytest.mark.gpu
+def test_prefill_equals_decode_on_single_rows(kx):
+    """One query token per sequence is what paged_decode4 computes (which rounds less)."""
+    lens = [1, 50, 700, 1290]
+    table, blocks = paged(3, lens, 256)
+    cache = filled(4, blocks, 256, 8, 128)
+    q = torch.randn(4, 16, 128, device="cuda").bfloat16()
+    one = run_decode(kx, q, cache, table, lens, 0.08)
+    out = torch.empty_like(q)
+    kx.paged_prefill4(q, *cache, starts([1] * 4), starts(lens), table, max_seqlen_q=1, max_seqlen_k=1290, scale=0.08,
+                      out=out)
+    for b, n in enumerate(lens):
+        _, tol = plain_attention(q[b:b + 1], cache, table[b], n, 0.08, prefill=True)
+        _, tol1 = plain_attention(q[b:b + 1], cache, table[b], n, 0.08)
+        check_close(out[b:b + 1], one[b:b + 1].double().cpu().numpy(), tol + tol1, f"row {b}")
+
+
+@pytest.mark.gpu
+def test_prefill_not_finite_keys_reach_only_the_rows_that_see_them(kx):
+    table, blocks = paged(2, [100, 100], 16)
+    cache = filled(3, blocks, 16, 2, 128)
+    q = torch.randn(200, 4, 128, device="cuda").bfloat16()
+    call = lambda: kx.paged_prefill4(  # noqa: E731
+        q, *cache, starts([100, 100]), starts([100, 100]), table, max_seqlen_q=100, max_seqlen_k=100, scale=0.1,
+        out=torch.empty_like(q))
+    clean = call()
+    for half in (slice(0, 2), slice(2, 4)):  # K, then V, of key 60 of the second sequence
+        kept = cache[2].clone()
+        cache[2][table[1, 3].long(), 12, 1, half] = float("nan")
+        got = call()
+        cache[2].copy_(kept)
+        hit = torch.zeros(200, 4, dtype=torch.bool, device="cuda")
+        hit[160:, 2:] = True
+        assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit])
+
+
+@pytest.mark.gpu
+def test_prefill_flags_and_capture(kx):
+    q_lens, k_lens = [30, 40], [60, 300]
+    table, blocks = paged(7, k_lens, 16)
+    cache = filled(8, blocks, 16, 2, 64)
+    q = torch.randn(70, 4, 64, device="cuda").bfloat16()
+    out, err = torch.empty_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    cq, ck = starts(q_lens), starts(k_lens)
+    call = lambda t: kx.paged_prefill4(  # noqa: E731
+        q, *cache, cq, ck, t, max_seqlen_q=40, max_seqlen_k=300, scale=0.1, out=out, error_flag=err)
+    bad = table.clone()
+    bad[1, 3] = -5
+    call(bad)
+    assert err.item() == 2
+    err.zero_()
+    call(table[:, :8])
+    assert err.item() == 8
+    err.zero_()
+    call(table)
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(table)
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want) and err.item() == 0

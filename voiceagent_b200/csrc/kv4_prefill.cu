@@ -1,0 +1,584 @@
+// Causal attention of many new tokens per sequence over the 4-bit paged KV cache (kv4.cuh has
+// the format): the 4-bit form of paged_prefill (layers/attention.py:87-107), the mask aligned
+// bottom-right, any number of query heads per KV head.
+//
+// Work item: 256 query rows of one (sequence, KV head), a row being one (token, query head of
+// the group) pair, token-major, so any group size fills the tile. The rows are two tiles of
+// 128 (the MMA's M) that share every K and V tile of 128 tokens:
+//   warps 0-3, 4-7  softmax of tile 0 / 1, thread = row = TMEM lane
+//   warps 8-11      codes to bf16: K and V tiles into shared memory, 128-byte swizzled
+//   warp 12         TMEM and tcgen05.mma
+// What bounds it: per 128 tokens of one KV head (D = 128) the tensor cores need 2048 cycles for
+// both row tiles, the 32768 exponentials 2048 cycles of the special-function units, and the
+// codes of K and V ~600 instructions per converting thread, a quarter of what two row
+// tiles' softmax issues; with one row tile the conversion would weigh twice as much.
+//  * P replaces its scores in TMEM (bf16, half the columns) and is the A operand from there.
+//    The next S of a row tile is issued right after its P V, so a tile's softmax runs under the
+//    other tile's products, and its scores being complete means that its previous P V is too:
+//    rescaling O needs no barrier of its own.
+//  * Online softmax with a lazy maximum: it moves only when a row passes it by 2^8.
+//  * A word of 8 codes gives the pairs (i, i + 4), so dims are permuted within groups of 8;
+//    q is laid out alike, and the output is put back in order as it is written.
+//  * K and V values are rounded to bf16 (2^-9 of the value, the precision of a bf16 cache); they
+//    are zero + code * scale in one rounding.
+//  * A V row that is not finite is written as zeros and its K row as NaN: the rows that may
+//    attend it become NaN, those that may not keep their values (0 * NaN would reach them).
+#include "kv4.cuh"
+
+namespace b200asr {
+
+constexpr int kP4Threads = 13 * 32;
+constexpr int kP4Rows = 256, kP4Keys = 128;
+constexpr float kP4Lazy = 8.f;
+
+struct Prefill4Args {
+  const __nv_bfloat16 *q;
+  int64_t q_row, q_head;
+  b200asr_kv4 c;
+  const int32_t *cu_q, *cu_k, *block_tables;
+  int64_t bt_stride;
+  int bt_width, batch, total_q, group, bs_shift;
+  float scale_log2;  // >= 0: the sign is in `flip`
+  uint32_t flip;     // sign bits to exchange in q
+  __nv_bfloat16 *out;
+  int64_t out_row, out_head;
+  int32_t *error_flag;
+};
+
+template <int D>
+struct Pre4 {
+  static constexpr int HALVES = D / 64;             // 64-dim column blocks of a tile
+  static constexpr int BLOCK = 128 * 128;           // bytes of one: 128 rows x 64 bf16
+  static constexpr int TILE = HALVES * BLOCK;       // Q, K or V
+  static constexpr int SMEM = 1024 + 6 * TILE + 256;  // 2 Q, 2 K, 2 V
+};
+
+// One sequence's part of the item list, and where an item lies.
+struct Item4 {
+  int b, h, rows, row0;  // rows of this item, the first one's index in the sequence
+  int q0, offset, n_kv, tiles;
+  bool cut;  // the table row is too short for the sequence
+};
+
+// Walks this CTA's items (item = row tile * KV heads + head, row tiles numbered sequence by
+// sequence). Every warp walks alone and sees the same items.
+struct Walk4 {
+  // query tokens of a sequence, held to the rows that q has
+  static __device__ __forceinline__ int q_len_of(const Prefill4Args &a, int b) {
+    return max(0, min(a.cu_q[b + 1], a.total_q) - max(0, a.cu_q[b]));
+  }
+  int i, scan, carry;  // next item; the sequences before `scan` hold `carry` row tiles
+  __device__ __forceinline__ bool next(const Prefill4Args &a, Item4 &it) {
+    const int lane = threadIdx.x & 31, heads = a.c.num_kv_heads;
+    while (true) {
+      const int t = i / heads;
+      it.h = i - t * heads;
+      i += gridDim.x;
+      while (true) {
+        if (scan >= a.batch) return false;
+        const int bb = scan + lane;
+        const int n = bb < a.batch ? (q_len_of(a, bb) * a.group + kP4Rows - 1) / kP4Rows : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, t < carry + incl);
+        if (here) {
+          const int src = __ffs(here) - 1;
+          it.b = scan + src;
+          it.row0 = (t - carry - __shfl_sync(0xffffffffu, incl - n, src)) * kP4Rows;
+          break;
+        }
+        carry += __shfl_sync(0xffffffffu, incl, 31);
+        scan += 32;
+      }
+      it.q0 = max(0, a.cu_q[it.b]);
+      const int q_len = q_len_of(a, it.b);
+      const int k_len = max(0, a.cu_k[it.b + 1] - a.cu_k[it.b]);
+      const int room = static_cast<int>(min(static_cast<int64_t>(0x7fffffff),
+                                            static_cast<int64_t>(a.bt_width) * a.c.block_size));
+      it.offset = k_len - q_len;
+      it.cut = k_len > room;
+      it.rows = min(kP4Rows, q_len * a.group - it.row0);
+      const int last = it.offset + (it.row0 + it.rows - 1) / a.group;  // last key of the last row
+      it.n_kv = max(0, min(last + 1, room));
+      it.tiles = (it.n_kv + kP4Keys - 1) / kP4Keys;
+      return true;
+    }
+  }
+};
+
+__device__ __forceinline__ void p4_mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void p4_tmem_st16(uint32_t taddr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// 8 codes as four bf16 pairs of values, dims (i, i + 4): zero + code * scale.
+__device__ __forceinline__ uint4 p4_values(uint32_t w, __nv_bfloat162 scale, __nv_bfloat162 zero) {
+  uint32_t out[4];
+  const uint32_t k = 0xc300c300u;  // -128, -128
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t p = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;  // 128 + code
+    __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&p);
+    x = __hadd2(x, *reinterpret_cast<const __nv_bfloat162 *>(&k));  // code, exact
+    x = __hfma2(x, scale, zero);
+    out[i] = *reinterpret_cast<uint32_t *>(&x);
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Prefill4Args a) {
+  using C = Pre4<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sQ = smem;                 // [row tile]
+  uint8_t *sK = sQ + 2 * C::TILE;     // [stage]
+  uint8_t *sV = sK + 2 * C::TILE;     // [stage]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sV + 2 * C::TILE);
+  uint64_t *q_full = bars;            // [2] rows of the item laid out
+  uint64_t *k_full = bars + 2, *k_empty = bars + 4, *v_full = bars + 6, *v_empty = bars + 8;  // [2] each
+  uint64_t *s_full = bars + 10;       // [2] scores of the row tile (and its earlier P V) done
+  uint64_t *p_full = bars + 12;       // [2] P written, O rescaled
+  uint64_t *o_full = bars + 14;       // [2] the item's last P V done
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
+  __shared__ int abort_flag;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_trigger();
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // S0 | S1 | O0 | O1, 128 columns each
+  pdl_wait();
+
+  Walk4 walk{static_cast<int>(blockIdx.x), 0, 0};
+  Item4 it;
+  // Waits as a whole warp: every lane of a role sees the same outcome.
+  auto wait = [&](uint64_t *bar, uint32_t phase) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.error_flag, &abort_flag)) != 0;
+  };
+  auto arrive = [&](uint64_t *bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ softmax
+    const int w = warp >> 2, r = tid & 127;
+    const uint32_t s_base = tmem + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t o_base = tmem + 256 + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // this thread's row of q into the tile, dims in the order of the codes' pairs
+    auto load_q = [&](const Item4 &t) {
+      const int row = w * 128 + r;
+      const bool in = row < t.rows;
+      const int tok = in ? (t.row0 + row) / a.group : 0, head = in ? (t.row0 + row) - tok * a.group : 0;
+      const __nv_bfloat16 *src = a.q + (t.q0 + tok) * a.q_row + (static_cast<int64_t>(t.h) * a.group + head) * a.q_head;
+      uint8_t *dst = sQ + w * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (in) u = *reinterpret_cast<const uint4 *>(src + j * 8);
+        const uint4 v = make_uint4(__byte_perm(u.x, u.z, 0x5410) ^ a.flip, __byte_perm(u.x, u.z, 0x7632) ^ a.flip,
+                                   __byte_perm(u.y, u.w, 0x5410) ^ a.flip, __byte_perm(u.y, u.w, 0x7632) ^ a.flip);
+        *reinterpret_cast<uint4 *>(dst + (j >> 3) * C::BLOCK + (((j & 7) ^ (r & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      arrive(&q_full[w]);
+    };
+    uint32_t ps = 0, po = 0;  // phases of this tile's scores and outputs
+    bool more = walk.next(a, it);
+    if (more && it.tiles > 0 && w * 128 < it.rows) load_q(it);
+    while (more) {
+      const Item4 cur = it;
+      const bool mine = cur.tiles > 0 && w * 128 < cur.rows;
+      const int row = w * 128 + r;
+      const int tok = (cur.row0 + row) / a.group;
+      const int last = row < cur.rows ? min(cur.offset + tok, cur.n_kv - 1) : -1;  // last key this row sees
+      const bool warp_rows = w * 128 + (r & ~31) < cur.rows;
+      // keys up to here are seen by every row of the warp that is written
+      const int first_row = cur.row0 + w * 128 + (r & ~31);
+      const int all_seen = min(cur.offset + first_row / a.group, cur.n_kv - 1);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      if (mine) {
+        for (int j = 0; j < cur.tiles; ++j, ++ps) {
+          if (!wait(&s_full[w], ps)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (warp_rows) {
+            const int key0 = j * kP4Keys;
+            const bool whole = key0 + kP4Keys - 1 <= all_seen;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+              float s[32];
+              tmem_ld32(s_base + c, s);
+              tmem_wait_ld();
+              if (whole) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, s[i]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, key0 + c + i <= last ? s[i] : -INFINITY);
+              }
+            }
+            mx *= a.scale_log2;
+            if (mx != mx) mx = -INFINITY;  // -inf * 0
+            const bool move = mx > m + kP4Lazy || m == -INFINITY;
+            const float m_new = move ? fmaxf(m, mx) : m;
+            const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
+            if (j > 0 && __any_sync(0xffffffffu, move && alpha != 1.f)) {
+#pragma unroll 1
+              for (int c = 0; c < D; c += 32) {
+                float o[32];
+                tmem_ld32(o_base + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                tmem_st32(o_base + c, o);
+              }
+            }
+            m = m_new;
+            l *= alpha;
+            const float shift = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+              float s[32];
+              tmem_ld32(s_base + c, s);
+              tmem_wait_ld();
+              if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (key0 + c + i > last) s[i] = -INFINITY;
+              }
+              uint32_t p[16];
+              float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float p0 = exp2f(fmaf(s[2 * i], a.scale_log2, shift));
+                float p1 = exp2f(fmaf(s[2 * i + 1], a.scale_log2, shift));
+                if (!whole) {  // -inf * 0 where the scale is zero
+                  if (key0 + c + 2 * i > last) p0 = 0.f;
+                  if (key0 + c + 2 * i + 1 > last) p1 = 0.f;
+                }
+                sum0 += p0;
+                sum1 += p1;
+                p[i] = pack2(p0, p1);
+              }
+              l += sum0 + sum1;
+              p4_tmem_st16(s_base + c / 2, p);  // over scores already read
+            }
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          arrive(&p_full[w]);
+        }
+      }
+      if (!ok) break;
+      // the next item's rows while this one's last product runs: its scores are done with Q
+      more = walk.next(a, it);
+      if (more && it.tiles > 0 && w * 128 < it.rows) load_q(it);
+      if (mine) {
+        if (!wait(&o_full[w], po)) break;
+        ++po;
+        tc_fence_after();
+      }
+      if (cur.tiles == 0 ? warp_rows : mine && warp_rows) {
+        const bool in = row < cur.rows;
+        const int head = (cur.row0 + row) - tok * a.group;
+        const float inv = last >= 0 ? 1.f / l : 0.f;
+        __nv_bfloat16 *dst = a.out + (cur.q0 + tok) * a.out_row +
+                             (static_cast<int64_t>(cur.h) * a.group + head) * a.out_head;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          if (mine) {
+            tmem_ld32(o_base + c, o);
+            tmem_wait_ld();
+          }
+          if (in) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              // columns 8 i + (0..7) hold dims 0, 4, 1, 5, 2, 6, 3, 7 of their group
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (last >= 0)
+                v = make_uint4(pack2(o[8 * i] * inv, o[8 * i + 2] * inv), pack2(o[8 * i + 4] * inv, o[8 * i + 6] * inv),
+                               pack2(o[8 * i + 1] * inv, o[8 * i + 3] * inv),
+                               pack2(o[8 * i + 5] * inv, o[8 * i + 7] * inv));
+              *reinterpret_cast<uint4 *>(dst + c + 8 * i) = v;
+            }
+          }
+        }
+        tc_fence_before();
+      }
+    }
+  } else if (warp < 12) {
+    // -------------------------------------------------------- codes to bf16 tiles
+    constexpr int CH = D / 32;            // 16-byte pieces of a row, and rounds of a warp's 32 rows
+    constexpr int PER = 32 / CH;          // rows of a round
+    const int t = lane % CH, rr = lane / CH;
+    // rows of one shared-memory phase differ in the swizzle
+    const int sub = D == 128 ? (rr & 4) | ((rr & 1) << 1) | ((rr >> 1) & 1) : rr;
+    const int row0 = (warp - 8) * 32 + sub;
+    uint32_t jg = 0;
+    bool ok = true;
+    while (ok && walk.next(a, it)) {
+      if (it.tiles == 0) continue;
+      const int32_t *table = a.block_tables + it.b * a.bt_stride;
+      uint4 kr[CH], vr[CH];
+      uint2 pr[CH];
+      auto fetch = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int key = j * kP4Keys + row0 + i * PER;
+          kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+          pr[i] = make_uint2(0, 0);
+          if (key < it.n_kv) {
+            const int page = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.c.block_size;
+            const int at = a.bs_shift >= 0 ? key & (a.c.block_size - 1) : key - page * a.c.block_size;
+            int block = table[page];
+            if (block < 0 || block >= a.c.num_blocks) {
+              raise_flag(a.error_flag, B200ASR_DEVERR_BLOCK);
+              block = 0;
+            }
+            const int64_t off = block * a.c.code_stride[0] + at * a.c.code_stride[1] + it.h * a.c.code_stride[2] + t * 16;
+            kr[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.c.k_codes) + off);
+            vr[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.c.v_codes) + off);
+            pr[i] = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.c.params) +
+                                                     block * a.c.param_stride[0] + at * a.c.param_stride[1] +
+                                                     it.h * a.c.param_stride[2]);
+          }
+        }
+      };
+      fetch(0);
+      for (int j = 0; j < it.tiles; ++j, ++jg) {
+        const int st = jg & 1;
+        uint4 k0[CH], v0[CH];
+        uint2 p0[CH];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          k0[i] = kr[i];
+          v0[i] = vr[i];
+          p0[i] = pr[i];
+          // a V row that is not finite: zeros, and NaN for its K row
+          const bool bad = (p0[i].y & 0x7f80u) == 0x7f80u || (p0[i].y & 0x7f800000u) == 0x7f800000u;
+          if (bad) {
+            p0[i] = make_uint2(0x7fc07fc0u, 0u);
+            v0[i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        if (j + 1 < it.tiles) fetch(j + 1);
+        auto write = [&](uint8_t *tile, const uint4 &codes, uint32_t sz, int row) {
+          const uint32_t s2 = __byte_perm(sz, sz, 0x1010), z2 = __byte_perm(sz, sz, 0x3232);
+          const __nv_bfloat162 scale = *reinterpret_cast<const __nv_bfloat162 *>(&s2);
+          const __nv_bfloat162 zero = *reinterpret_cast<const __nv_bfloat162 *>(&z2);
+          const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
+          uint8_t *dst = tile + (t >> 1) * (D == 128 ? C::BLOCK : 0) + (row >> 3) * 1024 + (row & 7) * 128;
+          const int turn = D == 128 ? t >> 1 : 0;  // halves of a row in different banks
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = turn ? word[i ^ 1] : word[i];
+            const int ch = (t & 1) * 4 + (i ^ turn);
+            *reinterpret_cast<uint4 *>(dst + ((ch ^ (row & 7)) << 4)) = p4_values(x, scale, zero);
+          }
+        };
+        if (!wait(&k_empty[st], (jg >> 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) write(sK + st * C::TILE, k0[i], p0[i].x, row0 + i * PER);
+        fence_proxy_async_smem();
+        arrive(&k_full[st]);
+        if (!wait(&v_empty[st], (jg >> 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) write(sV + st * C::TILE, v0[i], p0[i].y, row0 + i * PER);
+        fence_proxy_async_smem();
+        arrive(&v_full[st]);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------------- MMAs
+    constexpr uint32_t idesc_s = idesc_bf16_f32(128, kP4Keys, false, false);
+    constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true);
+    const uint32_t q_s = smem_addr(sQ), k_s = smem_addr(sK), v_s = smem_addr(sV);
+    uint32_t jg = 0, items = 0, items1 = 0, tile0 = 0, tile1 = 0;
+    bool ok = true;
+    auto scores = [&](int w, uint32_t jj) {  // S_w = Q_w K^T of global tile jj
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * C::BLOCK + (k & 3) * 32;
+          umma_f16_ss(tmem + w * 128, smem_desc_sw128(q_s + w * C::TILE + off, 16, 1024),
+                      smem_desc_sw128(k_s + (jj & 1) * C::TILE + off, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[w]);
+      }
+      __syncwarp();
+    };
+    while (ok && walk.next(a, it)) {
+      if (it.cut && lane == 0) raise_flag(a.error_flag, B200ASR_DEVERR_LENGTH);
+      if (it.tiles == 0) continue;
+      const int tiles_w = it.rows > 128 ? 2 : 1;
+      ok = wait(&q_full[0], items) && wait(&k_full[jg & 1], jg >> 1);
+      if (!ok) break;
+      tc_fence_after();
+      scores(0, jg);
+      if (tiles_w == 2) {
+        ok = wait(&q_full[1], items1);
+        if (!ok) break;
+        tc_fence_after();
+        scores(1, jg);
+      }
+      if (lane == 0) umma_commit(&k_empty[jg & 1]);
+      for (int j = 0; j < it.tiles && ok; ++j, ++jg) {
+        for (int w = 0; w < tiles_w && ok; ++w) {
+          ok = wait(&p_full[w], w ? tile1 : tile0);
+          if (!ok) break;
+          if (w) ++tile1;
+          else ++tile0;
+          if (w == 0) ok = wait(&v_full[jg & 1], jg >> 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < kP4Keys / 16; ++k)
+              p4_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8,
+                        smem_desc_sw128(v_s + (jg & 1) * C::TILE + k * 2048, C::BLOCK, 1024), idesc_o,
+                        (j > 0 || k > 0) ? 1u : 0u);
+            if (w == tiles_w - 1) umma_commit(&v_empty[jg & 1]);
+            if (j == it.tiles - 1) umma_commit(&o_full[w]);
+          }
+          __syncwarp();
+          if (j + 1 < it.tiles) {
+            if (w == 0) ok = wait(&k_full[(jg + 1) & 1], (jg + 1) >> 1);
+            if (!ok) break;
+            tc_fence_after();
+            scores(w, jg + 1);
+            if (w == tiles_w - 1 && lane == 0) umma_commit(&k_empty[(jg + 1) & 1]);
+          }
+        }
+      }
+      ++items;
+      if (tiles_w == 2) ++items1;
+    }
+  }
+
+  __syncwarp();
+  if (abort_flag) {  // after a timed-out wait: products already issued still read this memory
+    const uint64_t start = globaltimer_ns();
+    while (globaltimer_ns() - start < 2000000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D>
+int launch_prefill4(const Prefill4Args &a, int64_t total_q, cudaStream_t stream) {
+  using C = Pre4<D>;
+  const int64_t most = ((total_q * a.group + kP4Rows - 1) / kP4Rows + a.batch) * a.c.num_kv_heads;
+  B200_REQUIRE(most <= 0x3fffffff && total_q * a.group <= 0x3fffffff, "paged_prefill4: too many rows");
+  auto kfn = paged_prefill4_kernel<D>;
+  B200_LAUNCH_CHECK_ERR(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
+                        "paged_prefill4 (configuration)");
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(most, num_sms()));
+  B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(grid), dim3(kP4Threads), C::SMEM, stream, true, 1, a),
+                        "paged_prefill4");
+  return B200ASR_OK;
+}
+
+}  // namespace b200asr
+
+using namespace b200asr;
+
+extern "C" int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
+                                      const b200asr_kv4 *cache, int32_t num_heads,
+                                      const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                      const int32_t *block_tables, int64_t bt_stride,
+                                      int32_t bt_width, int32_t batch, int32_t total_q, float scale,
+                                      void *out, int64_t out_row_stride, int64_t out_head_stride,
+                                      int32_t *error_flag, b200asr_stream_t stream) {
+  B200_REQUIRE(cache != nullptr, "paged_prefill4: null cache");
+  const int D = cache->head_dim;
+  B200_REQUIRE(D == 64 || D == 128, "paged_prefill4: head_dim %d unsupported (64 or 128)", D);
+  B200_REQUIRE(batch >= 0 && total_q >= 0 && num_heads >= 1 && bt_width >= 0, "paged_prefill4: bad sizes");
+  B200_REQUIRE(cache->num_kv_heads >= 1 && num_heads % cache->num_kv_heads == 0,
+               "paged_prefill4: num_heads %d not a multiple of num_kv_heads %d", num_heads, cache->num_kv_heads);
+  if (batch == 0 || total_q == 0) return B200ASR_OK;
+  B200_REQUIRE(q && out && cu_seqlens_q && cu_seqlens_k && (block_tables || bt_width == 0) && cache->k_codes &&
+                   cache->v_codes && cache->params,
+               "paged_prefill4: null pointer");
+  B200_REQUIRE(kv4_cache_ok(*cache), "paged_prefill4: cache sizes, or rows not 16-byte (codes) and "
+               "8-byte (parameters) aligned");
+  B200_REQUIRE(aligned16(q) && aligned16(out) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0 &&
+                   out_row_stride % 8 == 0 && out_head_stride % 8 == 0,
+               "paged_prefill4: q and out rows must be 16-byte aligned");
+  Prefill4Args a{};
+  a.q = static_cast<const __nv_bfloat16 *>(q);
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.c = *cache;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.block_tables = block_tables;
+  a.bt_stride = bt_stride;
+  a.bt_width = bt_width;
+  a.batch = batch;
+  a.total_q = total_q;
+  a.group = num_heads / cache->num_kv_heads;
+  const int bs = cache->block_size;
+  a.bs_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
+  a.scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
+  a.flip = scale < 0 ? 0x80008000u : 0u;
+  a.out = static_cast<__nv_bfloat16 *>(out);
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  a.error_flag = error_flag;
+  return D == 128 ? launch_prefill4<128>(a, total_q, static_cast<cudaStream_t>(stream))
+                  : launch_prefill4<64>(a, total_q, static_cast<cudaStream_t>(stream));
+}

@@ -486,6 +486,27 @@ def paged_decode4(q, k_codes, v_codes, kv_params, cu_seqlens_k, block_tables, *,
     return out
 
 
+def paged_prefill4(q, k_codes, v_codes, kv_params, cu_seqlens_q, cu_seqlens_k, block_tables, *,
+                   max_seqlen_q: int, max_seqlen_k: int, scale: float, out,
+                   error_flag=None) -> torch.Tensor:
+    """:func:`paged_prefill` over a 4-bit cache: varlen causal attention (the mask aligned
+    bottom-right) of q [total_q, H, D], H any multiple of H_kv, D 64 or 128; a row that sees
+    no key gives zeros."""
+    what = "paged_prefill4"
+    cache = _kv4(what, k_codes, v_codes, kv_params)
+    _attention4_args(what, q, out, cu_seqlens_k, block_tables, cache)
+    _need(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous()
+          and cu_seqlens_q.shape == cu_seqlens_k.shape, f"{what}: cu_seqlens_q like cu_seqlens_k")
+    _here(what, q, out, cu_seqlens_q, cu_seqlens_k, block_tables, error_flag)
+    _count()
+    check(lib.b200asr_paged_prefill4(
+        _p(q), q.stride(0), q.stride(1), ctypes.byref(cache), q.shape[1], _p(cu_seqlens_q),
+        _p(cu_seqlens_k), _p(block_tables), block_tables.stride(0), block_tables.shape[1],
+        cu_seqlens_k.shape[0] - 1, q.shape[0], float(scale), _p(out), out.stride(0), out.stride(1),
+        _p(error_flag), _stream()), what)
+    return out
+
+
 # ------------------------------------------------- rotary positions with several axes
 
 

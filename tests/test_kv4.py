@@ -5,7 +5,7 @@ Tolerances of the attention outputs are element by element, from the roundings t
 * the output to bf16: 2^-8 of its value;
 * a probability times its V scale to bf16 before the product with the centred code (code - 8):
   2^-8 of sum_t p_t vs_t |code_t - 8|;
-* the score's 32-bit accumulation, whose terms are up to (128 + 15) |q_i| for at most
+* the score's 32-bit accumulation, whose terms are up to (1024 + 15) |q_i| for at most
   D / 16 + 1 additions of 2^-23 each: an absolute error e of the score (base e) changes each
   probability by the factor exp(+-e), so the output by at most 2 e sum_t p_t |v_t - out|
   <= 2 e (sum_t p_t |v_t| + |out|);
@@ -99,7 +99,7 @@ def plain_attention(q, cache, table, n, scale, prefill=False):
                 moved = (p * e) @ np.abs(v[:seen, g]) + (p @ e) * np.abs(o)  # exp(x) - 1 <= x exp(x)
                 moved = moved * np.exp(e.max())
             else:
-                e = abs(scale) * ks[:seen, g].max() * 143 * np.abs(q[i, h]).sum() * (d / 16 + 1) * 2.0 ** -23
+                e = abs(scale) * ks[:seen, g].max() * 1040 * np.abs(q[i, h]).sum() * (d / 16 + 1) * 2.0 ** -23
                 rounded = 2.0 ** -8 * (p @ (vs[:seen, g] * np.abs(vcode[:seen, g] - 8)))
                 moved = 2 * e * (mass + np.abs(o))
             out[i, h] = o

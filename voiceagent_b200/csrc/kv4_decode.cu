@@ -4,19 +4,20 @@
 //   out[b, h] = softmax(q[b, h] K_b^T * scale) V_b,
 // with a row's codes c and parameters (scale, zero):
 //   score_t = ks_t (q . c_t) + kz_t sum(q),     out = (sum_t (p_t vs_t) c'_t + sum_t p_t vz_t) / sum_t p_t.
-// Codes go through the tensor cores as bf16 whole numbers, exact in bf16: q . c needs no
-// dequantised K, and the V scale goes into the probability before its rounding to bf16
+// Codes go through the tensor cores as whole numbers, exact there: q . c needs no dequantised K, and the V scale goes into the probability before its rounding to bf16
 // (which the bf16 form of this kernel rounds as well). Everything else is held in 32 bits.
 //
 // What bounds it: at 136 bytes per cached (token, KV head) of D = 128 the bytes are a quarter
 // of the bf16 cache's, and turning codes into MMA operands costs ~240 instructions per 16
 // tokens, ~65 % of the SM's issue slots at the copy rate of HBM; so instructions are counted:
 //  * MMA m16n8k16 with cached tokens (scores) or dims (output) as its 16 rows and the group's
-//    query heads as its 8 columns. A word of 8 codes becomes four bf16 pairs by
-//    (w >> 4 i) & 0x000f000f | 0x43004300, each 128 + code. For K the 128 is taken off by
-//    the accumulator's start value -128 sum(q); for V, whose accumulator runs over the whole
-//    context, the pair is lowered by 136 to code - 8, small and centred, and the zero moves up
-//    by 8 steps.
+//    query heads as its 8 columns. Scores in fp16: a word of 8 codes becomes four pairs by a mask
+//    and an or, each 1024 + code or, in place, 1024 + 16 code (its q is a sixteenth), so a word
+//    needs one shift; the offsets are taken off by the accumulator's start value. q is
+//    brought to fp16 by a power of two per query head, undone in the score's factor: exact but
+//    for what is 2^-27 of the head's largest. Output in bf16, for the range of the V scales:
+//    pairs of 128 + code, lowered by 136 to code - 8, small and centred (the accumulator runs
+//    over the whole context), and the zero moves up by 8 steps.
 //  * The rows' dims are assigned to lanes so that a lane's codes are contiguous bytes: 16 of a
 //    K row, 8 of a V row.
 //  * A warp keeps its own ring of cp.async stages (32 tokens each) and its own softmax state:
@@ -26,6 +27,8 @@
 // end to end and divided evenly among the CTAs whatever the length mix. A pair that several
 // CTAs share leaves fp32 partials in the workspace, and a second kernel joins them in token
 // order (the result does not depend on timing). Nothing in the workspace outlives the call.
+#include <cuda_fp16.h>
+
 #include "kv4.cuh"
 
 namespace b200asr {
@@ -130,12 +133,27 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t movm_trans(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
+// Codes 0 and 4 of a word as the fp16 pair 1024 + code, codes 1 and 5 as 1024 + 16 code.
+__device__ __forceinline__ uint32_t code_low(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }
+__device__ __forceinline__ uint32_t code_high(uint32_t w) { return (w & 0x00f000f0u) | 0x64006400u; }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
 // Codes i and i + 4 of a word (or i of two words' halves) as the bf16 pair 128 + code.
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
   return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
@@ -271,29 +289,51 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
     const int j = a.bs_shift >= 0 ? tok >> a.bs_shift : tok / a.c.block_size;
     return a.block_tables[c.b * a.bt_stride + j];
   };
+  // Blocks of whole stages: a stage's rows lie at one base with the slots' stride, and only the
+  // sequence's last stage needs a check per row.
+  const bool even_blocks = a.bs_shift >= 5;
+  const int lane_row = lane / C::CHUNKS, lane_ch = lane % C::CHUNKS;
+  const int64_t lane_off = lane_row * a.c.code_stride[1] + lane_ch * 16;
+  const int64_t round_off = (32 / C::CHUNKS) * a.c.code_stride[1];
   auto issue = [&](const Cursor4 &c, int block, int stage) {
     const int tok = token_of(c);
-    const int valid = tok < c.len;
-    const int at = a.bs_shift >= 0 ? tok & (a.c.block_size - 1) : tok % a.c.block_size;
+    const bool valid = tok < c.len;
     if (valid && (block < 0 || block >= a.c.num_blocks)) {
       raise_flag(a.error_flag, B200ASR_DEVERR_BLOCK);
       block = 0;
     }
-    if (!valid) block = 0;
     const int h = c.p / a.subs;
+    const uint32_t ks = ring_s + stage * C::STAGE, vs = ks + kD4Tile * C::ROW, ps = vs + kD4Tile * C::ROW;
+    if (even_blocks && tok - lane + kD4Tile <= c.len) {
+      const int at = tok & (a.c.block_size - 1);
+      const int64_t off = block * a.c.code_stride[0] + (at - lane) * a.c.code_stride[1] +
+                          h * a.c.code_stride[2] + lane_off;
+      const uint8_t *kp = static_cast<const uint8_t *>(a.c.k_codes) + off;
+      const uint8_t *vp = static_cast<const uint8_t *>(a.c.v_codes) + off;
+      cp_async8(ps + lane * 8, static_cast<const __nv_bfloat16 *>(a.c.params) + block * a.c.param_stride[0] +
+                                   at * a.c.param_stride[1] + h * a.c.param_stride[2], true);
+#pragma unroll
+      for (int i = 0; i < C::CHUNKS; ++i) {
+        const int row = i * (32 / C::CHUNKS) + lane_row;
+        cp_async16(ks + row * C::ROW + lane_ch * 16, kp + i * round_off, true);
+        cp_async16(vs + v_place<D>(row) * C::ROW + (lane_ch ^ v_swap<D>(row)) * 16, vp + i * round_off, true);
+      }
+      return;
+    }
+    const int at = a.bs_shift >= 0 ? tok & (a.c.block_size - 1) : tok % a.c.block_size;
+    if (!valid) block = 0;
     const int64_t off = block * a.c.code_stride[0] + (valid ? at : 0) * a.c.code_stride[1] +
                         h * a.c.code_stride[2];
     const int64_t poff = block * a.c.param_stride[0] + (valid ? at : 0) * a.c.param_stride[1] +
                          h * a.c.param_stride[2];
-    const uint32_t ks = ring_s + stage * C::STAGE, vs = ks + kD4Tile * C::ROW, ps = vs + kD4Tile * C::ROW;
     cp_async8(ps + lane * 8, static_cast<const __nv_bfloat16 *>(a.c.params) + poff, valid);
 #pragma unroll
     for (int i = 0; i < C::CHUNKS; ++i) {
-      const int id = i * 32 + lane, row = id / C::CHUNKS, ch = id % C::CHUNKS;
-      const int64_t o = __shfl_sync(0xffffffffu, off, row) + ch * 16;
-      const bool ok = __shfl_sync(0xffffffffu, valid, row) != 0;
-      cp_async16(ks + row * C::ROW + ch * 16, static_cast<const uint8_t *>(a.c.k_codes) + o, ok);
-      cp_async16(vs + v_place<D>(row) * C::ROW + (ch ^ v_swap<D>(row)) * 16,
+      const int row = i * (32 / C::CHUNKS) + lane_row;
+      const int64_t o = __shfl_sync(0xffffffffu, off, row) + lane_ch * 16;
+      const bool ok = __shfl_sync(0xffffffffu, static_cast<int>(valid), row) != 0;
+      cp_async16(ks + row * C::ROW + lane_ch * 16, static_cast<const uint8_t *>(a.c.k_codes) + o, ok);
+      cp_async16(vs + v_place<D>(row) * C::ROW + (lane_ch ^ v_swap<D>(row)) * 16,
                  static_cast<const uint8_t *>(a.c.v_codes) + o, ok);
     }
   };
@@ -325,28 +365,55 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
     // q as the MMA's column operand, in the lane order of the codes: word j of a lane holds
     // dims 32 t + 8 j (D = 128) or 16 t + 8 j (D = 64) and up
     uint32_t qf[NT][KS][2];
-    float qs0[NT], qs1[NT];
+    float c0[NT], c1[NT];    // the accumulator's start: what the offsets of the codes add up to
+    float qs0[NT], qs1[NT];  // sum(q) of columns 2t and 2t + 1, times scale and log2(e)
+    float qx0[NT], qx1[NT];  // scale, log2(e) and the power of two of those columns
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float sum = 0.f;
+      uint4 u[KW];
+      float top = 0.f;
 #pragma unroll
       for (int j = 0; j < KW; ++j) {
-        uint4 u = make_uint4(0, 0, 0, 0);
+        u[j] = make_uint4(0, 0, 0, 0);
         if (n * 8 + g < cols)
-          u = *reinterpret_cast<const uint4 *>(qp + (n * 8 + g) * a.q_head + t * (D / 4) + j * 8);
+          u[j] = *reinterpret_cast<const uint4 *>(qp + (n * 8 + g) * a.q_head + t * (D / 4) + j * 8);
         float f[8];
-        unpack8(u, f);
+        unpack8(u[j], f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += f[e];
-        qf[n][2 * j][0] = __byte_perm(u.x, u.z, 0x5410);
-        qf[n][2 * j][1] = __byte_perm(u.x, u.z, 0x7632);
-        qf[n][2 * j + 1][0] = __byte_perm(u.y, u.w, 0x5410);
-        qf[n][2 * j + 1][1] = __byte_perm(u.y, u.w, 0x7632);
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      qs0[n] = __shfl_sync(0xffffffffu, sum, 8 * t);      // column 2t: lanes with g = 2t
-      qs1[n] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);  // column 2t + 1
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^x with the largest |q| 2^x in [2^13, 2^14); a row of zeros or beyond takes what it gets
+      const int ex = min(100, max(-114, 13 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
+      const float up = __int_as_float((ex + 127) << 23);
+      float even = 0.f, odd = 0.f;
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        float f[8];
+        unpack8(u[j], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= up;
+        even += (f[0] + f[4]) + (f[2] + f[6]);
+        odd += (f[1] + f[5]) + (f[3] + f[7]);
+        qf[n][2 * j][0] = pack_f16(f[0], f[4]);
+        qf[n][2 * j][1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
+        qf[n][2 * j + 1][0] = pack_f16(f[2], f[6]);
+        qf[n][2 * j + 1][1] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
+      }
+      even += __shfl_xor_sync(0xffffffffu, even, 1);
+      odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+      even += __shfl_xor_sync(0xffffffffu, even, 2);
+      odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+      const float start = -1024.f * even - 64.f * odd;
+      const float factor = a.scale_log2 * __int_as_float((127 - ex) << 23);
+      const float sum = (even + odd) * factor;
+      c0[n] = __shfl_sync(0xffffffffu, start, 8 * t);  // column 2t: lanes with g = 2t
+      c1[n] = __shfl_sync(0xffffffffu, start, 8 * t + 4);
+      qs0[n] = __shfl_sync(0xffffffffu, sum, 8 * t);
+      qs1[n] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      qx0[n] = __shfl_sync(0xffffffffu, factor, 8 * t);
+      qx1[n] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
     }
     float o[NT][KS][4], m0[NT], m1[NT], l0[NT], l1[NT], z0[NT], z1[NT];
 #pragma unroll
@@ -388,28 +455,26 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
         float acc[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          acc[n][0] = acc[n][2] = -128.f * qs0[n];
-          acc[n][1] = acc[n][3] = -128.f * qs1[n];
+          acc[n][0] = acc[n][2] = c0[n];
+          acc[n][1] = acc[n][3] = c1[n];
         }
 #pragma unroll
         for (int j = 0; j < KW; ++j)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t a0 = code_pair(ka[j], 2 * half), a2 = code_pair(ka[j], 2 * half + 1);
-            const uint32_t a1 = code_pair(kb[j], 2 * half), a3 = code_pair(kb[j], 2 * half + 1);
+            const uint32_t x = half ? ka[j] >> 8 : ka[j], y = half ? kb[j] >> 8 : kb[j];
+            const uint32_t a0 = code_low(x), a2 = code_high(x), a1 = code_low(y), a3 = code_high(y);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-              mma_bf16(acc[n], a0, a1, a2, a3, qf[n][2 * j + half][0], qf[n][2 * j + half][1]);
+              mma_f16(acc[n], a0, a1, a2, a3, qf[n][2 * j + half][0], qf[n][2 * j + half][1]);
           }
         const float2 kpa = unpack2(pa.x), kpb = unpack2(pb.x);
-        const float sa = kpa.x * a.scale_log2, za = kpa.y * a.scale_log2;
-        const float sb = kpb.x * a.scale_log2, zb = kpb.y * a.scale_log2;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          s[n][mt][0] = fmaf(sa, acc[n][0], za * qs0[n]);
-          s[n][mt][1] = fmaf(sa, acc[n][1], za * qs1[n]);
-          s[n][mt][2] = fmaf(sb, acc[n][2], zb * qs0[n]);
-          s[n][mt][3] = fmaf(sb, acc[n][3], zb * qs1[n]);
+          s[n][mt][0] = fmaf(kpa.x * qx0[n], acc[n][0], kpa.y * qs0[n]);
+          s[n][mt][1] = fmaf(kpa.x * qx1[n], acc[n][1], kpa.y * qs1[n]);
+          s[n][mt][2] = fmaf(kpb.x * qx0[n], acc[n][2], kpb.y * qs0[n]);
+          s[n][mt][3] = fmaf(kpb.x * qx1[n], acc[n][3], kpb.y * qs1[n]);
         }
       }
       if (left < kD4Tile) {  // the sequence ends in this stage

@@ -43,6 +43,8 @@
 // No TMA multicast is used. Every CTA takes part in the one (split) cluster barrier and
 // pushes all its bytes whatever happens (a timed-out wait only skips work and raises the
 // flag), so no CTA waits for one that left.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace b200asr {
@@ -986,13 +988,19 @@ int launch_linear(const void *x, int64_t x_stride, int m, int k, const void *w, 
   // Halve a split whose cluster cannot be resident (16 CTAs is a non-portable size). The
   // RMSNorm prologue needs the whole K slice in the ring, so it cannot go below that.
   const int min_split = NORM_IN ? (k / kLnBK + kLnStages - 1) / kLnStages : 1;
+  // (the answer depends on the kernel and the split alone: asked once, it costs microseconds)
+  static std::atomic<int> fits[kLnMaxSplit + 1];  // 0: not asked, 1: resident, 2: not
   while (a.k_split > 1) {
-    attr[0].val.clusterDim.x = a.k_split;
-    cfg.gridDim = dim3(tiles * a.k_split, 1, 1);
-    int clusters = 0;
-    if (cudaOccupancyMaxActiveClusters(&clusters, kfn, &cfg) == cudaSuccess && clusters > 0)
-      break;
-    cudaGetLastError();
+    int known = fits[a.k_split].load(std::memory_order_relaxed);
+    if (known == 0) {
+      attr[0].val.clusterDim.x = a.k_split;
+      cfg.gridDim = dim3(tiles * a.k_split, 1, 1);
+      int clusters = 0;
+      known = cudaOccupancyMaxActiveClusters(&clusters, kfn, &cfg) == cudaSuccess && clusters > 0 ? 1 : 2;
+      cudaGetLastError();
+      fits[a.k_split].store(known, std::memory_order_relaxed);
+    }
+    if (known == 1) break;
     if (a.k_split / 2 < min_split) {
       set_error("linear_small: a cluster of %d CTAs cannot be resident", a.k_split);
       return B200ASR_ERR_UNSUPPORTED;

@@ -9,10 +9,11 @@ CUDA stream. Nothing here allocates inside a captured region when the caller pas
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
-from voiceagent_b200._lib import Kv4, check, lib
+from voiceagent_b200._lib import check, lib
 
 BF16 = torch.bfloat16
 
@@ -36,9 +37,13 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream") and hasattr(torch._C, "_cuda_g
         Python and cost ~15 us per kernel call, which added up on the eager prefill and
         encode paths."""
         return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+    _device = torch._C._cuda_getDevice
 else:  # pragma: no cover - older torch
     def _stream():
         return torch.cuda.current_stream().cuda_stream
+
+    _device = torch.cuda.current_device
 
 
 def _need(cond: bool, msg: str) -> None:
@@ -371,86 +376,104 @@ def kv4_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int
             torch.zeros(*shape, 4, dtype=BF16, device=device))
 
 
+_U8, _I32 = torch.uint8, torch.int32
+_pack_kv4 = struct.Struct("@3P6q4i").pack  # a b200asr_kv4 (include/b200asr.h)
+
+
+def _bad(what: str, says: str):
+    raise ValueError(f"{what}: {says}")
+
+
 def _here(what: str, *tensors: torch.Tensor | None) -> None:
     """Every tensor on the current CUDA device: the launch goes to that device's stream."""
-    here = None
+    device = None
     for t in tensors:
         if t is None:
             continue
-        _need(t.is_cuda, f"{what}: b200asr kernels need CUDA tensors")
-        if here is None:
-            here = torch.cuda.current_device()
-        _need(t.get_device() == here, f"{what}: tensors on another device than the current one")
+        at = t.get_device()
+        if at < 0:
+            _bad(what, "b200asr kernels need CUDA tensors")
+        if device is None:
+            device = _device()
+        if at != device:
+            _bad(what, "tensors on another device than the current one")
 
 
-def _kv4(what: str, k_codes, v_codes, kv_params) -> Kv4:
-    """The cache as the C ABI takes it (strides of the first three axes are free)."""
-    _need(k_codes.dtype == torch.uint8 and v_codes.dtype == torch.uint8
-          and kv_params.dtype == BF16, f"{what}: uint8 codes and bf16 parameters")
-    _need(k_codes.dim() == 4 and k_codes.shape == v_codes.shape
-          and k_codes.stride() == v_codes.stride() and k_codes.stride(3) == 1,
-          f"{what}: codes [num_blocks, block_size, num_kv_heads, head_dim / 2], alike for K and V")
-    blocks, size, heads, row = k_codes.shape
-    _need(tuple(kv_params.shape) == (blocks, size, heads, 4) and kv_params.stride(3) == 1,
-          f"{what}: parameters [num_blocks, block_size, num_kv_heads, 4]")
-    _here(what, k_codes, v_codes, kv_params)
-    cs, ps = k_codes.stride(), kv_params.stride()
-    return Kv4(k_codes.data_ptr(), v_codes.data_ptr(), kv_params.data_ptr(), cs[:3], ps[:3], blocks,
-               size, heads, 2 * row)
+def _kv4(what: str, k_codes, v_codes, kv_params):
+    """The cache as the C ABI takes it (strides of the first three axes are free), its KV heads
+    and its head size."""
+    if k_codes.dtype is not _U8 or v_codes.dtype is not _U8 or kv_params.dtype is not BF16:
+        _bad(what, "uint8 codes and bf16 parameters")
+    shape, cs, ps = k_codes.shape, k_codes.stride(), kv_params.stride()
+    if len(shape) != 4 or v_codes.shape != shape or v_codes.stride() != cs or cs[3] != 1:
+        _bad(what, "codes [num_blocks, block_size, num_kv_heads, head_dim / 2], alike for K and V")
+    blocks, size, heads, row = shape
+    if kv_params.shape != (blocks, size, heads, 4) or ps[3] != 1:
+        _bad(what, "parameters [num_blocks, block_size, num_kv_heads, 4]")
+    return (_pack_kv4(k_codes.data_ptr(), v_codes.data_ptr(), kv_params.data_ptr(), cs[0], cs[1], cs[2],
+                      ps[0], ps[1], ps[2], blocks, size, heads, 2 * row), heads, 2 * row)
 
 
 def store_kvcache4(key, value, k_codes, v_codes, kv_params, slot_mapping, error_flag=None) -> None:
     """:func:`store_kvcache` into a 4-bit cache: key/value bf16 [T, H_kv, D] (free token and
     head strides), slot_mapping int32 [T], -1 skips; no slot twice."""
     what = "store_kvcache4"
-    cache = _kv4(what, k_codes, v_codes, kv_params)
-    _need(key.dtype == BF16 and value.dtype == BF16 and key.dim() == 3
-          and key.shape[1:] == (cache.num_kv_heads, cache.head_dim) and value.shape == key.shape
-          and key.stride(2) == 1 and value.stride(2) == 1,
-          f"{what}: key/value bf16 [T, num_kv_heads, head_dim] with contiguous rows")
-    _need(slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous()
-          and slot_mapping.shape == key.shape[:1], f"{what}: int32 slots, one per token")
-    _here(what, key, value, slot_mapping, error_flag)
+    cache, heads, dim = _kv4(what, k_codes, v_codes, kv_params)
+    shape, ks, vs = key.shape, key.stride(), value.stride()
+    if (key.dtype is not BF16 or value.dtype is not BF16 or len(shape) != 3 or shape[1] != heads
+            or shape[2] != dim or value.shape != shape or ks[2] != 1 or vs[2] != 1):
+        _bad(what, "key/value bf16 [T, num_kv_heads, head_dim] with contiguous rows")
+    if (slot_mapping.dtype is not _I32 or slot_mapping.shape != shape[:1]
+            or not slot_mapping.is_contiguous()):
+        _bad(what, "int32 slots, one per token")
+    _here(what, k_codes, v_codes, kv_params, key, value, slot_mapping, error_flag)
     _count()
     check(lib.b200asr_store_kvcache4(
-        _p(key), key.stride(0), key.stride(1), _p(value), value.stride(0), value.stride(1),
-        ctypes.byref(cache), _p(slot_mapping), key.shape[0], _p(error_flag), _stream()), what)
+        key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], cache, slot_mapping.data_ptr(),
+        shape[0], _p(error_flag), _stream()), what)
 
 
 def load_kvcache4(k_codes, v_codes, kv_params, slots, key=None, value=None, error_flag=None):
     """Rows of a 4-bit cache as bf16 ``(key, value)`` [T, H_kv, D]; slot -1 reads as zeros."""
     what = "load_kvcache4"
-    cache = _kv4(what, k_codes, v_codes, kv_params)
-    _need(slots.dtype == torch.int32 and slots.dim() == 1 and slots.is_contiguous(),
-          f"{what}: int32 slots [T]")
-    shape = (slots.shape[0], cache.num_kv_heads, cache.head_dim)
-    key = torch.empty(shape, dtype=BF16, device=slots.device) if key is None else key
-    value = torch.empty(shape, dtype=BF16, device=slots.device) if value is None else value
-    for x in (key, value):
-        _need(x.dtype == BF16 and tuple(x.shape) == shape and x.stride(2) == 1,
-              f"{what}: key/value bf16 [T, num_kv_heads, head_dim] with contiguous rows")
-    _here(what, slots, key, value, error_flag)
+    cache, heads, dim = _kv4(what, k_codes, v_codes, kv_params)
+    if slots.dtype is not _I32 or slots.dim() != 1 or not slots.is_contiguous():
+        _bad(what, "int32 slots [T]")
+    shape = (slots.shape[0], heads, dim)
+    if key is None:
+        key = torch.empty(shape, dtype=BF16, device=slots.device)
+    if value is None:
+        value = torch.empty(shape, dtype=BF16, device=slots.device)
+    ks, vs = key.stride(), value.stride()
+    if (key.dtype is not BF16 or value.dtype is not BF16 or key.shape != shape
+            or value.shape != shape or ks[2] != 1 or vs[2] != 1):
+        _bad(what, "key/value bf16 [T, num_kv_heads, head_dim] with contiguous rows")
+    _here(what, k_codes, v_codes, kv_params, slots, key, value, error_flag)
     _count()
     check(lib.b200asr_load_kvcache4(
-        ctypes.byref(cache), _p(slots), shape[0], _p(key), key.stride(0), key.stride(1), _p(value),
-        value.stride(0), value.stride(1), _p(error_flag), _stream()), what)
+        cache, slots.data_ptr(), shape[0], key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1],
+        _p(error_flag), _stream()), what)
     return key, value
 
 
-def _attention4_args(what: str, q, out, cu_seqlens_k, block_tables, cache: Kv4) -> None:
-    _need(q.dtype == BF16 and q.dim() == 3 and q.shape[2] == cache.head_dim and q.stride(2) == 1
-          and q.shape[1] % cache.num_kv_heads == 0,
-          f"{what}: q bf16 [rows, num_heads, head_dim] with contiguous rows, num_heads a multiple "
-          "of num_kv_heads")
-    _need(out.dtype == BF16 and out.shape == q.shape and out.stride(2) == 1,
-          f"{what}: out like q")
-    _need(block_tables.dtype == torch.int32 and cu_seqlens_k.dtype == torch.int32,
-          f"{what}: int32 metadata")
-    _need(cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous() and cu_seqlens_k.shape[0] >= 1,
-          f"{what}: cu_seqlens_k [batch + 1]")
-    _need(block_tables.dim() == 2 and block_tables.shape[0] >= cu_seqlens_k.shape[0] - 1
-          and (block_tables.stride(1) == 1 or block_tables.shape[1] <= 1),
-          f"{what}: block_tables [batch, blocks] with contiguous rows")
+def _attention4_args(what: str, q, out, cu_seqlens_k, block_tables, heads: int, dim: int):
+    """Checks shared by decode and prefill; strides of q and out, batch, strides and width of the
+    tables."""
+    shape, qs, os, bs = q.shape, q.stride(), out.stride(), block_tables.stride()
+    if q.dtype is not BF16 or len(shape) != 3 or shape[2] != dim or qs[2] != 1 or shape[1] % heads:
+        _bad(what, "q bf16 [rows, num_heads, head_dim] with contiguous rows, num_heads a multiple "
+                   "of num_kv_heads")
+    if out.dtype is not BF16 or out.shape != shape or os[2] != 1:
+        _bad(what, "out like q")
+    if block_tables.dtype is not _I32 or cu_seqlens_k.dtype is not _I32:
+        _bad(what, "int32 metadata")
+    starts = cu_seqlens_k.shape
+    if len(starts) != 1 or starts[0] < 1 or not cu_seqlens_k.is_contiguous():
+        _bad(what, "cu_seqlens_k [batch + 1]")
+    batch, table = starts[0] - 1, block_tables.shape
+    if len(table) != 2 or table[0] < batch or (bs[1] != 1 and table[1] > 1):
+        _bad(what, "block_tables [batch, blocks] with contiguous rows")
+    return qs, os, batch, bs[0], table[1]
 
 
 def paged_decode4_workspace_size(max_seqlen_k: int, num_heads: int, num_kv_heads: int,
@@ -467,22 +490,25 @@ def paged_decode4(q, k_codes, v_codes, kv_params, cu_seqlens_k, block_tables, *,
     ``workspace`` (uint8, :func:`paged_decode4_workspace_size` bytes, any contents, one call at
     a time) is taken from the caching allocator when not given."""
     what = "paged_decode4"
-    cache = _kv4(what, k_codes, v_codes, kv_params)
-    _attention4_args(what, q, out, cu_seqlens_k, block_tables, cache)
-    batch = cu_seqlens_k.shape[0] - 1
-    _need(batch <= q.shape[0], f"{what}: cu_seqlens_k longer than the batch")
-    if workspace is None:
-        need = paged_decode4_workspace_size(max_seqlen_k, q.shape[1], cache.num_kv_heads,
-                                            cache.head_dim)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _here(what, q, out, cu_seqlens_k, block_tables, workspace, error_flag)
+    cache, heads, dim = _kv4(what, k_codes, v_codes, kv_params)
+    qs, os, batch, bt_stride, bt_width = _attention4_args(what, q, out, cu_seqlens_k, block_tables,
+                                                          heads, dim)
+    rows, q_heads, _ = q.shape
+    if batch > rows:
+        _bad(what, "cu_seqlens_k longer than the batch")
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif max_seqlen_k > DECODE_SHORT_CTX:
+        ws_bytes = lib.b200asr_paged_decode4_workspace_size(max_seqlen_k, q_heads, heads, dim)
+        workspace = torch.empty(ws_bytes, dtype=_U8, device=q.device)
+        ws = workspace.data_ptr()
+    _here(what, k_codes, v_codes, kv_params, q, out, cu_seqlens_k, block_tables, workspace, error_flag)
     _count(1 if max_seqlen_k <= DECODE_SHORT_CTX else 2)  # + the join of split contexts
     check(lib.b200asr_paged_decode4(
-        _p(q), q.stride(0), q.stride(1), ctypes.byref(cache), q.shape[1], _p(cu_seqlens_k),
-        _p(block_tables), block_tables.stride(0), block_tables.shape[1], batch, max_seqlen_k,
-        float(scale), _p(out), out.stride(0), out.stride(1), _p(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), _p(error_flag),
-        _stream()), what)
+        q.data_ptr(), qs[0], qs[1], cache, q_heads, cu_seqlens_k.data_ptr(), block_tables.data_ptr(),
+        bt_stride, bt_width, batch, max_seqlen_k, scale, out.data_ptr(), os[0], os[1], ws, ws_bytes,
+        _p(error_flag), _stream()), what)
     return out
 
 
@@ -493,16 +519,19 @@ def paged_prefill4(q, k_codes, v_codes, kv_params, cu_seqlens_q, cu_seqlens_k, b
     bottom-right) of q [total_q, H, D], H any multiple of H_kv, D 64 or 128; a row that sees
     no key gives zeros."""
     what = "paged_prefill4"
-    cache = _kv4(what, k_codes, v_codes, kv_params)
-    _attention4_args(what, q, out, cu_seqlens_k, block_tables, cache)
-    _need(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous()
-          and cu_seqlens_q.shape == cu_seqlens_k.shape, f"{what}: cu_seqlens_q like cu_seqlens_k")
-    _here(what, q, out, cu_seqlens_q, cu_seqlens_k, block_tables, error_flag)
+    cache, heads, dim = _kv4(what, k_codes, v_codes, kv_params)
+    qs, os, batch, bt_stride, bt_width = _attention4_args(what, q, out, cu_seqlens_k, block_tables,
+                                                          heads, dim)
+    if (cu_seqlens_q.dtype is not _I32 or cu_seqlens_q.shape != cu_seqlens_k.shape
+            or not cu_seqlens_q.is_contiguous()):
+        _bad(what, "cu_seqlens_q like cu_seqlens_k")
+    rows, q_heads, _ = q.shape
+    _here(what, k_codes, v_codes, kv_params, q, out, cu_seqlens_q, cu_seqlens_k, block_tables,
+          error_flag)
     _count()
     check(lib.b200asr_paged_prefill4(
-        _p(q), q.stride(0), q.stride(1), ctypes.byref(cache), q.shape[1], _p(cu_seqlens_q),
-        _p(cu_seqlens_k), _p(block_tables), block_tables.stride(0), block_tables.shape[1],
-        cu_seqlens_k.shape[0] - 1, q.shape[0], float(scale), _p(out), out.stride(0), out.stride(1),
+        q.data_ptr(), qs[0], qs[1], cache, q_heads, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+        block_tables.data_ptr(), bt_stride, bt_width, batch, rows, scale, out.data_ptr(), os[0], os[1],
         _p(error_flag), _stream()), what)
     return out
 
@@ -536,48 +565,51 @@ def qk_norm_mrope_store(qkv, positions, freq_axis, *, num_heads: int, num_kv_hea
     ``v_cache``) or a 4-bit one (``k_codes``, ``v_codes``, ``kv_params``); returns q_out
     [T, num_heads, head_dim]."""
     what = "qk_norm_mrope_store"
-    tokens = qkv.shape[0]
-    _need(qkv.dtype == BF16 and qkv.dim() == 2 and qkv.stride(1) == 1
-          and qkv.shape[1] == (num_heads + 2 * num_kv_heads) * head_dim,
-          f"{what}: qkv bf16 [T, (num_heads + 2 num_kv_heads) head_dim] with contiguous rows")
-    _need(positions.dtype == torch.int64 and positions.dim() == 2 and positions.shape[1] == tokens
-          and (positions.stride(1) == 1 or tokens <= 1), f"{what}: positions int64 [axes, T]")
-    _need(freq_axis.dtype == torch.int32 and freq_axis.is_contiguous()
-          and freq_axis.numel() == head_dim // 2, f"{what}: freq_axis int32 [head_dim / 2]")
-    _need(q_weight.dtype == BF16 and k_weight.dtype == BF16 and q_weight.is_contiguous()
-          and k_weight.is_contiguous() and q_weight.numel() == k_weight.numel() == head_dim,
-          f"{what}: norm weights bf16 [head_dim]")
-    _need(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.is_contiguous()
-          and cos_sin_cache.shape[-1] == head_dim, f"{what}: fp32 rope table [positions, head_dim]")
-    _need(q_out.dtype == BF16 and tuple(q_out.shape) == (tokens, num_heads, head_dim)
-          and q_out.stride(2) == 1 and (q_out.stride(1) == head_dim or num_heads == 1),
-          f"{what}: q_out bf16 [T, num_heads, head_dim]")
+    (tokens, width), qkv_s, pos_s, out_s = qkv.shape, qkv.stride(), positions.stride(), q_out.stride()
+    if qkv.dtype is not BF16 or qkv_s[1] != 1 or width != (num_heads + 2 * num_kv_heads) * head_dim:
+        _bad(what, "qkv bf16 [T, (num_heads + 2 num_kv_heads) head_dim] with contiguous rows")
+    if (positions.dtype is not torch.int64 or positions.dim() != 2 or positions.shape[1] != tokens
+            or (pos_s[1] != 1 and tokens > 1)):
+        _bad(what, "positions int64 [axes, T]")
+    if freq_axis.dtype is not _I32 or freq_axis.numel() != head_dim // 2 or not freq_axis.is_contiguous():
+        _bad(what, "freq_axis int32 [head_dim / 2]")
+    if (q_weight.dtype is not BF16 or k_weight.dtype is not BF16 or q_weight.numel() != head_dim
+            or k_weight.numel() != head_dim or not q_weight.is_contiguous()
+            or not k_weight.is_contiguous()):
+        _bad(what, "norm weights bf16 [head_dim]")
+    if (cos_sin_cache.dtype is not torch.float32 or cos_sin_cache.shape[-1] != head_dim
+            or not cos_sin_cache.is_contiguous()):
+        _bad(what, "fp32 rope table [positions, head_dim]")
+    if (q_out.dtype is not BF16 or q_out.shape != (tokens, num_heads, head_dim) or out_s[2] != 1
+            or (out_s[1] != head_dim and num_heads > 1)):
+        _bad(what, "q_out bf16 [T, num_heads, head_dim]")
     num_slots, cache4 = 0, None
     if slot_mapping is not None:
-        _need(slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous()
-              and slot_mapping.numel() == tokens, f"{what}: int32 slots, one per token")
-        _need((k_cache is None) != (k_codes is None),
-              f"{what}: slot_mapping needs a bf16 cache or a 4-bit one")
+        if slot_mapping.dtype is not _I32 or slot_mapping.numel() != tokens or not slot_mapping.is_contiguous():
+            _bad(what, "int32 slots, one per token")
+        if (k_cache is None) == (k_codes is None):
+            _bad(what, "slot_mapping needs a bf16 cache or a 4-bit one")
         if k_codes is not None:
-            cache4 = _kv4(what, k_codes, v_codes, kv_params)
-            _need(cache4.num_kv_heads == num_kv_heads and cache4.head_dim == head_dim,
-                  f"{what}: the 4-bit cache has other heads")
+            cache4, heads4, dim4 = _kv4(what, k_codes, v_codes, kv_params)
+            if heads4 != num_kv_heads or dim4 != head_dim:
+                _bad(what, "the 4-bit cache has other heads")
         else:
             for c in (k_cache, v_cache):
-                _need(c is not None and c.dtype == BF16 and c.is_contiguous()
-                      and tuple(c.shape[-2:]) == (num_kv_heads, head_dim)
-                      and c.numel() == k_cache.numel(),
-                      f"{what}: contiguous bf16 caches [..., num_kv_heads, head_dim]")
+                if (c is None or c.dtype is not BF16 or c.shape[-2:] != (num_kv_heads, head_dim)
+                        or c.numel() != k_cache.numel() or not c.is_contiguous()):
+                    _bad(what, "contiguous bf16 caches [..., num_kv_heads, head_dim]")
             num_slots = k_cache.numel() // (num_kv_heads * head_dim)
+    else:
+        k_cache = v_cache = None
     _here(what, qkv, positions, freq_axis, q_weight, k_weight, cos_sin_cache, q_out, slot_mapping,
-          k_cache, v_cache, error_flag)
+          k_cache, v_cache, k_codes, v_codes, kv_params, error_flag)
     _count()
     check(lib.b200asr_qk_norm_mrope_store(
-        _p(qkv), qkv.stride(0), _p(positions), positions.stride(0), positions.shape[0], _p(freq_axis),
-        tokens, num_heads, num_kv_heads, head_dim, _p(q_weight), _p(k_weight), float(eps),
-        _p(cos_sin_cache), cos_sin_cache.shape[0], _p(q_out), q_out.stride(0), _p(slot_mapping),
-        _p(k_cache) if cache4 is None else None, _p(v_cache) if cache4 is None else None, num_slots,
-        None if cache4 is None else ctypes.byref(cache4), _p(error_flag), _stream()), what)
+        qkv.data_ptr(), qkv_s[0], positions.data_ptr(), pos_s[0], positions.shape[0],
+        freq_axis.data_ptr(), tokens, num_heads, num_kv_heads, head_dim, q_weight.data_ptr(),
+        k_weight.data_ptr(), eps, cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], q_out.data_ptr(),
+        out_s[0], _p(slot_mapping), _p(k_cache), _p(v_cache), num_slots, cache4, _p(error_flag),
+        _stream()), what)
     return q_out
 
 
@@ -675,45 +707,51 @@ def lora_linear(x, weight, lora_a, lora_b, scales, row_adapter, *, out=None,
     accumulator and one rounding; decode-size batches run on :func:`linear_small`'s kernel
     with the adapters in its epilogue."""
     what = "lora_linear"
-    _need(x.dtype == BF16 and x.dim() == 2 and x.stride(1) == 1, f"{what}: x bf16 [T, K] with contiguous rows")
-    _need(weight.dtype == BF16 and weight.dim() == 2 and weight.is_contiguous()
-          and weight.shape[1] == x.shape[1], f"{what}: weight bf16 [N, K]")
-    (m, k), n = x.shape, weight.shape[0]
-    _need(lora_a.dtype == BF16 and lora_a.dim() == 3 and lora_a.is_contiguous() and lora_a.shape[2] == k,
-          f"{what}: lora_a bf16 [adapters, rank, K]")
-    adapters, rank = lora_a.shape[:2]
-    _need(lora_b.dtype == BF16 and lora_b.is_contiguous() and tuple(lora_b.shape) == (adapters, n, rank),
-          f"{what}: lora_b bf16 [adapters, N, rank]")
-    _need(adapters >= 1 and 8 <= rank <= LORA_MAX_RANK and rank % 8 == 0,
-          f"{what}: rank a multiple of 8, at most {LORA_MAX_RANK}")
-    _need(k % 8 == 0 and n % 8 == 0 and k > 0 and n > 0 and x.stride(0) % 8 == 0,
-          f"{what}: K, N and the row stride of x multiples of 8")
-    _need(scales.dtype == torch.float32 and scales.is_contiguous() and scales.numel() == adapters,
-          f"{what}: fp32 scales, one per adapter")
-    _need(row_adapter.dtype == torch.int32 and row_adapter.is_contiguous() and row_adapter.numel() == m,
-          f"{what}: int32 row_adapter, one per row")
+    xs = x.stride()
+    if x.dtype is not BF16 or len(xs) != 2 or xs[1] != 1:
+        _bad(what, "x bf16 [T, K] with contiguous rows")
+    m, k = x.shape
+    if weight.dtype is not BF16 or weight.dim() != 2 or weight.shape[1] != k or not weight.is_contiguous():
+        _bad(what, "weight bf16 [N, K]")
+    n = weight.shape[0]
+    if lora_a.dtype is not BF16 or lora_a.dim() != 3 or lora_a.shape[2] != k or not lora_a.is_contiguous():
+        _bad(what, "lora_a bf16 [adapters, rank, K]")
+    adapters, rank, _ = lora_a.shape
+    if lora_b.dtype is not BF16 or lora_b.shape != (adapters, n, rank) or not lora_b.is_contiguous():
+        _bad(what, "lora_b bf16 [adapters, N, rank]")
+    if adapters < 1 or rank < 8 or rank > LORA_MAX_RANK or rank % 8:
+        _bad(what, f"rank a multiple of 8, at most {LORA_MAX_RANK}")
+    if k % 8 or n % 8 or k < 8 or n < 8 or xs[0] % 8:
+        _bad(what, "K, N and the row stride of x multiples of 8")
+    if scales.dtype is not torch.float32 or scales.numel() != adapters or not scales.is_contiguous():
+        _bad(what, "fp32 scales, one per adapter")
+    if row_adapter.dtype is not _I32 or row_adapter.numel() != m or not row_adapter.is_contiguous():
+        _bad(what, "int32 row_adapter, one per row")
     if out is None:
         out = torch.empty(m, n, dtype=BF16, device=x.device)
-    _need(out.dtype == BF16 and tuple(out.shape) == (m, n) and out.stride(1) == 1
-          and out.stride(0) % 8 == 0, f"{what}: out bf16 [T, N] with contiguous rows")
+    os = out.stride()
+    if out.dtype is not BF16 or out.shape != (m, n) or os[1] != 1 or os[0] % 8:
+        _bad(what, "out bf16 [T, N] with contiguous rows")
     _here(what, x, weight, lora_a, lora_b, scales, row_adapter, out, error_flag)
     if m == 0:
         return out
-    if linear_small_ok(x, weight):
+    err, stream = _p(error_flag), _stream()
+    _count(2)
+    if m <= LINEAR_SMALL_MAX_ROWS and k % 64 == 0 and n % 128 == 0:
         t = torch.empty(m, rank, dtype=torch.float32, device=x.device)
-        _count(2)
-        check(lib.b200asr_lora_down(_p(x), x.stride(0), m, k, _p(lora_a), adapters, rank, _p(scales),
-                                    _p(row_adapter), _p(t), _p(error_flag), _stream()), what)
-        check(lib.b200asr_linear_small_lora(_p(x), x.stride(0), m, k, _p(weight), n, _p(t), _p(lora_b),
-                                            adapters, rank, _p(row_adapter), _p(out), out.stride(0),
-                                            _p(error_flag), _stream()), what)
+        x_p, t_p, row_p = x.data_ptr(), t.data_ptr(), row_adapter.data_ptr()
+        check(lib.b200asr_lora_down(x_p, xs[0], m, k, lora_a.data_ptr(), adapters, rank,
+                                    scales.data_ptr(), row_p, t_p, err, stream), what)
+        check(lib.b200asr_linear_small_lora(x_p, xs[0], m, k, weight.data_ptr(), n, t_p,
+                                            lora_b.data_ptr(), adapters, rank, row_p, out.data_ptr(),
+                                            os[0], err, stream), what)
         return out
     size = lib.b200asr_lora_rows_workspace_size(m, rank)
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-    _count(2)
-    check(lib.b200asr_lora_rows(_p(x), x.stride(0), m, k, _p(weight), n, _p(lora_a), _p(lora_b), adapters,
-                                rank, _p(scales), _p(row_adapter), _p(out), out.stride(0), _p(workspace),
-                                size, _p(error_flag), _stream()), what)
+    workspace = torch.empty(size, dtype=_U8, device=x.device)
+    check(lib.b200asr_lora_rows(x.data_ptr(), xs[0], m, k, weight.data_ptr(), n, lora_a.data_ptr(),
+                                lora_b.data_ptr(), adapters, rank, scales.data_ptr(),
+                                row_adapter.data_ptr(), out.data_ptr(), os[0], workspace.data_ptr(),
+                                size, err, stream), what)
     return out
 
 

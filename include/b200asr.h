@@ -504,7 +504,7 @@ B200ASR_API int b200asr_load_kvcache4(const b200asr_kv4 *cache, const int32_t *s
  * cached token gives zeros; rows of out past `batch` are left alone. A length beyond
  * bt_width blocks is cut there (B200ASR_DEVERR_LENGTH); every length must be <=
  * max_seqlen_k. The workspace needs no initial value and keeps nothing between calls; it is
- * b200asr_paged_decode4_workspace_size bytes (0 for max_seqlen_k <= 512), 16-byte aligned,
+ * b200asr_paged_decode4_workspace_size bytes (0 for max_seqlen_k <= 1024), 16-byte aligned,
  * and serves one call at a time. */
 B200ASR_API size_t b200asr_paged_decode4_workspace_size(int32_t max_seqlen_k, int32_t num_heads,
                                                         int32_t num_kv_heads, int32_t head_dim);

@@ -358,7 +358,7 @@ def test_decode_peaked_scores(kx):
 @pytest.mark.gpu
 def test_decode_many_rows(kx):
     rng = np.random.default_rng(3)
-    check_decode(kx, [int(n) for n in rng.integers(0, 40, size=300)] + [600], 2, 1, 64, 16, seed=31)
+    check_decode(kx, [int(n) for n in rng.integers(0, 40, size=300)] + [1600], 2, 1, 64, 16, seed=31)
 
 
 @pytest.mark.gpu
@@ -390,19 +390,19 @@ def test_decode_is_the_same_every_time_and_under_capture(kx):
 
 @pytest.mark.gpu
 def test_decode_reads_strided_queries_and_a_given_workspace(kx):
-    lens = [900, 33]
+    lens = [1900, 33]
     table, blocks = paged(5, lens, 16)
     cache = filled(6, blocks, 16, 2, 64)
     wide = torch.randn(2, 3, 8, 64, device="cuda").bfloat16()
     q = wide[:, 1, ::2]  # 4 heads, every second one of a wider row
     out = torch.empty(2, 8, 64, dtype=BF16, device="cuda")[:, ::2]
-    ws = torch.full((kx.paged_decode4_workspace_size(900, 4, 2, 64),), 255, dtype=torch.uint8, device="cuda")
-    kx.paged_decode4(q, *cache, starts(lens), table, max_seqlen_k=900, scale=0.125, out=out, workspace=ws)
+    ws = torch.full((kx.paged_decode4_workspace_size(1900, 4, 2, 64),), 255, dtype=torch.uint8, device="cuda")
+    kx.paged_decode4(q, *cache, starts(lens), table, max_seqlen_k=1900, scale=0.125, out=out, workspace=ws)
     for b, n in enumerate(lens):
         want, tol = plain_attention(q[b:b + 1], cache, table[b], n, 0.125)
         check_close(out[b:b + 1], want, tol, f"row {b}")
     with pytest.raises(RuntimeError, match="workspace"):
-        kx.paged_decode4(q, *cache, starts(lens), table, max_seqlen_k=900, scale=0.125, out=out, workspace=ws[:-16])
+        kx.paged_decode4(q, *cache, starts(lens), table, max_seqlen_k=1900, scale=0.125, out=out, workspace=ws[:-16])
 
 
 @pytest.mark.gpu

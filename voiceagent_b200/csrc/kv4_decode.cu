@@ -23,10 +23,15 @@
 //  * A warp keeps its own ring of cp.async stages (32 tokens each) and its own softmax state:
 //    no barrier inside a segment. The running maximum moves only when a score passes it by 8
 //    (base 2), so most stages need one vote instead of reductions and rescales.
-// Work split: (sequence, KV head) pairs are cut into rounds of 128 tokens (4 warps x 32), laid
-// end to end and divided evenly among the CTAs whatever the length mix. A pair that several
-// CTAs share leaves fp32 partials in the workspace, and a second kernel joins them in token
-// order (the result does not depend on timing). Nothing in the workspace outlives the call.
+// Work split: a CTA's four warps take four KV heads of the same tokens, so that a slot's rows are
+// read together (one head's rows alone are 64-byte pieces 512 bytes apart: 213 us against 172
+// us for a cache laid out head by head, 32 sequences of 8k to 32k tokens); where the heads do
+// not divide so, or contexts are short and CTAs few, two or four warps take a head's tokens in
+// turn and their states are joined in shared memory. (sequence, head group) lists of rounds --
+// 32 tokens for each warp -- are laid end to end and divided evenly among the CTAs whatever the
+// length mix. A head that several CTAs share leaves fp32 partials in the workspace, and a second
+// kernel joins them in token order (the result does not depend on timing). Nothing in the
+// workspace outlives the call.
 #include <cuda_fp16.h>
 
 #include "kv4.cuh"
@@ -34,8 +39,9 @@
 namespace b200asr {
 
 constexpr int kD4Warps = 4;
+constexpr int kD4JoinWarps = 8;
+constexpr int kD4MaxCtas = 1024;                 // CTAs of a launch that splits
 constexpr int kD4Tile = 32;                      // tokens of a warp's stage
-constexpr int kD4Round = kD4Warps * kD4Tile;     // tokens of a CTA's round
 constexpr int kD4Stages = 3;
 constexpr int kD4CtasPerSm = 3;
 constexpr float kD4Lazy = 8.f;                   // base-2 slack of the running maximum
@@ -52,11 +58,13 @@ struct Decode4Args {
   int group;      // query heads of a KV head
   int subs;       // column groups of 8 * NT query heads per KV head
   int bs_shift;   // log2(block_size), or -1
-  int whole;      // a CTA per (sequence, head) pair: nothing is split
-  float scale_log2;
+  int hw_log2;    // log2 of the heads that a CTA's warps take side by side
+  int whole;      // a CTA per (sequence, head group): nothing is split
+  float scale_log2;  // >= 0: the sign is in `flip`
+  int flip;          // sign bit to exchange in q
   __nv_bfloat16 *out;
   int64_t out_row, out_head;
-  float *ws;      // partials: [2 * ctas][8 * NT][D + 2]
+  float *ws;      // partials: [2 * ctas][heads side by side][columns][D + 4]
   int32_t *error_flag;
 };
 
@@ -67,15 +75,19 @@ __device__ __forceinline__ int decode4_len(const Decode4Args &a, int b) {
                               static_cast<int64_t>(a.bt_width) * a.c.block_size));
 }
 
-__device__ __forceinline__ int rounds_of(int len) { return (len + kD4Round - 1) / kD4Round; }
+// Rounds of a sequence: 32 tokens for each of the 4 >> hw_log2 warps that share a head.
+__device__ __forceinline__ int rounds_of(const Decode4Args &a, int len) {
+  const int shift = 7 - a.hw_log2;
+  return (len + (1 << shift) - 1) >> shift;
+}
 
-// Rounds of all pairs, and of the pairs of sequences before `upto` (block-wide; 128 threads).
-__device__ __forceinline__ int64_t decode4_rounds(const Decode4Args &a, int pairs, int upto,
+// Rounds of all head groups, and of those of sequences before `upto` (block-wide).
+__device__ __forceinline__ int64_t decode4_rounds(const Decode4Args &a, int groups, int upto,
                                                   int64_t &before) {
-  __shared__ int64_t part[2][kD4Warps];
+  __shared__ int64_t part[2][kD4JoinWarps];
   int64_t all = 0, some = 0;
   for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
-    const int r = rounds_of(decode4_len(a, b));
+    const int r = rounds_of(a, decode4_len(a, b));
     all += r;
     if (b < upto) some += r;
   }
@@ -90,14 +102,13 @@ __device__ __forceinline__ int64_t decode4_rounds(const Decode4Args &a, int pair
   }
   __syncthreads();
   all = some = 0;
-#pragma unroll
-  for (int w = 0; w < kD4Warps; ++w) {
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
     all += part[0][w];
     some += part[1][w];
   }
-  before = some * pairs;
+  before = some * groups;
   __syncthreads();
-  return all * pairs;
+  return all * groups;
 }
 
 // CTA c's first unit of `units` dealt evenly to `ctas`, and the CTA of unit u.
@@ -147,16 +158,29 @@ __device__ __forceinline__ uint32_t movm_trans(uint32_t x) {
   return y;
 }
 
+// (x & MASK) | bits in one instruction: `bits` has to be a register (held_constant), two
+// immediates would take two.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(MASK), "r"(bits));
+  return y;
+}
+__device__ __forceinline__ uint32_t held_constant(uint32_t v) {
+  uint32_t y;
+  asm volatile("mov.b32 %0, %1;" : "=r"(y) : "r"(v));
+  return y;
+}
 // Codes 0 and 4 of a word as the fp16 pair 1024 + code, codes 1 and 5 as 1024 + 16 code.
-__device__ __forceinline__ uint32_t code_low(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }
-__device__ __forceinline__ uint32_t code_high(uint32_t w) { return (w & 0x00f000f0u) | 0x64006400u; }
+__device__ __forceinline__ uint32_t code_low(uint32_t w, uint32_t f16_1024) { return and_or<0x000f000fu>(w, f16_1024); }
+__device__ __forceinline__ uint32_t code_high(uint32_t w, uint32_t f16_1024) { return and_or<0x00f000f0u>(w, f16_1024); }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 // Codes i and i + 4 of a word (or i of two words' halves) as the bf16 pair 128 + code.
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
-  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, uint32_t bf16_128) {
+  return and_or<0x000f000fu>(w >> (4 * i), bf16_128);
 }
 // 128 + code -> code - 8, exact in bf16.
 __device__ __forceinline__ uint32_t centre_pair(uint32_t p) {
@@ -173,7 +197,8 @@ struct Dec4 {
   static constexpr int STAGE = kD4Tile * (2 * ROW + 8);    // K, V, parameters
   static constexpr int RING = kD4Stages * STAGE;
   static constexpr int STATE = NT * (4 * (D / 16) + 4) * 32 * 4;  // one warp's softmax state
-  static constexpr int SMEM = kD4Warps * RING + 3 * STATE;
+  // the joins' states only where warps share a head
+  static constexpr int smem(int hw_log2) { return kD4Warps * RING + (hw_log2 < 2 ? 3 * STATE : 0); }
 };
 
 // Where row `r` of a V stage lies: the lanes of one shared-memory phase read rows 2t of four
@@ -188,17 +213,17 @@ __device__ __forceinline__ int v_swap(int r) {
   return D == 128 ? ((r >> 2) & 1) << 1 : 0;
 }
 
-// A position in the flattened (sequence, pair, round) list.
+// A position in the flattened (sequence, head group, round) list.
 struct Cursor4 {
   int b, p, r, rounds, len;
   __device__ __forceinline__ void load(const Decode4Args &a) {
     len = decode4_len(a, b);
-    rounds = rounds_of(len);
+    rounds = rounds_of(a, len);
   }
-  __device__ __forceinline__ void next(const Decode4Args &a, int pairs) {
+  __device__ __forceinline__ void next(const Decode4Args &a, int groups) {
     if (++r < rounds) return;
     r = 0;
-    if (++p < pairs) return;
+    if (++p < groups) return;
     p = 0;
     do {
       ++b;
@@ -220,7 +245,12 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
   uint8_t *ring = smem + warp * C::RING;
   float *state = reinterpret_cast<float *>(smem + kD4Warps * C::RING);
   const uint32_t ring_s = smem_addr(ring);
-  const int pairs = a.c.num_kv_heads * a.subs;
+  // Column groups of KV heads, 1 << hw_log2 of them side by side; this warp's one, and its turn
+  // among the warps that share it.
+  const int groups = (a.c.num_kv_heads * a.subs) >> a.hw_log2;
+  const int side = warp & ((1 << a.hw_log2) - 1), turn = warp >> a.hw_log2;
+  const int round_log2 = 7 - a.hw_log2;
+  const uint32_t f16_1024 = held_constant(0x64006400u), bf16_128 = held_constant(0x43004300u);
 
   pdl_trigger();
   pdl_wait();
@@ -239,22 +269,22 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
   int64_t u0, u1;
   Cursor4 ld;
   if (a.whole) {
-    ld.b = blockIdx.x / pairs;
-    ld.p = blockIdx.x - ld.b * pairs;
+    ld.b = blockIdx.x / groups;
+    ld.p = blockIdx.x - ld.b * groups;
     ld.r = 0;
     ld.load(a);
     u0 = 0;
     u1 = ld.rounds;
   } else {
     int64_t unused;
-    const int64_t units = decode4_rounds(a, pairs, 0, unused);
+    const int64_t units = decode4_rounds(a, groups, 0, unused);
     u0 = first_unit(units, gridDim.x, blockIdx.x);
     u1 = first_unit(units, gridDim.x, blockIdx.x + 1);
     if (u0 < u1) {  // find the sequence: a warp scan, the same in every warp
       int64_t carry = 0;
       for (int base = 0;; base += 32) {
         const int b = base + lane;
-        const int n = b < a.batch ? rounds_of(decode4_len(a, b)) * pairs : 0;
+        const int n = b < a.batch ? rounds_of(a, decode4_len(a, b)) * groups : 0;
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -281,7 +311,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
   Cursor4 cur = ld;
 
   // ------------------------------------------------------------------ loads of a stage
-  auto token_of = [&](const Cursor4 &c) { return c.r * kD4Round + warp * kD4Tile + lane; };
+  auto token_of = [&](const Cursor4 &c) { return (c.r << round_log2) + turn * kD4Tile + lane; };
   // the block of this lane's token (its table entry is read one stage ahead of its use)
   auto block_of = [&](const Cursor4 &c) -> int {
     const int tok = token_of(c);
@@ -289,65 +319,82 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
     const int j = a.bs_shift >= 0 ? tok >> a.bs_shift : tok / a.c.block_size;
     return a.block_tables[c.b * a.bt_stride + j];
   };
-  // Blocks of whole stages: a stage's rows lie at one base with the slots' stride, and only the
-  // sequence's last stage needs a check per row.
-  const bool even_blocks = a.bs_shift >= 5;
+  // Where this lane's pieces of a stage go, and the rows that its next pieces are apart.
+  constexpr int STEP_ROWS = 32 / C::CHUNKS;
   const int lane_row = lane / C::CHUNKS, lane_ch = lane % C::CHUNKS;
-  const int64_t lane_off = lane_row * a.c.code_stride[1] + lane_ch * 16;
-  const int64_t round_off = (32 / C::CHUNKS) * a.c.code_stride[1];
-  auto issue = [&](const Cursor4 &c, int block, int stage) {
-    const int tok = token_of(c);
-    const bool valid = tok < c.len;
-    if (valid && (block < 0 || block >= a.c.num_blocks)) {
-      raise_flag(a.error_flag, B200ASR_DEVERR_BLOCK);
-      block = 0;
-    }
-    const int h = c.p / a.subs;
-    const uint32_t ks = ring_s + stage * C::STAGE, vs = ks + kD4Tile * C::ROW, ps = vs + kD4Tile * C::ROW;
-    if (even_blocks && tok - lane + kD4Tile <= c.len) {
-      const int at = tok & (a.c.block_size - 1);
-      const int64_t off = block * a.c.code_stride[0] + (at - lane) * a.c.code_stride[1] +
-                          h * a.c.code_stride[2] + lane_off;
-      const uint8_t *kp = static_cast<const uint8_t *>(a.c.k_codes) + off;
-      const uint8_t *vp = static_cast<const uint8_t *>(a.c.v_codes) + off;
-      cp_async8(ps + lane * 8, static_cast<const __nv_bfloat16 *>(a.c.params) + block * a.c.param_stride[0] +
-                                   at * a.c.param_stride[1] + h * a.c.param_stride[2], true);
-#pragma unroll
-      for (int i = 0; i < C::CHUNKS; ++i) {
-        const int row = i * (32 / C::CHUNKS) + lane_row;
-        cp_async16(ks + row * C::ROW + lane_ch * 16, kp + i * round_off, true);
-        cp_async16(vs + v_place<D>(row) * C::ROW + (lane_ch ^ v_swap<D>(row)) * 16, vp + i * round_off, true);
-      }
-      return;
-    }
-    const int at = a.bs_shift >= 0 ? tok & (a.c.block_size - 1) : tok % a.c.block_size;
-    if (!valid) block = 0;
-    const int64_t off = block * a.c.code_stride[0] + (valid ? at : 0) * a.c.code_stride[1] +
-                        h * a.c.code_stride[2];
-    const int64_t poff = block * a.c.param_stride[0] + (valid ? at : 0) * a.c.param_stride[1] +
-                         h * a.c.param_stride[2];
-    cp_async8(ps + lane * 8, static_cast<const __nv_bfloat16 *>(a.c.params) + poff, valid);
-#pragma unroll
-    for (int i = 0; i < C::CHUNKS; ++i) {
-      const int row = i * (32 / C::CHUNKS) + lane_row;
-      const int64_t o = __shfl_sync(0xffffffffu, off, row) + lane_ch * 16;
-      const bool ok = __shfl_sync(0xffffffffu, static_cast<int>(valid), row) != 0;
-      cp_async16(ks + row * C::ROW + lane_ch * 16, static_cast<const uint8_t *>(a.c.k_codes) + o, ok);
-      cp_async16(vs + v_place<D>(row) * C::ROW + (lane_ch ^ v_swap<D>(row)) * 16,
-                 static_cast<const uint8_t *>(a.c.v_codes) + o, ok);
-    }
-  };
-
-  int issued = 0, next_block = block_of(ld);
+  const uint32_t k_dst = ring_s + lane_row * C::ROW + lane_ch * 16;
+  const uint32_t v_dst = ring_s + (kD4Tile + v_place<D>(lane_row)) * C::ROW + (lane_ch ^ v_swap<D>(lane_row)) * 16;
+  const uint32_t p_dst = ring_s + 2 * kD4Tile * C::ROW + lane * 8;
+  const int64_t step_off = STEP_ROWS * a.c.code_stride[1];
+  // Blocks of whole stages (a power of two, 32 tokens at least): the stages of a block lie one
+  // stride apart, so only the first takes the table and the address arithmetic, and `run` more
+  // follow by adding. kp, vp and pp are this lane's first pieces of the stage last issued.
+  const bool even_blocks = a.bs_shift >= 5;
+  const int64_t code_step = a.c.code_stride[1] << round_log2, param_step = a.c.param_stride[1] << round_log2;
+  const uint8_t *kp = nullptr, *vp = nullptr;
+  const __nv_bfloat16 *pp = nullptr;
+  int issued = 0, run = 0, span = 0, next_block = block_of(ld);
+  uint32_t fill = 0;  // byte offset of the next stage in the ring
   auto issue_next = [&]() {
     if (issued < total) {
-      const Cursor4 c = ld;
-      const int block = next_block;
-      if (++issued < total) {
-        ld.next(a, pairs);
+      const bool stepped = run > 0;
+      if (stepped) {
+        --run;
+        kp += code_step;
+        vp += code_step;
+        pp += param_step;
+      }
+      bool whole = stepped;
+      int block = next_block, at = 0;
+      bool valid = true;
+      int64_t off = 0;
+      if (!stepped) {
+        const int tok = token_of(ld), first = tok - lane;
+        valid = tok < ld.len;
+        if (valid && (block < 0 || block >= a.c.num_blocks)) {
+          raise_flag(a.error_flag, B200ASR_DEVERR_BLOCK);
+          block = 0;
+        }
+        if (!valid) block = 0;
+        const int pair = (ld.p << a.hw_log2) + side, h = a.subs == 1 ? pair : pair / a.subs;
+        whole = even_blocks && first + kD4Tile <= ld.len;
+        at = !valid ? 0 : a.bs_shift >= 0 ? tok & (a.c.block_size - 1) : tok % a.c.block_size;
+        off = block * a.c.code_stride[0] + at * a.c.code_stride[1] + h * a.c.code_stride[2];
+        pp = static_cast<const __nv_bfloat16 *>(a.c.params) + block * a.c.param_stride[0] +
+             at * a.c.param_stride[1] + h * a.c.param_stride[2];
+        if (whole) {
+          const int64_t mine = off + (lane_row - lane) * a.c.code_stride[1] + lane_ch * 16;
+          kp = static_cast<const uint8_t *>(a.c.k_codes) + mine;
+          vp = static_cast<const uint8_t *>(a.c.v_codes) + mine;
+          span = run = min(min((a.c.block_size - kD4Tile - (at - lane)) >> round_log2,
+                               (ld.len - kD4Tile - first) >> round_log2),
+                           ld.rounds - 1 - ld.r);
+        }
+      }
+      cp_async8(p_dst + fill, pp, valid);
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < C::CHUNKS; ++i) {
+          cp_async16(k_dst + fill + i * STEP_ROWS * C::ROW, kp + i * step_off, true);
+          cp_async16(v_dst + fill + i * STEP_ROWS * C::ROW, vp + i * step_off, true);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < C::CHUNKS; ++i) {
+          const int row = i * STEP_ROWS + lane_row;
+          const int64_t o = __shfl_sync(0xffffffffu, off, row) + lane_ch * 16;
+          const bool ok = __shfl_sync(0xffffffffu, static_cast<int>(valid), row) != 0;
+          cp_async16(k_dst + fill + i * STEP_ROWS * C::ROW, static_cast<const uint8_t *>(a.c.k_codes) + o, ok);
+          cp_async16(v_dst + fill + i * STEP_ROWS * C::ROW, static_cast<const uint8_t *>(a.c.v_codes) + o, ok);
+        }
+      }
+      fill = fill == (kD4Stages - 1) * C::STAGE ? 0 : fill + C::STAGE;
+      if (++issued < total && run == 0) {  // the next stage starts anew
+        ld.r += span;
+        span = 0;
+        ld.next(a, groups);
         next_block = block_of(ld);
       }
-      issue(c, block, (issued - 1) % kD4Stages);
     }
     cp_commit();
   };
@@ -355,9 +402,16 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
   for (int s = 0; s < kD4Stages - 1; ++s) issue_next();
 
   // ------------------------------------------------------------------ segments
-  int done = 0;
+  // This lane's codes and parameters within a stage: its 16-byte (D = 64: 8) piece of K rows g
+  // and g + 8, and its 8-byte (4) piece of V rows 2t, 2t + 1, 2t + 8, 2t + 9.
+  const uint8_t *k_lane = ring + g * C::ROW + t * (C::ROW / 4);
+  const uint8_t *p_lane = ring + 2 * kD4Tile * C::ROW + g * 8;
+  const uint8_t *v_lane = ring + kD4Tile * C::ROW + v_place<D>(2 * t) * C::ROW +
+                          (D == 128 ? (((g >> 1) ^ v_swap<D>(2 * t)) << 4) + (g & 1) * 8 : g * 4);
+  constexpr int V_NEXT = (D == 128 ? 2 : 4) * C::ROW;  // v_place of the odd row
+  int done = 0, stage = 0;
   while (done < total) {
-    const int b = cur.b, p = cur.p, r_first = cur.r;
+    const int b = cur.b, p = (cur.p << a.hw_log2) + side, r_first = cur.r;
     const int r_last = min(cur.rounds, cur.r + (total - done));  // one past
     const int h = p / a.subs, col0 = (p - h * a.subs) * 8 * NT;
     const int cols = min(8 * NT, a.group - col0);
@@ -366,8 +420,9 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
     // dims 32 t + 8 j (D = 128) or 16 t + 8 j (D = 64) and up
     uint32_t qf[NT][KS][2];
     float c0[NT], c1[NT];    // the accumulator's start: what the offsets of the codes add up to
-    float qs0[NT], qs1[NT];  // sum(q) of columns 2t and 2t + 1, times scale and log2(e)
-    float qx0[NT], qx1[NT];  // scale, log2(e) and the power of two of those columns
+    // Columns 2t and 2t + 1: sum(q) as it went into the products, and the factor -- scale, log2(e)
+    // and the power of two -- that makes a score of x = ks (q . c) + kz sum(q).
+    float qs0[NT], qs1[NT], qx0[NT], qx1[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       uint4 u[KW];
@@ -386,7 +441,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^x with the largest |q| 2^x in [2^13, 2^14); a row of zeros or beyond takes what it gets
       const int ex = min(100, max(-114, 13 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
-      const float up = __int_as_float((ex + 127) << 23);
+      const float up = __int_as_float(((ex + 127) << 23) | a.flip);
       float even = 0.f, odd = 0.f;
 #pragma unroll
       for (int j = 0; j < KW; ++j) {
@@ -406,8 +461,9 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
       even += __shfl_xor_sync(0xffffffffu, even, 2);
       odd += __shfl_xor_sync(0xffffffffu, odd, 2);
       const float start = -1024.f * even - 64.f * odd;
-      const float factor = a.scale_log2 * __int_as_float((127 - ex) << 23);
-      const float sum = (even + odd) * factor;
+      // (at least 1e-30: a scale of zero must not meet the -inf of masked tokens)
+      const float factor = fmaxf(1e-30f, a.scale_log2 * __int_as_float((127 - ex) << 23));
+      const float sum = even + odd;
       c0[n] = __shfl_sync(0xffffffffu, start, 8 * t);  // column 2t: lanes with g = 2t
       c1[n] = __shfl_sync(0xffffffffu, start, 8 * t + 4);
       qs0[n] = __shfl_sync(0xffffffffu, sum, 8 * t);
@@ -415,10 +471,11 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
       qx0[n] = __shfl_sync(0xffffffffu, factor, 8 * t);
       qx1[n] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
     }
-    float o[NT][KS][4], m0[NT], m1[NT], l0[NT], l1[NT], z0[NT], z1[NT];
+    // m: the maximum in use (base 2); t: the x past which it moves
+    float o[NT][KS][4], m0[NT], m1[NT], t0[NT], t1[NT], l0[NT], l1[NT], z0[NT], z1[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      m0[n] = m1[n] = -INFINITY;
+      m0[n] = m1[n] = t0[n] = t1[n] = -INFINITY;
       l0[n] = l1[n] = z0[n] = z1[n] = 0.f;
 #pragma unroll
       for (int j = 0; j < KS; ++j)
@@ -429,20 +486,20 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
     for (int r = r_first; r < r_last; ++r, ++done) {
       cp_wait<kD4Stages - 2>();
       __syncwarp();
-      const int stage = done % kD4Stages;
-      const uint8_t *kst = ring + stage * C::STAGE, *vst = kst + kD4Tile * C::ROW;
-      const uint8_t *pst = vst + kD4Tile * C::ROW;
-      const int left = cur.len - (r * kD4Round + warp * kD4Tile);  // tokens of this stage and on
+      const int in_ring = stage * C::STAGE;
+      stage = stage + 1 == kD4Stages ? 0 : stage + 1;
+      const uint8_t *kst = k_lane + in_ring, *vst = v_lane + in_ring, *pst = p_lane + in_ring;
+      const int left = cur.len - ((r << round_log2) + turn * kD4Tile);  // tokens of this stage and on
       float s[NT][2][4];
       uint32_t vpar[2][2];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        const uint2 pa = *reinterpret_cast<const uint2 *>(pst + (mt * 16 + g) * 8);
-        const uint2 pb = *reinterpret_cast<const uint2 *>(pst + (mt * 16 + g + 8) * 8);
+        const uint2 pa = *reinterpret_cast<const uint2 *>(pst + mt * 128);
+        const uint2 pb = *reinterpret_cast<const uint2 *>(pst + mt * 128 + 64);
         vpar[mt][0] = pa.y;
         vpar[mt][1] = pb.y;
         uint32_t ka[KW], kb[KW];
-        const uint8_t *ra = kst + (mt * 16 + g) * C::ROW + t * (C::ROW / 4), *rb = ra + 8 * C::ROW;
+        const uint8_t *ra = kst + mt * 16 * C::ROW, *rb = ra + 8 * C::ROW;
         if constexpr (KW == 4) {
           const uint4 x = *reinterpret_cast<const uint4 *>(ra), y = *reinterpret_cast<const uint4 *>(rb);
           ka[0] = x.x; ka[1] = x.y; ka[2] = x.z; ka[3] = x.w;
@@ -463,7 +520,8 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t x = half ? ka[j] >> 8 : ka[j], y = half ? kb[j] >> 8 : kb[j];
-            const uint32_t a0 = code_low(x), a2 = code_high(x), a1 = code_low(y), a3 = code_high(y);
+            const uint32_t a0 = code_low(x, f16_1024), a2 = code_high(x, f16_1024);
+            const uint32_t a1 = code_low(y, f16_1024), a3 = code_high(y, f16_1024);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               mma_f16(acc[n], a0, a1, a2, a3, qf[n][2 * j + half][0], qf[n][2 * j + half][1]);
@@ -471,10 +529,10 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
         const float2 kpa = unpack2(pa.x), kpb = unpack2(pb.x);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          s[n][mt][0] = fmaf(kpa.x * qx0[n], acc[n][0], kpa.y * qs0[n]);
-          s[n][mt][1] = fmaf(kpa.x * qx1[n], acc[n][1], kpa.y * qs1[n]);
-          s[n][mt][2] = fmaf(kpb.x * qx0[n], acc[n][2], kpb.y * qs0[n]);
-          s[n][mt][3] = fmaf(kpb.x * qx1[n], acc[n][3], kpb.y * qs1[n]);
+          s[n][mt][0] = fmaf(kpa.x, acc[n][0], kpa.y * qs0[n]);
+          s[n][mt][1] = fmaf(kpa.x, acc[n][1], kpa.y * qs1[n]);
+          s[n][mt][2] = fmaf(kpb.x, acc[n][2], kpb.y * qs0[n]);
+          s[n][mt][3] = fmaf(kpb.x, acc[n][3], kpb.y * qs1[n]);
         }
       }
       if (left < kD4Tile) {  // the sequence ends in this stage
@@ -491,7 +549,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
       for (int n = 0; n < NT; ++n) {
         const float x0 = fmaxf(fmaxf(s[n][0][0], s[n][0][2]), fmaxf(s[n][1][0], s[n][1][2]));
         const float x1 = fmaxf(fmaxf(s[n][0][1], s[n][0][3]), fmaxf(s[n][1][1], s[n][1][3]));
-        move = move || x0 > m0[n] + kD4Lazy || x1 > m1[n] + kD4Lazy;
+        move = move || x0 > t0[n] || x1 > t1[n];
       }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -503,8 +561,10 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
           }
-          x0 = fmaxf(x0, m0[n]);
-          x1 = fmaxf(x1, m1[n]);
+          t0[n] = fmaxf(t0[n], x0 + kD4Lazy / qx0[n]);
+          t1[n] = fmaxf(t1[n], x1 + kD4Lazy / qx1[n]);
+          x0 = fmaxf(x0 * qx0[n], m0[n]);
+          x1 = fmaxf(x1 * qx1[n], m1[n]);
           const float f0 = x0 == -INFINITY ? 1.f : exp2f(m0[n] - x0);
           const float f1 = x1 == -INFINITY ? 1.f : exp2f(m1[n] - x1);
           m0[n] = x0;
@@ -531,8 +591,8 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
         for (int mt = 0; mt < 2; ++mt) {
           const float2 va = unpack2(vpar[mt][0]), vb = unpack2(vpar[mt][1]);
           const float ca = fmaf(8.f, va.x, va.y), cb = fmaf(8.f, vb.x, vb.y);  // zero of code - 8
-          const float p0 = exp2f(s[n][mt][0] - r0), p1 = exp2f(s[n][mt][1] - r1);
-          const float p2 = exp2f(s[n][mt][2] - r0), p3 = exp2f(s[n][mt][3] - r1);
+          const float p0 = exp2f(fmaf(s[n][mt][0], qx0[n], -r0)), p1 = exp2f(fmaf(s[n][mt][1], qx1[n], -r1));
+          const float p2 = exp2f(fmaf(s[n][mt][2], qx0[n], -r0)), p3 = exp2f(fmaf(s[n][mt][3], qx1[n], -r1));
           l0[n] += p0 + p2;
           l1[n] += p1 + p3;
           z0[n] = fmaf(p0, ca, fmaf(p2, cb, z0[n]));
@@ -547,14 +607,13 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
         uint32_t w[4][VW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = mt * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+          const uint8_t *row = vst + mt * 16 * C::ROW + (i & 1) * V_NEXT + (i >> 1) * 8 * C::ROW;
           if constexpr (VW == 2) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(
-                vst + v_place<D>(row) * C::ROW + (((g >> 1) ^ v_swap<D>(row)) << 4) + (g & 1) * 8);
+            const uint2 x = *reinterpret_cast<const uint2 *>(row);
             w[i][0] = x.x;
             w[i][1] = x.y;
           } else {
-            w[i][0] = *reinterpret_cast<const uint32_t *>(vst + v_place<D>(row) * C::ROW + g * 4);
+            w[i][0] = *reinterpret_cast<const uint32_t *>(row);
           }
         }
 #pragma unroll
@@ -566,8 +625,8 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
             const uint32_t y = __byte_perm(w[2][j], w[3][j], sel);  // tokens 2t + 8, 2t + 9
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              const uint32_t a0 = centre_pair(code_pair(x, i)), a1 = centre_pair(code_pair(x, i + 1));
-              const uint32_t a2 = centre_pair(code_pair(y, i)), a3 = centre_pair(code_pair(y, i + 1));
+              const uint32_t a0 = centre_pair(code_pair(x, i, bf16_128)), a1 = centre_pair(code_pair(x, i + 1, bf16_128));
+              const uint32_t a2 = centre_pair(code_pair(y, i, bf16_128)), a3 = centre_pair(code_pair(y, i + 1, bf16_128));
               // output rows of this tile: dims (D / 8) g + e and e + 1, e = 8 j + 4 half + i
               const int tile = 4 * j + 2 * half + i / 2;
 #pragma unroll
@@ -597,7 +656,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
         o[n][j][3] += z1[n];
       }
     }
-    // the four warps' states: 2 and 3 into 0 and 1, then 1 into 0
+    // the states of warps that share a head: 2 and 3 into 0 and 1, then 1 into 0
     auto put = [&](float *to) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -635,13 +694,15 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
       }
     };
     constexpr int SF = C::STATE / 4;
-    if (warp >= 2) put(state + (warp - 2) * SF);
-    __syncthreads();
-    if (warp < 2) join(state + warp * SF);
-    if (warp == 1) put(state + 2 * SF);
-    __syncthreads();
-    if (warp == 0) {
-      join(state + 2 * SF);
+    if (a.hw_log2 < 2) {
+      if (warp >= 2) put(state + (warp - 2) * SF);
+      __syncthreads();
+      if (warp < 2) join(state + warp * SF);
+      if (a.hw_log2 == 0 && warp == 1) put(state + 2 * SF);
+      __syncthreads();
+      if (a.hw_log2 == 0 && warp == 0) join(state + 2 * SF);
+    }
+    if (turn == 0) {
       const bool full = r_first == 0 && r_last == cur.rounds;
       const int slot = 2 * blockIdx.x + (r_first > 0 ? 0 : 1);
 #pragma unroll
@@ -663,7 +724,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
                              pack2(o[n][j + 2][e] * inv, o[n][j + 2][e + 2] * inv),
                              pack2(o[n][j + 3][e] * inv, o[n][j + 3][e + 2] * inv));
           } else {
-            float *w = a.ws + (static_cast<int64_t>(slot) * 8 * NT + col) * (D + 4);
+            float *w = a.ws + (((static_cast<int64_t>(slot) << a.hw_log2) + side) * min(8 * NT, a.group) + col) * (D + 4);
             if (g == 0) {
               w[0] = e ? m1[n] : m0[n];
               w[1] = l;
@@ -677,72 +738,121 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
     }
     // the compute cursor follows the rounds just done
     cur.r = r_last - 1;
-    cur.next(a, pairs);
+    cur.next(a, groups);
   }
   cp_wait<0>();
 }
 
-// Joins the partials of the pairs that several CTAs shared: one CTA per (sequence, pair).
+// Joins the partials of the heads that several CTAs shared: one CTA per (sequence, head, column).
+// The partials' maxima give every weight at once; the eight warps then sum rows of partials
+// side by side (a lane holds four dims), with no load waiting for another, and their sums are
+// added in order.
 template <int D, int NT>
-__global__ void __launch_bounds__(kD4Warps * 32) paged_decode4_join_kernel(const Decode4Args a, int ctas) {
+__global__ void __launch_bounds__(kD4JoinWarps * 32) paged_decode4_join_kernel(const Decode4Args a, int ctas) {
+  __shared__ float weight[kD4MaxCtas], red[2][kD4JoinWarps];
+  __shared__ float4 part[kD4JoinWarps][32];
   pdl_trigger();
   pdl_wait();
-  const int pairs = a.c.num_kv_heads * a.subs;
-  const int b = blockIdx.x / pairs, p = blockIdx.x - b * pairs;
-  const int rounds = rounds_of(decode4_len(a, b));
-  int64_t first;
-  const int64_t units = decode4_rounds(a, pairs, b, first);
-  if (rounds == 0) return;
-  first += static_cast<int64_t>(p) * rounds;
-  const int c0 = cta_of_unit(units, ctas, first), c1 = cta_of_unit(units, ctas, first + rounds - 1);
-  if (c0 == c1) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pairs = a.c.num_kv_heads * a.subs, groups = pairs >> a.hw_log2;
+  const int most = min(8 * NT, a.group);
+  const int bp = blockIdx.x / most, col = blockIdx.x - bp * most;
+  const int b = bp / pairs, p = bp - b * pairs;
+  const int side = p & ((1 << a.hw_log2) - 1);
   const int h = p / a.subs, col0 = (p - h * a.subs) * 8 * NT;
-  const int cols = min(8 * NT, a.group - col0);
-  for (int i = threadIdx.x; i < cols * D; i += blockDim.x) {
-    const int col = i / D, d = i - col * D;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      // a CTA's share begins inside the pair (slot 0) unless it holds the pair's first round
-      const float *w = a.ws + (static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * 8 * NT + col) * (D + 4);
-      const float wm = w[0], x = fmaxf(m, wm);
-      const float fo = m == -INFINITY ? 0.f : exp2f(m - x);
-      const float fw = wm == -INFINITY && x == -INFINITY ? 1.f : exp2f(wm - x);
-      l = l * fo + w[1] * fw;
-      o = o * fo + w[4 + d] * fw;
-      m = x;
+  const int rounds = rounds_of(a, decode4_len(a, b));
+  if (rounds == 0 || col >= a.group - col0) return;
+  int64_t first;
+  const int64_t units = decode4_rounds(a, groups, b, first);
+  first += static_cast<int64_t>(p >> a.hw_log2) * rounds;
+  const int c0 = cta_of_unit(units, ctas, first), n = cta_of_unit(units, ctas, first + rounds - 1) - c0 + 1;
+  if (n == 1) return;
+  // partial i: a CTA's share begins inside the list (slot 0) unless it holds the first round
+  auto partial = [&](int i) {
+    return a.ws + (((static_cast<int64_t>(2 * (c0 + i) + (i == 0 ? 1 : 0)) << a.hw_log2) + side) * most + col) * (D + 4);
+  };
+  float m = -INFINITY;
+  for (int i = tid; i < n; i += blockDim.x) m = fmaxf(m, weight[i] = partial(i)[0]);
+  m = warp_max(m);
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+  m = red[0][0];
+#pragma unroll
+  for (int w = 1; w < kD4JoinWarps; ++w) m = fmaxf(m, red[0][w]);
+  float l = 0.f;
+  for (int i = tid; i < n; i += blockDim.x) {
+    const float w = weight[i] == -INFINITY && m == -INFINITY ? 1.f : exp2f(weight[i] - m);
+    weight[i] = w;
+    l = fmaf(w, partial(i)[1], l);
+  }
+  l = warp_sum(l);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  constexpr int LANES = D / 4, SIDE = 32 / LANES;  // lanes of a row, rows of a warp at once
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = warp * SIDE + lane / LANES; i < n; i += kD4JoinWarps * SIDE) {
+    const float4 x = *reinterpret_cast<const float4 *>(partial(i) + 4 + (lane % LANES) * 4);
+    const float w = weight[i];
+    o.x = fmaf(w, x.x, o.x);
+    o.y = fmaf(w, x.y, o.y);
+    o.z = fmaf(w, x.z, o.z);
+    o.w = fmaf(w, x.w, o.w);
+  }
+  part[warp][lane] = o;
+  __syncthreads();
+  if (tid < D) {
+    float sum = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kD4JoinWarps; ++w) {
+      den += red[1][w];
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k) sum += reinterpret_cast<const float *>(&part[w][k * LANES])[tid];
     }
-    a.out[b * a.out_row + (static_cast<int64_t>(h) * a.group + col0 + col) * a.out_head + d] = f2bf(o / l);
+    a.out[b * a.out_row + (static_cast<int64_t>(h) * a.group + col0 + col) * a.out_head + tid] = f2bf(sum / den);
   }
 }
 
-constexpr int kD4WholeMax = 512;  // longest context whose pairs are not split
+// Longest context that is not split. Device time split / whole, us: one sequence of 1000 tokens
+// 11 / 11, of 2000 11 / 18; 32 of 64 to 1024 14.6 / 12.8; 64 of 500 to 2000 33 / 36. A whole
+// context is one launch and takes no workspace, ~3 us of the host's time.
+constexpr int kD4WholeMax = 1024;
+
+inline int decode4_per_sm(int group) { return group <= 8 ? kD4CtasPerSm : 2; }
+
+// Bytes of partials: two per CTA, head side by side and column.
+inline size_t decode4_ws(int group, int head_dim) {
+  return static_cast<size_t>(decode4_per_sm(group)) * num_sms() * 2 * 4 *
+         std::min(group, group <= 8 ? 8 : 16) * (head_dim + 4) * 4;
+}
 
 template <int D, int NT>
 int launch_decode4(Decode4Args a, int max_seqlen_k, size_t ws_bytes, cudaStream_t stream) {
   using C = Dec4<D, NT>;
   a.subs = (a.group + 8 * NT - 1) / (8 * NT);
-  const int64_t pairs = static_cast<int64_t>(a.c.num_kv_heads) * a.subs * a.batch;
-  const int64_t most = pairs * ((max_seqlen_k + kD4Round - 1) / kD4Round);
-  const int per_sm = NT == 1 ? kD4CtasPerSm : 2;
+  const int heads = a.c.num_kv_heads * a.subs;
   a.whole = max_seqlen_k <= kD4WholeMax;
-  const int64_t grid = a.whole ? pairs : std::min<int64_t>(std::max<int64_t>(most, 1), per_sm * num_sms());
-  B200_REQUIRE(grid <= 0x7fffffff && pairs <= 0x7fffffff, "paged_decode4: too many rows");
-  if (!a.whole) {
-    const size_t need = static_cast<size_t>(per_sm) * num_sms() * 2 * 8 * NT * (D + 4) * 4;
-    if (a.ws == nullptr || ws_bytes < need) {
-      set_error("paged_decode4: workspace of %zu bytes, %zu needed", ws_bytes, need);
-      return B200ASR_ERR_WORKSPACE;
-    }
+  a.hw_log2 = a.whole || heads % 2 ? 0 : heads % 4 ? 1 : 2;
+  const int64_t pairs = static_cast<int64_t>(heads) * a.batch;
+  const int round = 128 >> a.hw_log2;
+  const int64_t most = (pairs >> a.hw_log2) * ((max_seqlen_k + round - 1) / round);
+  const int64_t grid = a.whole ? pairs
+                               : std::min<int64_t>(std::max<int64_t>(most, 1), decode4_per_sm(a.group) * num_sms());
+  const int64_t joins = pairs * std::min(8 * NT, a.group);
+  B200_REQUIRE(grid <= 0x7fffffff && joins <= 0x7fffffff && (a.whole || grid <= kD4MaxCtas), "paged_decode4: too many rows");
+  if (!a.whole && (a.ws == nullptr || ws_bytes < decode4_ws(a.group, D))) {
+    set_error("paged_decode4: workspace of %zu bytes, %zu needed", ws_bytes, decode4_ws(a.group, D));
+    return B200ASR_ERR_WORKSPACE;
   }
   auto kfn = paged_decode4_kernel<D, NT>;
-  const cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  const cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(0));
   B200_LAUNCH_CHECK_ERR(e, "paged_decode4 (configuration)");
   B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(static_cast<unsigned>(grid)), dim3(kD4Warps * 32),
-                                      C::SMEM, stream, true, 1, a),
+                                      C::smem(a.hw_log2), stream, true, 1, a),
                         "paged_decode4");
   if (!a.whole)
-    B200_LAUNCH_CHECK_ERR(launch_kernel(paged_decode4_join_kernel<D, NT>, dim3(static_cast<unsigned>(pairs)),
-                                        dim3(kD4Warps * 32), 0, stream, true, 1, a, static_cast<int>(grid)),
+    B200_LAUNCH_CHECK_ERR(launch_kernel(paged_decode4_join_kernel<D, NT>, dim3(static_cast<unsigned>(joins)),
+                                        dim3(kD4JoinWarps * 32), 0, stream, true, 1, a, static_cast<int>(grid)),
                           "paged_decode4 (join)");
   return B200ASR_OK;
 }
@@ -753,10 +863,8 @@ using namespace b200asr;
 
 extern "C" size_t b200asr_paged_decode4_workspace_size(int32_t max_seqlen_k, int32_t num_heads,
                                                        int32_t num_kv_heads, int32_t head_dim) {
-  if (max_seqlen_k <= kD4WholeMax || num_heads < 1 || num_kv_heads < 1 || head_dim < 1) return 0;
-  const int nt = num_heads / num_kv_heads > 8 ? 2 : 1;
-  const int per_sm = nt == 1 ? kD4CtasPerSm : 2;
-  return static_cast<size_t>(per_sm) * num_sms() * 2 * 8 * nt * (head_dim + 4) * 4;
+  if (max_seqlen_k <= kD4WholeMax || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
+  return decode4_ws(num_heads / num_kv_heads, head_dim);
 }
 
 extern "C" int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
@@ -798,7 +906,8 @@ extern "C" int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64_
   a.group = num_heads / cache->num_kv_heads;
   const int bs = cache->block_size;
   a.bs_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
+  a.flip = scale < 0 ? static_cast<int>(0x80000000u) : 0;
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.out_row = out_row_stride;
   a.out_head = out_head_stride;

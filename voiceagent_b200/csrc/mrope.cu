@@ -126,15 +126,14 @@ __global__ void __launch_bounds__(kMrWarps * 32) qk_norm_mrope_store_kernel(cons
         if (slot >= 0)
           *reinterpret_cast<uint4 *>((is_v ? a.v_cache : a.k_cache) + (slot * a.num_kv_heads + h) * D + gl * 8) = v;
       } else if (__any_sync(0xffffffffu, slot >= 0)) {  // the reductions below need every lane
-        float f[8];
-        unpack8(v, f);
-        uint32_t codes, sz;
-        kv4_quantise<LANES>(f, codes, sz);
+        const uint32_t rows[4] = {v.x, v.y, v.z, v.w};
+        uint32_t codes[1], sz;
+        kv4_quantise<LANES, 4>(rows, codes, sz);
         if (slot >= 0) {
           const int64_t block = slot / a.c.block_size, at = slot - block * a.c.block_size;
           reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(is_v ? a.c.v_codes : a.c.k_codes) +
                                        block * a.c.code_stride[0] + at * a.c.code_stride[1] +
-                                       h * a.c.code_stride[2])[gl] = codes;
+                                       h * a.c.code_stride[2])[gl] = codes[0];
           if (gl == 0)
             reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.c.params) +
                                          block * a.c.param_stride[0] + at * a.c.param_stride[1] +

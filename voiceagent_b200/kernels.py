@@ -476,6 +476,11 @@ def _attention4_args(what: str, q, out, cu_seqlens_k, block_tables, heads: int, 
     return qs, os, batch, bs[0], table[1]
 
 
+# max_seqlen_k at or below this is one launch without a workspace; must match kD4WholeMax in
+# csrc/kv4_decode.cu.
+DECODE4_WHOLE_CTX = 1024
+
+
 def paged_decode4_workspace_size(max_seqlen_k: int, num_heads: int, num_kv_heads: int,
                                  head_dim: int = 128) -> int:
     return int(lib.b200asr_paged_decode4_workspace_size(max_seqlen_k, num_heads, num_kv_heads,
@@ -499,12 +504,12 @@ def paged_decode4(q, k_codes, v_codes, kv_params, cu_seqlens_k, block_tables, *,
     ws, ws_bytes = None, 0
     if workspace is not None:
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    elif max_seqlen_k > DECODE_SHORT_CTX:
+    elif max_seqlen_k > DECODE4_WHOLE_CTX:
         ws_bytes = lib.b200asr_paged_decode4_workspace_size(max_seqlen_k, q_heads, heads, dim)
         workspace = torch.empty(ws_bytes, dtype=_U8, device=q.device)
         ws = workspace.data_ptr()
     _here(what, k_codes, v_codes, kv_params, q, out, cu_seqlens_k, block_tables, workspace, error_flag)
-    _count(1 if max_seqlen_k <= DECODE_SHORT_CTX else 2)  # + the join of split contexts
+    _count(1 if max_seqlen_k <= DECODE4_WHOLE_CTX else 2)  # + the join of split contexts
     check(lib.b200asr_paged_decode4(
         q.data_ptr(), qs[0], qs[1], cache, q_heads, cu_seqlens_k.data_ptr(), block_tables.data_ptr(),
         bt_stride, bt_width, batch, max_seqlen_k, scale, out.data_ptr(), os[0], os[1], ws, ws_bytes,

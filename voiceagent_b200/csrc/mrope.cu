@@ -9,10 +9,12 @@
 // 4-bit one (kv4.cuh), quantised from the rounded K.
 //
 // Bound by memory (the projection in, q and the cache out) and, for a decode step, by latency.
-// A CTA takes whole tokens: D / 2 threads per token turn the axes into cos and sin once, in
-// shared memory, while every warp's head vectors are already on their way; a vector is D / 8
-// lanes of 8 consecutive dims, one 16-byte load, and a lane's rotation partner is the lane
-// half a vector away.
+// A CTA takes groups of whole tokens, one after another: D / 2 threads per token turn the axes
+// into cos and sin once, in shared memory, and the next group's (a chain of three dependent
+// loads) and its first head vectors are on their way under the arithmetic of this one. A vector
+// is D / 8 lanes, each with 4 dims of the first half and the 4 they turn with, so the rotation
+// stays in the lane and only the sum of squares is a shuffle reduction. A warp keeps its heads
+// for all tokens of a group: what depends on the head (kind, weights, offsets) is worked out once.
 #include "kv4.cuh"
 
 namespace b200asr {
@@ -39,118 +41,206 @@ struct MropeArgs {
 };
 
 constexpr int kMrWarps = 8;
+// Tokens of a group where there are many, and CTAs of an SM; 7829 tokens of 16 + 2 x 8 heads of 128:
+// (2, 4) 29.0 us, (4, 3) 29.6, (2, 3) 32.1, (4, 2) 34.5; a CTA per 4 tokens and none resident 33.3.
+constexpr int kMrTok = 2, kMrCtasPerSm = 4;
 
-// TOK tokens per CTA; a warp's step is 32 / LANES head vectors of one token, STEPS at a time.
-template <int LANES, int TOK, int STEPS, bool KV4>
-__global__ void __launch_bounds__(kMrWarps * 32) qk_norm_mrope_store_kernel(const MropeArgs a) {
+// TOK tokens per group; a warp takes 32 / LANES neighbouring heads of all of them at a time.
+template <int LANES, int TOK, bool KV4>
+__global__ void __launch_bounds__(kMrWarps * 32, kMrCtasPerSm) qk_norm_mrope_store_kernel(const MropeArgs a) {
   constexpr int D = LANES * 8, PER = 32 / LANES;
-  __shared__ float cs[TOK][D];  // cos | sin of each frequency at its own position
+  constexpr int CS = (TOK * (D / 2) + kMrWarps * 32 - 1) / (kMrWarps * 32);  // angles of a thread
+  __shared__ __align__(16) float cs_all[2][TOK][D];  // cos | sin of each frequency at its position
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gl = lane & (LANES - 1);
-  const int t0 = blockIdx.x * TOK;
   const int heads = a.num_heads + 2 * a.num_kv_heads;
-  const int steps = (heads + PER - 1) / PER;  // of one token
-  const int total = min(TOK, a.num_tokens - t0) * steps;
+  constexpr int step = kMrWarps * PER;
+  const int groups = (a.num_tokens + TOK - 1) / TOK;
+  uint2 raw[TOK][2];
+  auto fetch = [&](int group, int first) {
+    const int head = first + lane / LANES, t0 = group * TOK;
+    const __nv_bfloat16 *src = a.qkv + t0 * a.qkv_stride + head * D + gl * 4;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      raw[i][0] = raw[i][1] = make_uint2(0, 0);
+      if (t0 + i < a.num_tokens && head < heads) {
+        raw[i][0] = *reinterpret_cast<const uint2 *>(src + i * a.qkv_stride);
+        raw[i][1] = *reinterpret_cast<const uint2 *>(src + i * a.qkv_stride + D / 2);
+      }
+    }
+  };
+  // this thread's angles (token i / (D / 2) of the group, frequency i % (D / 2)): their axis, and
+  // their position, -1 for none
+  int axis[CS];
+  int64_t pos[CS];
+  float2 turn[CS];
+#pragma unroll
+  for (int k = 0; k < CS; ++k) {
+    const int i = tid + k * kMrWarps * 32;
+    axis[k] = i < TOK * (D / 2) ? a.axis[i % (D / 2)] : 0;
+  }
+  auto fetch_pos = [&](int group) {
+#pragma unroll
+    for (int k = 0; k < CS; ++k) {
+      const int i = tid + k * kMrWarps * 32, t = group * TOK + i / (D / 2);
+      pos[k] = -1;
+      if (i < TOK * (D / 2) && t < a.num_tokens) {
+        if (axis[k] >= 0 && axis[k] < a.axes) pos[k] = a.positions[axis[k] * a.pos_stride + t];
+        if (pos[k] < 0 || pos[k] >= a.max_position) {
+          raise_flag(a.error_flag, B200ASR_DEVERR_POSITION);
+          pos[k] = 0;
+        }
+      }
+    }
+  };
+  auto fetch_turn = [&]() {
+#pragma unroll
+    for (int k = 0; k < CS; ++k) {
+      const int j = (tid + k * kMrWarps * 32) % (D / 2);
+      turn[k] = make_float2(0.f, 0.f);
+      if (pos[k] >= 0) turn[k] = make_float2(a.cos_sin[pos[k] * D + j], a.cos_sin[pos[k] * D + D / 2 + j]);
+    }
+  };
+  auto put_turn = [&](int buffer) {
+#pragma unroll
+    for (int k = 0; k < CS; ++k) {
+      const int i = tid + k * kMrWarps * 32, tk = i / (D / 2), j = i % (D / 2);
+      if (i < TOK * (D / 2)) {
+        cs_all[buffer][tk][j] = turn[k].x;
+        cs_all[buffer][tk][D / 2 + j] = turn[k].y;
+      }
+    }
+  };
   pdl_wait();
-  bool ready = false;
-  for (int first = warp * STEPS; first < total || !ready; first += kMrWarps * STEPS) {
-    uint4 raw[STEPS];
+  fetch(blockIdx.x, warp * PER);
+  fetch_pos(blockIdx.x);
+  fetch_turn();
+  put_turn(0);
+  __syncthreads();
+
+  int buffer = 0;
+  for (int group = blockIdx.x; group < groups; group += gridDim.x, buffer ^= 1) {
+    const float (*cs)[D] = cs_all[buffer];
+    const int t0 = group * TOK, tokens = min(TOK, a.num_tokens - t0), after = group + gridDim.x;
+    if (after < groups) fetch_pos(after);
+    int slot[TOK];
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int s = first + i, tk = s / steps, head = (s - tk * steps) * PER + lane / LANES;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (s < total && head < heads)
-        raw[i] = *reinterpret_cast<const uint4 *>(a.qkv + (t0 + tk) * a.qkv_stride +
-                                                  static_cast<int64_t>(head) * D + gl * 8);
-    }
-    if (!ready) {
-      for (int i = tid; i < TOK * (D / 2); i += kMrWarps * 32) {
-        const int tk = i / (D / 2), j = i - tk * (D / 2);
-        if (t0 + tk < a.num_tokens) {
-          const int ax = a.axis[j];
-          const bool ax_ok = ax >= 0 && ax < a.axes;
-          int64_t p = ax_ok ? a.positions[ax * a.pos_stride + t0 + tk] : -1;
-          if (p < 0 || p >= a.max_position) {
-            raise_flag(a.error_flag, B200ASR_DEVERR_POSITION);
-            p = 0;
-          }
-          cs[tk][j] = a.cos_sin[p * D + j];
-          cs[tk][D / 2 + j] = a.cos_sin[p * D + D / 2 + j];
-        }
+    for (int i = 0; i < TOK; ++i) {
+      slot[i] = a.slots != nullptr && i < tokens ? a.slots[t0 + i] : -1;
+      if (slot[i] != -1 && (slot[i] < 0 || slot[i] >= a.num_slots)) {
+        if (tid == 0) raise_flag(a.error_flag, B200ASR_DEVERR_SLOT);
+        slot[i] = -1;
       }
-      __syncthreads();
-      ready = true;
     }
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int s = first + i;
-      if (s >= total) break;
-      const int tk = s / steps, head = (s - tk * steps) * PER + lane / LANES;
-      const int64_t t = t0 + tk;
+    bool turned = false;
+    for (int first = warp * PER; first < heads; first += step) {
+      const int head = first + lane / LANES;
       const bool is_q = head < a.num_heads, is_v = head >= a.num_heads + a.num_kv_heads;
-      float x[8];
-      unpack8(raw[i], x);
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(ss * (1.f / D) + a.eps);
-      float w[8];
-      unpack8(*reinterpret_cast<const uint4 *>((is_q ? a.qw : a.kw) + gl * 8), w);
-      const float *row = cs[tk] + (gl & (LANES / 2 - 1)) * 8;
-      const bool low = gl < LANES / 2;
-      uint32_t y[4];
-      float out[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= r * w[e];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_xor_sync(0xffffffffu, x[e], LANES / 2);
-        out[e] = fmaf(x[e], row[e], (low ? -other : other) * row[D / 2 + e]);
+      const bool none = first >= a.num_heads + a.num_kv_heads;  // nothing of the warp's is turned
+      const int h = is_v ? head - a.num_heads - a.num_kv_heads : head - a.num_heads;
+      float2 w[4];
+      {
+        const __nv_bfloat16 *nw = (is_q ? a.qw : a.kw) + gl * 4;
+        const uint2 lo = *reinterpret_cast<const uint2 *>(nw), hi = *reinterpret_cast<const uint2 *>(nw + D / 2);
+        w[0] = unpack2(lo.x);
+        w[1] = unpack2(lo.y);
+        w[2] = unpack2(hi.x);
+        w[3] = unpack2(hi.y);
       }
+      uint32_t v[TOK][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = pack2(out[2 * e], out[2 * e + 1]);
-      const uint4 v = is_v ? raw[i] : make_uint4(y[0], y[1], y[2], y[3]);
-      if (is_q) *reinterpret_cast<uint4 *>(a.q_out + t * a.q_out_stride + static_cast<int64_t>(head) * D + gl * 8) = v;
-      int64_t slot = -1;
-      if (!is_q && head < heads && a.slots != nullptr) {
-        slot = a.slots[t];
-        if (slot != -1 && (slot < 0 || slot >= a.num_slots)) {
-          if (gl == 0) raise_flag(a.error_flag, B200ASR_DEVERR_SLOT);
-          slot = -1;
+      for (int i = 0; i < TOK; ++i) {
+        v[i][0] = raw[i][0].x;
+        v[i][1] = raw[i][0].y;
+        v[i][2] = raw[i][1].x;
+        v[i][3] = raw[i][1].y;
+      }
+      if (first + step < heads) fetch(group, first + step);  // under this step's arithmetic
+      else if (after < groups) fetch(after, warp * PER);
+      if (!none) {
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) {
+          float2 x[4];
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = unpack2(v[i][e]);
+            ss = fmaf(x[e].x, x[e].x, fmaf(x[e].y, x[e].y, ss));
+          }
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float r = rsqrtf(ss * (1.f / D) + a.eps);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e].x *= r * w[e].x;
+            x[e].y *= r * w[e].y;
+          }
+          const float4 c = *reinterpret_cast<const float4 *>(&cs[i][gl * 4]);
+          const float4 s = *reinterpret_cast<const float4 *>(&cs[i][D / 2 + gl * 4]);
+          if (!is_v) {
+            v[i][0] = pack2(x[0].x * c.x - x[2].x * s.x, x[0].y * c.y - x[2].y * s.y);
+            v[i][1] = pack2(x[1].x * c.z - x[3].x * s.z, x[1].y * c.w - x[3].y * s.w);
+            v[i][2] = pack2(x[2].x * c.x + x[0].x * s.x, x[2].y * c.y + x[0].y * s.y);
+            v[i][3] = pack2(x[3].x * c.z + x[1].x * s.z, x[3].y * c.w + x[1].y * s.w);
+          }
         }
       }
-      const int h = is_v ? head - a.num_heads - a.num_kv_heads : head - a.num_heads;
-      if (!KV4) {
-        if (slot >= 0)
-          *reinterpret_cast<uint4 *>((is_v ? a.v_cache : a.k_cache) + (slot * a.num_kv_heads + h) * D + gl * 8) = v;
-      } else if (__any_sync(0xffffffffu, slot >= 0)) {  // the reductions below need every lane
-        const uint32_t rows[4] = {v.x, v.y, v.z, v.w};
-        uint32_t codes[1], sz;
-        kv4_quantise<LANES, 4>(rows, codes, sz);
-        if (slot >= 0) {
-          const int64_t block = slot / a.c.block_size, at = slot - block * a.c.block_size;
-          reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(is_v ? a.c.v_codes : a.c.k_codes) +
-                                       block * a.c.code_stride[0] + at * a.c.code_stride[1] +
-                                       h * a.c.code_stride[2])[gl] = codes[0];
-          if (gl == 0)
-            reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.c.params) +
-                                         block * a.c.param_stride[0] + at * a.c.param_stride[1] +
-                                         h * a.c.param_stride[2])[is_v ? 1 : 0] = sz;
+      if (!turned && after < groups) {
+        fetch_turn();
+        turned = true;
+      }
+      if (is_q) {
+        __nv_bfloat16 *dst = a.q_out + t0 * a.q_out_stride + head * D + gl * 4;
+#pragma unroll
+        for (int i = 0; i < TOK; ++i)
+          if (i < tokens) {
+            *reinterpret_cast<uint2 *>(dst + i * a.q_out_stride) = make_uint2(v[i][0], v[i][1]);
+            *reinterpret_cast<uint2 *>(dst + i * a.q_out_stride + D / 2) = make_uint2(v[i][2], v[i][3]);
+          }
+      }
+      if (a.slots == nullptr || first + PER <= a.num_heads) continue;  // query heads alone
+#pragma unroll
+      for (int i = 0; i < TOK; ++i) {
+        const bool keep = slot[i] >= 0 && !is_q && head < heads;
+        if (!KV4) {
+          if (keep) {
+            __nv_bfloat16 *dst = (is_v ? a.v_cache : a.k_cache) +
+                                 (static_cast<int64_t>(slot[i]) * a.num_kv_heads + h) * D + gl * 4;
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(v[i][0], v[i][1]);
+            *reinterpret_cast<uint2 *>(dst + D / 2) = make_uint2(v[i][2], v[i][3]);
+          }
+        } else if (slot[i] >= 0) {  // as a whole warp: the reductions below need every lane
+          uint32_t codes[1], sz;
+          kv4_quantise<LANES, 4>(v[i], codes, sz);
+          if (keep) {
+            const int block = slot[i] / a.c.block_size, at = slot[i] - block * a.c.block_size;
+            uint16_t *dst = reinterpret_cast<uint16_t *>(
+                static_cast<uint8_t *>(is_v ? a.c.v_codes : a.c.k_codes) + block * a.c.code_stride[0] +
+                at * a.c.code_stride[1] + h * a.c.code_stride[2]);
+            dst[gl] = static_cast<uint16_t>(codes[0]);
+            dst[D / 8 + gl] = static_cast<uint16_t>(codes[0] >> 16);
+            if (gl == 0)
+              reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.c.params) +
+                                           block * a.c.param_stride[0] + at * a.c.param_stride[1] +
+                                           h * a.c.param_stride[2])[is_v ? 1 : 0] = sz;
+          }
         }
       }
     }
+    if (after < groups) {
+      if (!turned) fetch_turn();  // a warp without a head
+      put_turn(buffer ^ 1);
+    }
+    __syncthreads();
   }
 }
 
 template <int LANES, bool KV4>
 int launch_mrope(const MropeArgs &a, cudaStream_t stream) {
-  // One token per CTA while that leaves SMs idle; two, with two steps in flight per warp, from
-  // there on.
+  // One token per CTA while that leaves SMs idle; groups of kMrTok on resident CTAs from there on.
   const bool wide = a.num_tokens > 2 * num_sms();
-  auto kfn = wide ? qk_norm_mrope_store_kernel<LANES, 2, 2, KV4> : qk_norm_mrope_store_kernel<LANES, 1, 1, KV4>;
-  const unsigned grid = wide ? (a.num_tokens + 1) / 2 : a.num_tokens;
+  auto kfn = wide ? qk_norm_mrope_store_kernel<LANES, kMrTok, KV4> : qk_norm_mrope_store_kernel<LANES, 1, KV4>;
+  const int grid = wide ? std::min((a.num_tokens + kMrTok - 1) / kMrTok, kMrCtasPerSm * num_sms()) : a.num_tokens;
   B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(grid), dim3(kMrWarps * 32), 0, stream, true, 1, a),
                         "qk_norm_mrope_store");
   return B200ASR_OK;
@@ -167,7 +257,8 @@ extern "C" int b200asr_qk_norm_mrope_store(
     float eps, const float *cos_sin_cache, int32_t max_position, void *q_out,
     int64_t q_out_row_stride, const int32_t *slot_mapping, void *k_cache, void *v_cache,
     int64_t num_slots, const b200asr_kv4 *cache4, int32_t *error_flag, b200asr_stream_t stream) {
-  B200_REQUIRE(num_tokens >= 0 && num_heads >= 1 && num_kv_heads >= 1 && max_position >= 1 && axes >= 1,
+  B200_REQUIRE(num_tokens >= 0 && num_heads >= 1 && num_kv_heads >= 1 && max_position >= 1 && axes >= 1 &&
+                   num_heads <= 65536 && num_kv_heads <= 65536,
                "qk_norm_mrope_store: bad sizes");
   B200_REQUIRE(head_dim == 64 || head_dim == 128, "qk_norm_mrope_store: head_dim %d unsupported (64 or 128)",
                head_dim);

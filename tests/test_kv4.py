@@ -9,9 +9,10 @@ Tolerances of the attention outputs are element by element, from the roundings t
   D / 16 + 1 additions of 2^-23 each: an absolute error e of the score (base e) changes each
   probability by the factor exp(+-e), so the output by at most 2 e sum_t p_t |v_t - out|
   <= 2 e (sum_t p_t |v_t| + |out|);
-* prefill rounds the cache's values to bf16 as a bf16 cache would hold them: a score (base e)
-  then moves by at most e = 2^-8 |scale| sum_i |q_i k_i| + (the 32-bit part, terms |q_i k_i|),
-  and V by 2^-8 of |v|; its probability alone is rounded, 2^-8 of sum_t p_t |v_t|;
+* prefill takes q, K, V and P as fp16 (2^-11 of the value each; below fp16's smallest normal
+  number, 2^-27 of the largest of a q row or of 32 K rows, 2^-24 for V, which no test reaches
+  unless it says so): a score (base e) moves by at most e = |scale| (2 * 2^-11 + 2^-20)
+  sum_i |q_i k_i|, 2^-20 for the 32-bit sums, and the output by 2 * 2^-11 of sum_t p_t |v_t|;
 * 2^-16 of sum_t p_t (|v_t| + |zero_t|) for the other 32-bit sums, exp2 and the division (up to a
   few hundred additions of 2^-24 each and exp2 within 2^-22).
 """
@@ -72,7 +73,7 @@ def sequence_rows(cache, table, n):
     return k, unpack_codes(vc).astype(np.float64), par[..., 2:3], par[..., 3:4], par[..., 0:1]
 
 
-def plain_attention(q, cache, table, n, scale, prefill=False):
+def plain_attention(q, cache, table, n, scale, prefill=False, bf16_v=False):
     """out [q_len, H, D] and its tolerance, causal with the mask aligned bottom-right."""
     q = q.double().cpu().numpy()
     m, heads, d = q.shape
@@ -94,8 +95,8 @@ def plain_attention(q, cache, table, n, scale, prefill=False):
             o = p @ v[:seen, g]
             mass = p @ np.abs(v[:seen, g])
             if prefill:  # a key's e weighs with its probability
-                e = (2.0 ** -8 + (d / 16 + 1) * 2.0 ** -23) * abs(scale) * (np.abs(k[:seen, g]) @ np.abs(q[i, h]))
-                rounded = 2 * 2.0 ** -8 * mass
+                e = (2 * 2.0 ** -11 + 2.0 ** -20) * abs(scale) * (np.abs(k[:seen, g]) @ np.abs(q[i, h]))
+                rounded = (2 * 2.0 ** -8 if bf16_v else 2 * 2.0 ** -11) * mass
                 moved = (p * e) @ np.abs(v[:seen, g]) + (p @ e) * np.abs(o)  # exp(x) - 1 <= x exp(x)
                 moved = moved * np.exp(e.max())
             else:
@@ -440,9 +441,9 @@ def test_decode_not_finite_rows_reach_only_their_sequence(kx):
 # ------------------------------------------------------------------------------ prefill
 
 
-def check_prefill(kx, q_lens, k_lens, heads, hkv, d, bs, layout="slots", q_scale=1.5, seed=0, scale=None):
+def check_prefill(kx, q_lens, k_lens, heads, hkv, d, bs, layout="slots", q_scale=1.5, seed=0, scale=None, spread=1.0):
     table, blocks = paged(seed, k_lens, bs)
-    cache = filled(seed + 1, blocks, bs, hkv, d, layout)
+    cache = filled(seed + 1, blocks, bs, hkv, d, layout, spread)
     poison_unused(cache, table, k_lens)
     gen = torch.Generator().manual_seed(seed + 2)
     total = sum(q_lens)
@@ -456,7 +457,7 @@ def check_prefill(kx, q_lens, k_lens, heads, hkv, d, bs, layout="slots", q_scale
     assert err.item() == 0 and out[total:].isnan().all()
     at = 0
     for b, (m, n) in enumerate(zip(q_lens, k_lens)):
-        want, tol = plain_attention(q[at:at + m], cache, table[b], n, scale, prefill=True)
+        want, tol = plain_attention(q[at:at + m], cache, table[b], n, scale, prefill=True, bf16_v=spread != 1.0)
         check_close(out[at:at + m], want, tol, f"sequence {b}: {m} rows, {n} keys")
         at += m
 
@@ -480,6 +481,25 @@ def test_prefill_lengths(kx, q_lens, k_lens):
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
 def test_prefill_scales(kx, scale):
     check_prefill(kx, [70, 1], [200, 140], 4, 2, 128, 256, seed=5, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spread,q_scale", [(1e-5, 1e5), (1e6, 1e-6), (1e30, 1e-30), (1e-30, 1e30)])
+def test_prefill_values_outside_fp16(kx, spread, q_scale):
+    """K and V of any size of bf16 (V then goes through as bf16, 2^-8 for it and for P)."""
+    check_prefill(kx, [70, 1], [200, 140], 4, 2, 128, 256, seed=5, spread=spread, q_scale=q_scale)
+
+
+@pytest.mark.gpu
+def test_decode_values_of_any_size(kx):
+    for spread in (1e-30, 1e-5, 1e6, 1e30):
+        table, blocks = paged(3, [700, 33], 256)
+        cache = filled(4, blocks, 256, 2, 128, spread=spread)
+        q = (torch.randn(2, 4, 128, device="cuda") / spread).bfloat16()
+        out = run_decode(kx, q, cache, table, [700, 33], 0.08)
+        for b, n in enumerate((700, 33)):
+            want, tol = plain_attention(q[b:b + 1], cache, table[b], n, 0.08)
+            check_close(out[b:b + 1], want, tol, f"spread {spread}, row {b}")
 
 
 @pytest.mark.gpu

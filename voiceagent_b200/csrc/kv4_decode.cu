@@ -461,8 +461,8 @@ __global__ void __launch_bounds__(kD4Warps * 32, NT == 1 ? kD4CtasPerSm : 2)
       even += __shfl_xor_sync(0xffffffffu, even, 2);
       odd += __shfl_xor_sync(0xffffffffu, odd, 2);
       const float start = -1024.f * even - 64.f * odd;
-      // (at least 1e-30: a scale of zero must not meet the -inf of masked tokens)
-      const float factor = fmaxf(1e-30f, a.scale_log2 * __int_as_float((127 - ex) << 23));
+      // (not zero, for a scale of zero must not meet the -inf of masked tokens)
+      const float factor = fmaxf(1e-37f, a.scale_log2 * __int_as_float((127 - ex) << 23));
       const float sum = even + odd;
       c0[n] = __shfl_sync(0xffffffffu, start, 8 * t);  // column 2t: lanes with g = 2t
       c1[n] = __shfl_sync(0xffffffffu, start, 8 * t + 4);

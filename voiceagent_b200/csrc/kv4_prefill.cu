@@ -19,10 +19,18 @@
 //  * Online softmax with a lazy maximum: it moves only when a row passes it by 2^8.
 //  * A word of 8 codes gives the pairs (i, i + 4), so dims are permuted within groups of 8;
 //    q is laid out alike, and the output is put back in order as it is written.
-//  * K and V values are rounded to bf16 (2^-9 of the value, the precision of a bf16 cache); they
-//    are zero + code * scale in one rounding.
+//  * Values are zero + code * scale in one rounding, and q, K, V and P go through the tensor
+//    cores as fp16, 11 bits where bf16 keeps 8 (error of the output against 64 bits, relative:
+//    0.0042 with bf16, of which the output's own rounding is 0.0017). q is brought to fp16's
+//    range by a power of two per row, K by one per 32 tokens, both undone in the factor of the
+//    scores. V carries no such factor, so 32 tokens whose V rows do not lie within
+//    [2^-10, 2^15] (or are zero) go through as bf16, with their P.
 //  * A V row that is not finite is written as zeros and its K row as NaN: the rows that may
 //    attend it become NaN, those that may not keep their values (0 * NaN would reach them).
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace b200asr {
@@ -128,19 +136,46 @@ __device__ __forceinline__ void p4_tmem_st16(uint32_t taddr, const uint32_t *v) 
       : "memory");
 }
 
-// 8 codes as four bf16 pairs of values, dims (i, i + 4): zero + code * scale.
-__device__ __forceinline__ uint4 p4_values(uint32_t w, __nv_bfloat162 scale, __nv_bfloat162 zero) {
+__device__ __forceinline__ uint32_t p4_and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
+__device__ __forceinline__ uint32_t p4_f16x2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 8 codes as four pairs of values zero + code * scale, dims (i, i + 4); bf16 from 128 + code.
+__device__ __forceinline__ uint4 p4_values_bf16(uint32_t w, uint32_t scale2, uint32_t zero2) {
   uint32_t out[4];
   const uint32_t k = 0xc300c300u;  // -128, -128
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t p = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;  // 128 + code
+    const uint32_t p = p4_and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
     __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&p);
     x = __hadd2(x, *reinterpret_cast<const __nv_bfloat162 *>(&k));  // code, exact
-    x = __hfma2(x, scale, zero);
+    x = __hfma2(x, *reinterpret_cast<const __nv_bfloat162 *>(&scale2), *reinterpret_cast<const __nv_bfloat162 *>(&zero2));
     out[i] = *reinterpret_cast<uint32_t *>(&x);
   }
   return make_uint4(out[0], out[1], out[2], out[3]);
+}
+// The same in fp16, from 1024 + code and, in place, 1024 + 16 code with a sixteenth of the scale.
+__device__ __forceinline__ uint4 p4_values_f16(uint32_t w, uint32_t scale2, uint32_t scale16, uint32_t zero2) {
+  uint32_t out[4];
+  const uint32_t k = 0xe400e400u;  // -1024, -1024
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t p = p4_and_or(i & 2 ? w >> 8 : w, i & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
+    __half2 x = *reinterpret_cast<const __half2 *>(&p);
+    x = __hadd2(x, *reinterpret_cast<const __half2 *>(&k));  // code or 16 code, exact
+    x = __hfma2(x, *reinterpret_cast<const __half2 *>(i & 1 ? &scale16 : &scale2), *reinterpret_cast<const __half2 *>(&zero2));
+    out[i] = *reinterpret_cast<uint32_t *>(&x);
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+// Instruction descriptor: kind::f16 with fp16 A and B (common.cuh has the bf16 form).
+__host__ __device__ constexpr uint32_t p4_idesc_f16(int m, int n, bool b_mn_major) {
+  return idesc_bf16_f32(m, n, false, b_mn_major) & ~((1u << 7) | (1u << 10));
 }
 
 template <int D>
@@ -159,6 +194,10 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   uint64_t *o_full = bars + 14;       // [2] the item's last P V done
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
   __shared__ int abort_flag;
+  // Per K/V tile (global count, modulo 4) and 32 tokens of it: what undoes K's power of two,
+  // negative where V and P are bf16. Four tiles deep: a tile's entry is written anew only after
+  // the V tile three before has been waited for, so after both softmaxes of the tile itself.
+  __shared__ float chunk_factor[4][4];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
@@ -202,29 +241,48 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
     const int w = warp >> 2, r = tid & 127;
     const uint32_t s_base = tmem + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t o_base = tmem + 256 + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // this thread's row of q into the tile, dims in the order of the codes' pairs
-    auto load_q = [&](const Item4 &t) {
+    // This thread's row of q into the tile, dims in the order of the codes' pairs, times the power
+    // of two that brings its largest into [2^13, 2^14); gives the factor of the row's scores.
+    auto load_q = [&](const Item4 &t) -> float {
       const int row = w * 128 + r;
       const bool in = row < t.rows;
       const int tok = in ? (t.row0 + row) / a.group : 0, head = in ? (t.row0 + row) - tok * a.group : 0;
       const __nv_bfloat16 *src = a.q + (t.q0 + tok) * a.q_row + (static_cast<int64_t>(t.h) * a.group + head) * a.q_head;
       uint8_t *dst = sQ + w * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
-#pragma unroll
+      float top = 0.f;
+#pragma unroll 4
       for (int j = 0; j < D / 8; ++j) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (in) u = *reinterpret_cast<const uint4 *>(src + j * 8);
-        const uint4 v = make_uint4(__byte_perm(u.x, u.z, 0x5410) ^ a.flip, __byte_perm(u.x, u.z, 0x7632) ^ a.flip,
-                                   __byte_perm(u.y, u.w, 0x5410) ^ a.flip, __byte_perm(u.y, u.w, 0x7632) ^ a.flip);
-        *reinterpret_cast<uint4 *>(dst + (j >> 3) * C::BLOCK + (((j & 7) ^ (r & 7)) << 4)) = v;
+        float f[8];
+        unpack8(u, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+      }
+      const int ex = min(100, max(-114, 13 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
+      const float up = __int_as_float(((ex + 127) << 23) | a.flip);
+#pragma unroll 4
+      for (int j = 0; j < D / 8; ++j) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (in) u = *reinterpret_cast<const uint4 *>(src + j * 8);
+        float f[8];
+        unpack8(u, f);
+        *reinterpret_cast<uint4 *>(dst + (j >> 3) * C::BLOCK + (((j & 7) ^ (r & 7)) << 4)) =
+            make_uint4(p4_f16x2(f[0] * up, f[4] * up), p4_f16x2(f[1] * up, f[5] * up),
+                       p4_f16x2(f[2] * up, f[6] * up), p4_f16x2(f[3] * up, f[7] * up));
       }
       fence_proxy_async_smem();
       arrive(&q_full[w]);
+      return a.scale_log2 * __int_as_float((127 - ex) << 23);
     };
-    uint32_t ps = 0, po = 0;  // phases of this tile's scores and outputs
+    uint32_t ps = 0, po = 0;  // phases of this row tile's scores and outputs
+    uint32_t jg = 0;          // K/V tiles of the items so far
+    float next_factor = 0.f;
     bool more = walk.next(a, it);
-    if (more && it.tiles > 0 && w * 128 < it.rows) load_q(it);
+    if (more && it.tiles > 0 && w * 128 < it.rows) next_factor = load_q(it);
     while (more) {
       const Item4 cur = it;
+      const float factor = next_factor;
       const bool mine = cur.tiles > 0 && w * 128 < cur.rows;
       const int row = w * 128 + r;
       const int tok = (cur.row0 + row) / a.group;
@@ -235,6 +293,74 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
       const int all_seen = min(cur.offset + first_row / a.group, cur.n_kv - 1);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
+      // One tile: scores to P. MASKED where some row of the warp does not see all its keys.
+      auto softmax_tile = [&](auto masked, int j, const float *factors) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const int lim = last - j * kP4Keys;  // the last column this row sees
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          float s[64];
+          tmem_ld32(s_base + c, s);
+          tmem_ld32(s_base + c + 32, s + 32);
+          tmem_wait_ld();
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              x = fmaxf(x, !MASKED || c + hf * 32 + i <= lim ? s[hf * 32 + i] : -INFINITY);
+            mx = fmaxf(mx, x * (factor * fabsf(factors[(c >> 5) + hf])));
+          }
+        }
+        const bool move = mx > m + kP4Lazy || m == -INFINITY;
+        const float m_new = move ? fmaxf(m, mx) : m;
+        const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
+        if (j > 0 && __any_sync(0xffffffffu, move && alpha != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            tmem_ld32(o_base + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= alpha;
+            tmem_st32(o_base + c, o);
+          }
+        }
+        m = m_new;
+        l *= alpha;
+        const float shift = m == -INFINITY ? 0.f : -m;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          float s[64];
+          tmem_ld32(s_base + c, s);
+          tmem_ld32(s_base + c + 32, s + 32);
+          tmem_wait_ld();
+          uint32_t p[32];
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float fc = factors[(c >> 5) + hf], f = factor * fabsf(fc);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float e = exp2f(fmaf(s[hf * 32 + i], f, shift));
+              s[hf * 32 + i] = !MASKED || c + hf * 32 + i <= lim ? e : 0.f;
+              sum[i & 3] += s[hf * 32 + i];
+            }
+            if (fc > 0.f) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) p[hf * 16 + i] = p4_f16x2(s[hf * 32 + 2 * i], s[hf * 32 + 2 * i + 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) p[hf * 16 + i] = pack2(s[hf * 32 + 2 * i], s[hf * 32 + 2 * i + 1]);
+            }
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          p4_tmem_st16(s_base + c / 2, p);  // over scores already read
+          p4_tmem_st16(s_base + c / 2 + 16, p + 16);
+        }
+        tmem_wait_st();
+      };
       if (mine) {
         for (int j = 0; j < cur.tiles; ++j, ++ps) {
           if (!wait(&s_full[w], ps)) {
@@ -243,78 +369,21 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
           }
           tc_fence_after();
           if (warp_rows) {
-            const int key0 = j * kP4Keys;
-            const bool whole = key0 + kP4Keys - 1 <= all_seen;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-              float s[32];
-              tmem_ld32(s_base + c, s);
-              tmem_wait_ld();
-              if (whole) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, s[i]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, key0 + c + i <= last ? s[i] : -INFINITY);
-              }
-            }
-            mx *= a.scale_log2;
-            if (mx != mx) mx = -INFINITY;  // -inf * 0
-            const bool move = mx > m + kP4Lazy || m == -INFINITY;
-            const float m_new = move ? fmaxf(m, mx) : m;
-            const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
-            if (j > 0 && __any_sync(0xffffffffu, move && alpha != 1.f)) {
-#pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                float o[32];
-                tmem_ld32(o_base + c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= alpha;
-                tmem_st32(o_base + c, o);
-              }
-            }
-            m = m_new;
-            l *= alpha;
-            const float shift = m == -INFINITY ? 0.f : -m;
-#pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-              float s[32];
-              tmem_ld32(s_base + c, s);
-              tmem_wait_ld();
-              if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (key0 + c + i > last) s[i] = -INFINITY;
-              }
-              uint32_t p[16];
-              float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float p0 = exp2f(fmaf(s[2 * i], a.scale_log2, shift));
-                float p1 = exp2f(fmaf(s[2 * i + 1], a.scale_log2, shift));
-                if (!whole) {  // -inf * 0 where the scale is zero
-                  if (key0 + c + 2 * i > last) p0 = 0.f;
-                  if (key0 + c + 2 * i + 1 > last) p1 = 0.f;
-                }
-                sum0 += p0;
-                sum1 += p1;
-                p[i] = pack2(p0, p1);
-              }
-              l += sum0 + sum1;
-              p4_tmem_st16(s_base + c / 2, p);  // over scores already read
-            }
-            tmem_wait_st();
+            const float *factors = chunk_factor[(jg + j) & 3];
+            if (__all_sync(0xffffffffu, j * kP4Keys + kP4Keys - 1 <= all_seen))
+              softmax_tile(std::false_type(), j, factors);
+            else
+              softmax_tile(std::true_type(), j, factors);
           }
           tc_fence_before();
           arrive(&p_full[w]);
         }
       }
+      jg += cur.tiles;
       if (!ok) break;
       // the next item's rows while this one's last product runs: its scores are done with Q
       more = walk.next(a, it);
-      if (more && it.tiles > 0 && w * 128 < it.rows) load_q(it);
+      if (more && it.tiles > 0 && w * 128 < it.rows) next_factor = load_q(it);
       if (mine) {
         if (!wait(&o_full[w], po)) break;
         ++po;
@@ -405,10 +474,28 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
           }
         }
         if (j + 1 < it.tiles) fetch(j + 1);
-        auto write = [&](uint8_t *tile, const uint4 &codes, uint32_t sz, int row) {
-          const uint32_t s2 = __byte_perm(sz, sz, 0x1010), z2 = __byte_perm(sz, sz, 0x3232);
-          const __nv_bfloat162 scale = *reinterpret_cast<const __nv_bfloat162 *>(&s2);
-          const __nv_bfloat162 zero = *reinterpret_cast<const __nv_bfloat162 *>(&z2);
+        // K's power of two: the warp's 32 rows' largest into [2^13, 2^14). V in fp16 if its rows
+        // allow it.
+        float top = 0.f;
+        bool v16 = true;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const float2 kp = unpack2(p0[i].x), vp = unpack2(p0[i].y);
+          const float kb = fmaf(15.f, fabsf(kp.x), fabsf(kp.y));
+          if (kb < INFINITY) top = fmaxf(top, kb);  // (not NaN)
+          const float vb = fmaxf(fabsf(vp.y), fabsf(fmaf(15.f, vp.x, vp.y)));
+          v16 = v16 && (vb == 0.f || (vb >= 0x1p-10f && vb <= 0x1p15f));
+        }
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        v16 = __all_sync(0xffffffffu, v16);
+        const int ex = min(100, max(-114, 13 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
+        const float up = __int_as_float((ex + 127) << 23);
+        if (lane == 0) {
+          const float down = __int_as_float((127 - ex) << 23);
+          chunk_factor[jg & 3][warp - 8] = v16 ? down : -down;
+        }
+        // one row's 16 bytes of codes: four 16-byte pieces of values, at their swizzled places
+        auto write = [&](uint8_t *tile, const uint4 &codes, int row, auto values) {
           const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
           uint8_t *dst = tile + (t >> 1) * (D == 128 ? C::BLOCK : 0) + (row >> 3) * 1024 + (row & 7) * 128;
           const int turn = D == 128 ? t >> 1 : 0;  // halves of a row in different banks
@@ -416,31 +503,45 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
           for (int i = 0; i < 4; ++i) {
             const uint32_t x = turn ? word[i ^ 1] : word[i];
             const int ch = (t & 1) * 4 + (i ^ turn);
-            *reinterpret_cast<uint4 *>(dst + ((ch ^ (row & 7)) << 4)) = p4_values(x, scale, zero);
+            *reinterpret_cast<uint4 *>(dst + ((ch ^ (row & 7)) << 4)) = values(x);
           }
+        };
+        auto write16 = [&](uint8_t *tile, const uint4 &codes, uint32_t sz, float by, int row) {
+          const float2 f = unpack2(sz);
+          const uint32_t s2 = p4_f16x2(f.x * by, f.x * by), z2 = p4_f16x2(f.y * by, f.y * by);
+          const uint32_t s16 = p4_f16x2(f.x * by * 0.0625f, f.x * by * 0.0625f);
+          write(tile, codes, row, [&](uint32_t x) { return p4_values_f16(x, s2, s16, z2); });
         };
         if (!wait(&k_empty[st], (jg >> 1) ^ 1)) {
           ok = false;
           break;
         }
 #pragma unroll
-        for (int i = 0; i < CH; ++i) write(sK + st * C::TILE, k0[i], p0[i].x, row0 + i * PER);
+        for (int i = 0; i < CH; ++i) write16(sK + st * C::TILE, k0[i], p0[i].x, up, row0 + i * PER);
         fence_proxy_async_smem();
         arrive(&k_full[st]);
         if (!wait(&v_empty[st], (jg >> 1) ^ 1)) {
           ok = false;
           break;
         }
+        if (v16) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) write(sV + st * C::TILE, v0[i], p0[i].y, row0 + i * PER);
+          for (int i = 0; i < CH; ++i) write16(sV + st * C::TILE, v0[i], p0[i].y, 1.f, row0 + i * PER);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < CH; ++i) {
+            const uint32_t sz = p0[i].y, s2 = __byte_perm(sz, sz, 0x1010), z2 = __byte_perm(sz, sz, 0x3232);
+            write(sV + st * C::TILE, v0[i], row0 + i * PER, [&](uint32_t x) { return p4_values_bf16(x, s2, z2); });
+          }
+        }
         fence_proxy_async_smem();
         arrive(&v_full[st]);
       }
     }
   } else {
     // ---------------------------------------------------------------------- MMAs
-    constexpr uint32_t idesc_s = idesc_bf16_f32(128, kP4Keys, false, false);
-    constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true);
+    constexpr uint32_t idesc_s = p4_idesc_f16(128, kP4Keys, false);
+    constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true), idesc_o16 = p4_idesc_f16(128, D, true);
     const uint32_t q_s = smem_addr(sQ), k_s = smem_addr(sK), v_s = smem_addr(sV);
     uint32_t jg = 0, items = 0, items1 = 0, tile0 = 0, tile1 = 0;
     bool ok = true;
@@ -484,7 +585,8 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
 #pragma unroll
             for (int k = 0; k < kP4Keys / 16; ++k)
               p4_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8,
-                        smem_desc_sw128(v_s + (jg & 1) * C::TILE + k * 2048, C::BLOCK, 1024), idesc_o,
+                        smem_desc_sw128(v_s + (jg & 1) * C::TILE + k * 2048, C::BLOCK, 1024),
+                        chunk_factor[jg & 3][k >> 1] > 0.f ? idesc_o16 : idesc_o,
                         (j > 0 || k > 0) ? 1u : 0u);
             if (w == tiles_w - 1) umma_commit(&v_empty[jg & 1]);
             if (j == it.tiles - 1) umma_commit(&o_full[w]);

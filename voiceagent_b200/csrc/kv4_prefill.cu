@@ -118,12 +118,33 @@ struct Walk4 {
   }
 };
 
+// Products and commits by one elected lane of a converged warp, so that descriptors stay in
+// uniform registers: with a branch around them for one lane, issuing eight took ~1000 cycles
+// beside three busy warps, twice what they run.
+__device__ __forceinline__ void p4_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A from TMEM.
 __device__ __forceinline__ void p4_mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void p4_commit(uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
       : "memory");
 }
 
@@ -197,7 +218,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   // Per K/V tile (global count, modulo 4) and 32 tokens of it: what undoes K's power of two,
   // negative where V and P are bf16. Four tiles deep: a tile's entry is written anew only after
   // the V tile three before has been waited for, so after both softmaxes of the tile itself.
-  __shared__ float chunk_factor[4][4];
+  __shared__ __align__(16) float chunk_factor[4][4];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
@@ -542,20 +563,23 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
     // ---------------------------------------------------------------------- MMAs
     constexpr uint32_t idesc_s = p4_idesc_f16(128, kP4Keys, false);
     constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true), idesc_o16 = p4_idesc_f16(128, D, true);
-    const uint32_t q_s = smem_addr(sQ), k_s = smem_addr(sK), v_s = smem_addr(sV);
+    uint64_t q_desc[2], k_desc[2], v_desc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      q_desc[i] = smem_desc_sw128(smem_addr(sQ + i * C::TILE), 16, 1024);
+      k_desc[i] = smem_desc_sw128(smem_addr(sK + i * C::TILE), 16, 1024);
+      v_desc[i] = smem_desc_sw128(smem_addr(sV + i * C::TILE), C::BLOCK, 1024);
+    }
     uint32_t jg = 0, items = 0, items1 = 0, tile0 = 0, tile1 = 0;
     bool ok = true;
     auto scores = [&](int w, uint32_t jj) {  // S_w = Q_w K^T of global tile jj
-      if (lane == 0) {
+      const uint64_t qd = w ? q_desc[1] : q_desc[0], kd = jj & 1 ? k_desc[1] : k_desc[0];
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * C::BLOCK + (k & 3) * 32;
-          umma_f16_ss(tmem + w * 128, smem_desc_sw128(q_s + w * C::TILE + off, 16, 1024),
-                      smem_desc_sw128(k_s + (jj & 1) * C::TILE + off, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[w]);
+      for (int k = 0; k < D / 16; ++k) {
+        const uint64_t off = ((k >> 2) * C::BLOCK + (k & 3) * 32) >> 4;
+        p4_mma_ss(tmem + w * 128, qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
       }
-      __syncwarp();
+      p4_commit(&s_full[w]);
     };
     while (ok && walk.next(a, it)) {
       if (it.cut && lane == 0) raise_flag(a.error_flag, B200ASR_DEVERR_LENGTH);
@@ -571,7 +595,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
         tc_fence_after();
         scores(1, jg);
       }
-      if (lane == 0) umma_commit(&k_empty[jg & 1]);
+      p4_commit(&k_empty[jg & 1]);
       for (int j = 0; j < it.tiles && ok; ++j, ++jg) {
         for (int w = 0; w < tiles_w && ok; ++w) {
           ok = wait(&p_full[w], w ? tile1 : tile0);
@@ -581,23 +605,22 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
           if (w == 0) ok = wait(&v_full[jg & 1], jg >> 1);
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
+          const float4 f = *reinterpret_cast<const float4 *>(chunk_factor[jg & 3]);
+          const uint32_t ids[4] = {f.x > 0.f ? idesc_o16 : idesc_o, f.y > 0.f ? idesc_o16 : idesc_o,
+                                   f.z > 0.f ? idesc_o16 : idesc_o, f.w > 0.f ? idesc_o16 : idesc_o};
+          const uint64_t vd = jg & 1 ? v_desc[1] : v_desc[0];
 #pragma unroll
-            for (int k = 0; k < kP4Keys / 16; ++k)
-              p4_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8,
-                        smem_desc_sw128(v_s + (jg & 1) * C::TILE + k * 2048, C::BLOCK, 1024),
-                        chunk_factor[jg & 3][k >> 1] > 0.f ? idesc_o16 : idesc_o,
-                        (j > 0 || k > 0) ? 1u : 0u);
-            if (w == tiles_w - 1) umma_commit(&v_empty[jg & 1]);
-            if (j == it.tiles - 1) umma_commit(&o_full[w]);
-          }
-          __syncwarp();
+          for (int k = 0; k < kP4Keys / 16; ++k)
+            p4_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, vd + ((k * 2048) >> 4), ids[k >> 1],
+                      (j > 0 || k > 0) ? 1u : 0u);
+          if (w == tiles_w - 1) p4_commit(&v_empty[jg & 1]);
+          if (j == it.tiles - 1) p4_commit(&o_full[w]);
           if (j + 1 < it.tiles) {
             if (w == 0) ok = wait(&k_full[(jg + 1) & 1], (jg + 1) >> 1);
             if (!ok) break;
             tc_fence_after();
             scores(w, jg + 1);
-            if (w == tiles_w - 1 && lane == 0) umma_commit(&k_empty[(jg + 1) & 1]);
+            if (w == tiles_w - 1) p4_commit(&k_empty[(jg + 1) & 1]);
           }
         }
       }

@@ -35,7 +35,7 @@
 
 namespace b200asr {
 
-constexpr int kP4Threads = 13 * 32;
+constexpr int kP4Threads = 16 * 32;  // warps 13 to 15 only give their registers away
 constexpr int kP4Rows = 256, kP4Keys = 128;
 constexpr float kP4Lazy = 8.f;
 
@@ -157,6 +157,38 @@ __device__ __forceinline__ void p4_tmem_st16(uint32_t taddr, const uint32_t *v) 
       : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void p4_more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void p4_fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// Registers of a softmax, a converting and an MMA thread: what the launch has, 512 x 128.
+constexpr int kP4RegSoftmax = 144, kP4RegConvert = 128, kP4RegMma = 96;
+static_assert(256 * kP4RegSoftmax + 128 * kP4RegConvert + 128 * kP4RegMma <= 512 * 128,
+              "more registers than the block was launched with: the wait for them would not end");
+
+// Two neighbouring numbers at a time: s * f + b, and sums.
+__device__ __forceinline__ float2 p4_fma2(float2 s, float2 f, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, c, d, e;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\tmov.b64 d, {%6, %7};\n\t"
+      "fma.rn.f32x2 e, a, c, d;\n\tmov.b64 {%0, %1}, e;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(s.x), "f"(s.y), "f"(f.x), "f"(f.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+__device__ __forceinline__ float2 p4_add2(float2 s, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, c, e;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\t"
+      "add.rn.f32x2 e, a, c;\n\tmov.b64 {%0, %1}, e;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(s.x), "f"(s.y), "f"(b.x), "f"(b.y));
+  return y;
+}
 __device__ __forceinline__ uint32_t p4_and_or(uint32_t x, uint32_t mask, uint32_t bits) {
   uint32_t y;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
@@ -259,6 +291,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
 
   if (warp < 8) {
     // ------------------------------------------------------------------ softmax
+    p4_more_registers<kP4RegSoftmax>();
     const int w = warp >> 2, r = tid & 127;
     const uint32_t s_base = tmem + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t o_base = tmem + 256 + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -319,20 +352,18 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
         constexpr bool MASKED = decltype(masked)::value;
         const int lim = last - j * kP4Keys;  // the last column this row sees
         float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 64) {
-          float s[64];
-          tmem_ld32(s_base + c, s);
-          tmem_ld32(s_base + c + 32, s + 32);
+        float s[2][32];  // 32 columns at hand and the next 32 on their way
+        tmem_ld32(s_base, s[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
           tmem_wait_ld();
+          tmem_ld32(s_base + ((c + 1) & 3) * 32, s[(c + 1) & 1]);
+          const float *x = s[c & 1];
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            float x = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              x = fmaxf(x, !MASKED || c + hf * 32 + i <= lim ? s[hf * 32 + i] : -INFINITY);
-            mx = fmaxf(mx, x * (factor * fabsf(factors[(c >> 5) + hf])));
-          }
+          for (int i = 0; i < 32; ++i)
+            top[i & 3] = fmaxf(top[i & 3], !MASKED || c * 32 + i <= lim ? x[i] : -INFINITY);
+          mx = fmaxf(mx, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (factor * fabsf(factors[c])));
         }
         const bool move = mx > m + kP4Lazy || m == -INFINITY;
         const float m_new = move ? fmaxf(m, mx) : m;
@@ -351,35 +382,37 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
         m = m_new;
         l *= alpha;
         const float shift = m == -INFINITY ? 0.f : -m;
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 64) {
-          float s[64];
-          tmem_ld32(s_base + c, s);
-          tmem_ld32(s_base + c + 32, s + 32);
-          tmem_wait_ld();
-          uint32_t p[32];
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const float fc = factors[(c >> 5) + hf], f = factor * fabsf(fc);
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld();  // (columns 0 to 31 again since the maxima)
+          if (c < 3) tmem_ld32(s_base + (c + 1) * 32, s[(c + 1) & 1]);
+          const float *x = s[c & 1];
+          const float fc = factors[c], f = factor * fabsf(fc);
+          uint32_t p[16];
+          float2 e[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float e = exp2f(fmaf(s[hf * 32 + i], f, shift));
-              s[hf * 32 + i] = !MASKED || c + hf * 32 + i <= lim ? e : 0.f;
-              sum[i & 3] += s[hf * 32 + i];
-            }
-            if (fc > 0.f) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) p[hf * 16 + i] = p4_f16x2(s[hf * 32 + 2 * i], s[hf * 32 + 2 * i + 1]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) p[hf * 16 + i] = pack2(s[hf * 32 + 2 * i], s[hf * 32 + 2 * i + 1]);
+          for (int i = 0; i < 16; ++i) {
+            e[i] = p4_fma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(f, f), make_float2(shift, shift));
+            e[i].x = exp2f(e[i].x);
+            e[i].y = exp2f(e[i].y);
+            if (MASKED) {
+              if (c * 32 + 2 * i > lim) e[i].x = 0.f;
+              if (c * 32 + 2 * i + 1 > lim) e[i].y = 0.f;
             }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          p4_tmem_st16(s_base + c / 2, p);  // over scores already read
-          p4_tmem_st16(s_base + c / 2 + 16, p + 16);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[i & 1] = p4_add2(sum[i & 1], e[i]);
+          if (fc > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = p4_f16x2(e[i].x, e[i].y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = pack2(e[i].x, e[i].y);
+          }
+          p4_tmem_st16(s_base + c * 16, p);  // over scores already read
         }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
       };
       if (mine) {
@@ -440,7 +473,8 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
       }
     }
   } else if (warp < 12) {
-    // -------------------------------------------------------- codes to bf16 tiles
+    // ------------------------------------------------------ codes to tiles of values
+    p4_fewer_registers<kP4RegConvert>();
     constexpr int CH = D / 32;            // 16-byte pieces of a row, and rounds of a warp's 32 rows
     constexpr int PER = 32 / CH;          // rows of a round
     const int t = lane % CH, rr = lane / CH;
@@ -561,6 +595,8 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
     }
   } else {
     // ---------------------------------------------------------------------- MMAs
+    p4_fewer_registers<kP4RegMma>();
+    if (warp == 12) {
     constexpr uint32_t idesc_s = p4_idesc_f16(128, kP4Keys, false);
     constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true), idesc_o16 = p4_idesc_f16(128, D, true);
     uint64_t q_desc[2], k_desc[2], v_desc[2];
@@ -626,6 +662,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
       }
       ++items;
       if (tiles_w == 2) ++items1;
+    }
     }
   }
 

@@ -475,49 +475,88 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   } else if (warp < 12) {
     // ------------------------------------------------------ codes to tiles of values
     p4_fewer_registers<kP4RegConvert>();
-    constexpr int CH = D / 32;            // 16-byte pieces of a row, and rounds of a warp's 32 rows
-    constexpr int PER = 32 / CH;          // rows of a round
+    constexpr int CH = D / 32;            // 16-byte pieces of a row
+    constexpr int PER = 32 / CH;          // rows of a warp's load
+    constexpr int N = 32 / PER;           // loads for its 32 rows
     const int t = lane % CH, rr = lane / CH;
     // rows of one shared-memory phase differ in the swizzle
     const int sub = D == 128 ? (rr & 4) | ((rr & 1) << 1) | ((rr >> 1) & 1) : rr;
     const int row0 = (warp - 8) * 32 + sub;
+    // Blocks of whole 32-token pieces: a warp's rows lie in one, whose table entry is read two
+    // tiles ahead, so that no load waits for another.
+    const bool even_blocks = a.bs_shift >= 5;
+    const int64_t step_off = PER * a.c.code_stride[1], step_poff = PER * a.c.param_stride[1];
     uint32_t jg = 0;
     bool ok = true;
     while (ok && walk.next(a, it)) {
       if (it.tiles == 0) continue;
       const int32_t *table = a.block_tables + it.b * a.bt_stride;
-      uint4 kr[CH], vr[CH];
-      uint2 pr[CH];
-      auto fetch = [&](int j) {
+      const int64_t head_off = it.h * a.c.code_stride[2] + t * 16, head_poff = it.h * a.c.param_stride[2];
+      uint4 kr[N], vr[N];
+      uint2 pr[N];
+      auto entry = [&](int j) -> int {  // the block of the warp's rows of tile j
+        const int key = j * kP4Keys + (warp - 8) * 32;
+        return even_blocks && key < it.n_kv ? table[key >> a.bs_shift] : 0;
+      };
+      auto usable = [&](int block) -> int {
+        if (block >= 0 && block < a.c.num_blocks) return block;
+        raise_flag(a.error_flag, B200ASR_DEVERR_BLOCK);
+        return 0;
+      };
+      auto fetch = [&](int j, int block) {
+        const int first = j * kP4Keys + row0;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int key = j * kP4Keys + row0 + i * PER;
+        for (int i = 0; i < N; ++i) {
           kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
           pr[i] = make_uint2(0, 0);
+        }
+        if (even_blocks) {
+          const int at = first & (a.c.block_size - 1);
+          block = usable(block);
+          const int64_t off = block * a.c.code_stride[0] + at * a.c.code_stride[1] + head_off;
+          const int64_t poff = block * a.c.param_stride[0] + at * a.c.param_stride[1] + head_poff;
+          const uint8_t *kp = static_cast<const uint8_t *>(a.c.k_codes) + off;
+          const uint8_t *vp = static_cast<const uint8_t *>(a.c.v_codes) + off;
+          const __nv_bfloat16 *pp = static_cast<const __nv_bfloat16 *>(a.c.params) + poff;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (first + i * PER < it.n_kv) {
+              kr[i] = *reinterpret_cast<const uint4 *>(kp + i * step_off);
+              vr[i] = *reinterpret_cast<const uint4 *>(vp + i * step_off);
+              pr[i] = *reinterpret_cast<const uint2 *>(pp + i * step_poff);
+            }
+          return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+          const int key = first + i * PER;
           if (key < it.n_kv) {
             const int page = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.c.block_size;
-            const int at = a.bs_shift >= 0 ? key & (a.c.block_size - 1) : key - page * a.c.block_size;
-            int block = table[page];
-            if (block < 0 || block >= a.c.num_blocks) {
-              raise_flag(a.error_flag, B200ASR_DEVERR_BLOCK);
-              block = 0;
-            }
-            const int64_t off = block * a.c.code_stride[0] + at * a.c.code_stride[1] + it.h * a.c.code_stride[2] + t * 16;
-            kr[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.c.k_codes) + off);
-            vr[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.c.v_codes) + off);
-            pr[i] = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.c.params) +
-                                                     block * a.c.param_stride[0] + at * a.c.param_stride[1] +
-                                                     it.h * a.c.param_stride[2]);
+            const int at = key - page * a.c.block_size, blk = usable(table[page]);
+            const int64_t off = blk * a.c.code_stride[0] + at * a.c.code_stride[1] + head_off;
+            const uint4 k = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.c.k_codes) + off);
+            const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.c.v_codes) + off);
+            const uint2 z = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.c.params) +
+                                                             blk * a.c.param_stride[0] + at * a.c.param_stride[1] +
+                                                             head_poff);
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+              if (n == i) {
+                kr[n] = k;
+                vr[n] = v;
+                pr[n] = z;
+              }
           }
         }
       };
-      fetch(0);
+      fetch(0, entry(0));
+      int next_block = entry(1);
       for (int j = 0; j < it.tiles; ++j, ++jg) {
         const int st = jg & 1;
-        uint4 k0[CH], v0[CH];
-        uint2 p0[CH];
+        uint4 k0[N], v0[N];
+        uint2 p0[N];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
+        for (int i = 0; i < N; ++i) {
           k0[i] = kr[i];
           v0[i] = vr[i];
           p0[i] = pr[i];
@@ -528,13 +567,16 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
             v0[i] = make_uint4(0, 0, 0, 0);
           }
         }
-        if (j + 1 < it.tiles) fetch(j + 1);
+        if (j + 1 < it.tiles) {
+          fetch(j + 1, next_block);
+          next_block = entry(j + 2);
+        }
         // K's power of two: the warp's 32 rows' largest into [2^13, 2^14). V in fp16 if its rows
         // allow it.
         float top = 0.f;
         bool v16 = true;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
+        for (int i = 0; i < N; ++i) {
           const float2 kp = unpack2(p0[i].x), vp = unpack2(p0[i].y);
           const float kb = fmaf(15.f, fabsf(kp.x), fabsf(kp.y));
           if (kb < INFINITY) top = fmaxf(top, kb);  // (not NaN)
@@ -572,7 +614,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
           break;
         }
 #pragma unroll
-        for (int i = 0; i < CH; ++i) write16(sK + st * C::TILE, k0[i], p0[i].x, up, row0 + i * PER);
+        for (int i = 0; i < N; ++i) write16(sK + st * C::TILE, k0[i], p0[i].x, up, row0 + i * PER);
         fence_proxy_async_smem();
         arrive(&k_full[st]);
         if (!wait(&v_empty[st], (jg >> 1) ^ 1)) {
@@ -581,10 +623,10 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
         }
         if (v16) {
 #pragma unroll
-          for (int i = 0; i < CH; ++i) write16(sV + st * C::TILE, v0[i], p0[i].y, 1.f, row0 + i * PER);
+          for (int i = 0; i < N; ++i) write16(sV + st * C::TILE, v0[i], p0[i].y, 1.f, row0 + i * PER);
         } else {
 #pragma unroll 1
-          for (int i = 0; i < CH; ++i) {
+          for (int i = 0; i < N; ++i) {
             const uint32_t sz = p0[i].y, s2 = __byte_perm(sz, sz, 0x1010), z2 = __byte_perm(sz, sz, 0x3232);
             write(sV + st * C::TILE, v0[i], row0 + i * PER, [&](uint32_t x) { return p4_values_bf16(x, s2, z2); });
           }

@@ -571,3 +571,27 @@ def test_prefill_flags_and_capture(kx):
     out.zero_()
     graph.replay()
     assert torch.equal(out, want) and err.item() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_maximum_that_jumps(kx, d):
+    """Scores that rise by 2^8, 2^15 and far beyond within a tile and from tile to tile."""
+    n, m = 400, 130
+    table, blocks = paged(1, [n], 256)
+    gen = torch.Generator().manual_seed(d)
+    rows = torch.randn(n, 1, d, generator=gen) * 0.3
+    rows[:, 0, 0] = torch.arange(n) % 97 * 0.07  # within a tile
+    for key, size in ((40, 30.0), (70, 55.0), (129, 80.0), (300, 140.0), (301, 90.0)):
+        rows[key, 0, 0] = size
+    cache = kx.kv4_cache(blocks, 256, 1, d)
+    slots = (table[0].long()[torch.arange(n) // 256] * 256 + torch.arange(n).cuda() % 256).int()
+    value = torch.randn(n, 1, d, generator=gen).bfloat16().cuda()
+    kx.store_kvcache4(rows.bfloat16().cuda(), value, *cache, slots)
+    q = torch.randn(m, 2, d, generator=gen) * 0.2
+    q[:, 0, 0], q[:, 1, 0] = 1.0, -1.0
+    q = q.bfloat16().cuda()
+    out = torch.empty_like(q)
+    kx.paged_prefill4(q, *cache, starts([m]), starts([n]), table, max_seqlen_q=m, max_seqlen_k=n, scale=0.6, out=out)
+    want, tol = plain_attention(q, cache, table[0], n, 0.6, prefill=True)
+    check_close(out, want, tol, "jumps")

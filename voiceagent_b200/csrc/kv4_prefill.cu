@@ -47,7 +47,7 @@ struct Prefill4Args {
   int64_t bt_stride;
   int bt_width, batch, total_q, group, bs_shift;
   float scale_log2;  // >= 0: the sign is in `flip`
-  uint32_t flip;     // sign bits to exchange in q
+  uint32_t flip;     // sign bit to exchange in q
   __nv_bfloat16 *out;
   int64_t out_row, out_head;
   int32_t *error_flag;
@@ -69,22 +69,28 @@ struct Item4 {
 };
 
 // Walks this CTA's items (item = row tile * KV heads + head, row tiles numbered sequence by
-// sequence). Every warp walks alone and sees the same items.
+// sequence). The list begins with what takes longest -- sequences by falling length, their last
+// rows first -- and is dealt back and forth, c, 2 G - 1 - c, 2 G + c, ... to CTA c of G: with 496
+// items of 2 to 64 tiles the fullest CTA has 148 tiles, 172 when dealt in order, 135 on average.
+// Every warp walks alone and sees the same items.
+constexpr int kP4Sorted = 256;  // sequences up to which they are sorted
 struct Walk4 {
   // query tokens of a sequence, held to the rows that q has
   static __device__ __forceinline__ int q_len_of(const Prefill4Args &a, int b) {
     return max(0, min(a.cu_q[b + 1], a.total_q) - max(0, a.cu_q[b]));
   }
-  int i, scan, carry;  // next item; the sequences before `scan` hold `carry` row tiles
+  int i, scan, carry;      // turn of the CTA; the sequences before `scan` hold `carry` row tiles
+  const uint16_t *order;   // sequences by falling length, or null
   __device__ __forceinline__ bool next(const Prefill4Args &a, Item4 &it) {
     const int lane = threadIdx.x & 31, heads = a.c.num_kv_heads;
     while (true) {
-      const int t = i / heads;
-      it.h = i - t * heads;
-      i += gridDim.x;
+      const int item = i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const int t = item / heads;
+      it.h = item - t * heads;
+      ++i;
       while (true) {
         if (scan >= a.batch) return false;
-        const int bb = scan + lane;
+        const int bb = scan + lane < a.batch ? order ? order[scan + lane] : scan + lane : a.batch;
         const int n = bb < a.batch ? (q_len_of(a, bb) * a.group + kP4Rows - 1) / kP4Rows : 0;
         int incl = n;
 #pragma unroll
@@ -95,8 +101,9 @@ struct Walk4 {
         const unsigned here = __ballot_sync(0xffffffffu, t < carry + incl);
         if (here) {
           const int src = __ffs(here) - 1;
-          it.b = scan + src;
-          it.row0 = (t - carry - __shfl_sync(0xffffffffu, incl - n, src)) * kP4Rows;
+          it.b = __shfl_sync(0xffffffffu, bb, src);
+          // the sequence's row tiles from the last to the first
+          it.row0 = (carry + __shfl_sync(0xffffffffu, incl, src) - 1 - t) * kP4Rows;
           break;
         }
         carry += __shfl_sync(0xffffffffu, incl, 31);
@@ -169,6 +176,8 @@ __device__ __forceinline__ void p4_fewer_registers() {
 constexpr int kP4RegSoftmax = 144, kP4RegConvert = 128, kP4RegMma = 96;
 static_assert(256 * kP4RegSoftmax + 128 * kP4RegConvert + 128 * kP4RegMma <= 512 * 128,
               "more registers than the block was launched with: the wait for them would not end");
+static_assert(kP4RegSoftmax >= 128 && kP4RegConvert <= 128 && kP4RegMma <= 128,
+              "a thread's share can only be raised by the first, and lowered by the others");
 
 // Two neighbouring numbers at a time: s * f + b, and sums.
 __device__ __forceinline__ float2 p4_fma2(float2 s, float2 f, float2 b) {
@@ -247,6 +256,8 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   uint64_t *o_full = bars + 14;       // [2] the item's last P V done
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
   __shared__ int abort_flag;
+  __shared__ int lens[kP4Sorted];
+  __shared__ uint16_t order[kP4Sorted];
   // Per K/V tile (global count, modulo 4) and 32 tokens of it: what undoes K's power of two,
   // negative where V and P are bf16. Four tiles deep: a tile's entry is written anew only after
   // the V tile three before has been waited for, so after both softmaxes of the tile itself.
@@ -277,8 +288,18 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // S0 | S1 | O0 | O1, 128 columns each
   pdl_wait();
+  if (a.batch <= kP4Sorted) {
+    for (int b = tid; b < a.batch; b += kP4Threads) lens[b] = a.cu_k[b + 1] - a.cu_k[b];
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += kP4Threads) {
+      int rank = 0;
+      for (int o = 0; o < a.batch; ++o) rank += lens[o] > lens[b] || (lens[o] == lens[b] && o < b);
+      order[rank] = static_cast<uint16_t>(b);
+    }
+    __syncthreads();
+  }
 
-  Walk4 walk{static_cast<int>(blockIdx.x), 0, 0};
+  Walk4 walk{0, 0, 0, a.batch <= kP4Sorted ? order : nullptr};
   Item4 it;
   // Waits as a whole warp: every lane of a role sees the same outcome.
   auto wait = [&](uint64_t *bar, uint32_t phase) {
@@ -295,39 +316,40 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
     const int w = warp >> 2, r = tid & 127;
     const uint32_t s_base = tmem + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t o_base = tmem + 256 + w * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // This thread's row of q into the tile, dims in the order of the codes' pairs, times the power
-    // of two that brings its largest into [2^13, 2^14); gives the factor of the row's scores.
+    // The warp's 32 rows of q into the tile, D / 8 lanes a row, dims in the order of the codes'
+    // pairs, times the power of two that brings a row's largest into [2^13, 2^14); gives the
+    // factor of the scores of this thread's row.
     auto load_q = [&](const Item4 &t) -> float {
-      const int row = w * 128 + r;
-      const bool in = row < t.rows;
-      const int tok = in ? (t.row0 + row) / a.group : 0, head = in ? (t.row0 + row) - tok * a.group : 0;
-      const __nv_bfloat16 *src = a.q + (t.q0 + tok) * a.q_row + (static_cast<int64_t>(t.h) * a.group + head) * a.q_head;
-      uint8_t *dst = sQ + w * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
-      float top = 0.f;
+      constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row, rows at a time
+      const int j = lane % LPR;
+      float mine = 0.f;
 #pragma unroll 4
-      for (int j = 0; j < D / 8; ++j) {
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const int rt = (warp & 3) * 32 + i * RPI + lane / LPR, row = w * 128 + rt;
         uint4 u = make_uint4(0, 0, 0, 0);
-        if (in) u = *reinterpret_cast<const uint4 *>(src + j * 8);
-        float f[8];
+        if (row < t.rows) {
+          const int tok = (t.row0 + row) / a.group, head = (t.row0 + row) - tok * a.group;
+          u = *reinterpret_cast<const uint4 *>(a.q + (t.q0 + tok) * a.q_row +
+                                               (static_cast<int64_t>(t.h) * a.group + head) * a.q_head + j * 8);
+        }
+        float f[8], top = 0.f;
         unpack8(u, f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
-      }
-      const int ex = min(100, max(-114, 13 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
-      const float up = __int_as_float(((ex + 127) << 23) | a.flip);
-#pragma unroll 4
-      for (int j = 0; j < D / 8; ++j) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (in) u = *reinterpret_cast<const uint4 *>(src + j * 8);
-        float f[8];
-        unpack8(u, f);
-        *reinterpret_cast<uint4 *>(dst + (j >> 3) * C::BLOCK + (((j & 7) ^ (r & 7)) << 4)) =
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = min(100, max(-114, 13 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
+        const float up = __int_as_float(static_cast<uint32_t>(ex + 127) << 23 | a.flip);
+        *reinterpret_cast<uint4 *>(sQ + w * C::TILE + (j >> 3) * C::BLOCK + (rt >> 3) * 1024 + (rt & 7) * 128 +
+                                   (((j & 7) ^ (rt & 7)) << 4)) =
             make_uint4(p4_f16x2(f[0] * up, f[4] * up), p4_f16x2(f[1] * up, f[5] * up),
                        p4_f16x2(f[2] * up, f[6] * up), p4_f16x2(f[3] * up, f[7] * up));
+        const float down = __shfl_sync(0xffffffffu, __int_as_float((127 - ex) << 23), (lane % RPI) * LPR);
+        if (lane / RPI == i) mine = down;
       }
       fence_proxy_async_smem();
       arrive(&q_full[w]);
-      return a.scale_log2 * __int_as_float((127 - ex) << 23);
+      return a.scale_log2 * mine;
     };
     uint32_t ps = 0, po = 0;  // phases of this row tile's scores and outputs
     uint32_t jg = 0;          // K/V tiles of the items so far
@@ -778,7 +800,7 @@ extern "C" int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64
   const int bs = cache->block_size;
   a.bs_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
   a.scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
-  a.flip = scale < 0 ? 0x80008000u : 0u;
+  a.flip = scale < 0 ? 0x80000000u : 0u;
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.out_row = out_row_stride;
   a.out_head = out_head_stride;

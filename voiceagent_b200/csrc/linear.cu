@@ -34,9 +34,10 @@
 //        per-head RMSNorm, the rotation (partner dims in lane ^ 16) and the paged-cache
 //        store of K and V happen on the reduced tile, with the rounding of the unfused
 //        kernels (bf16 projection, bf16 after the norm, after the weight, after RoPE).
-//      - low-rank adapter epilogue: a column's row belongs to one request, whose adapter's
-//        up-projection of lora_down's t (lora.cu) is added to the reduced sums in fp32, before
-//        their one rounding; the split columns spread the adapters' rows over the CTAs.
+//      - low-rank adapter epilogue: a batch column is a request, whose adapter's up-projection of
+//        lora_down's t (lora.cu) is worked out by four more warps while the weights stream, and
+//        added to the reduced sums in fp32 before their one rounding; the K split, which deals
+//        the columns to the CTAs of a cluster, spreads the adapters' rows over the GPU too.
 //    A decode layer is then qkv (norm + rope + store) -> attention -> o_proj (+residual)
 //    -> gate_up (norm, SiLU*mul) -> down (+residual): five launches instead of eight.
 //
@@ -391,26 +392,94 @@ __device__ __forceinline__ void qk_rope_store4(const LinearFuse &f, const Linear
                              lane * 4) = packed;
 }
 
-// Four neighbouring outputs of row c: += t[c] . B_ad[n .. n + 3] (B's rows are contiguous).
-__device__ __forceinline__ void lora_up4(float (&y)[4], const LinearFuse &f, int c, int ad, int n) {
-  const float *t = f.lora_t + static_cast<int64_t>(c) * f.rank;
-  const __nv_bfloat16 *b = f.lora_b + (static_cast<int64_t>(ad) * f.lora_n + n) * f.rank;
-#pragma unroll 2
-  for (int r = 0; r < f.rank; r += 8) {
-    const float4 t0 = *reinterpret_cast<const float4 *>(t + r);
-    const float4 t1 = *reinterpret_cast<const float4 *>(t + r + 4);
+// The low-rank adapters' part of this CTA's `cols` batch columns and 128 output rows, [col][row],
+// by four warps of 32 rows each while the others stream the weights: t B_a^T by mma m16n8k16 with
+// B's rows as its rows (a lane's 8 consecutive ranks are its operands of two k-steps) and up to 8
+// columns of one adapter as its columns, so that requests sharing an adapter read it once. t, held
+// in 32 bits, goes in as the sum of two bf16 numbers. Columns without an adapter become zero.
+__device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void lora_columns(float *out, const LinearFuse &f, int m, int c0, int cols, int n0) {
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int row0 = warp * 32;
+  for (int base = 0; base < cols; base += 32) {
+    const int c = c0 + base + lane;
+    int mine = base + lane < cols && c < m ? f.row_adapter[c] : -1;
+    if (mine >= f.num_adapters) mine = -1;  // (flagged by lora_down)
+    for (unsigned none = __ballot_sync(0xffffffffu, mine < 0 && base + lane < cols); none; none &= none - 1)
+      out[(base + __ffs(none) - 1) * kLnRows + row0 + lane] = 0.f;
+    for (unsigned left = __ballot_sync(0xffffffffu, mine >= 0); left;) {
+      const int ad = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
+      unsigned group = __ballot_sync(0xffffffffu, mine == ad) & left;
+      int col = -1, c_even = -1, c_odd = -1;  // the group's column g, and 2q and 2q + 1
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float v[8];
-      unpack8(*reinterpret_cast<const uint4 *>(b + e * f.rank + r), v);
-      y[e] = fmaf(t0.x, v[0], fmaf(t0.y, v[1], fmaf(t0.z, v[2], fmaf(t0.w, v[3], y[e]))));
-      y[e] = fmaf(t1.x, v[4], fmaf(t1.y, v[5], fmaf(t1.z, v[6], fmaf(t1.w, v[7], y[e]))));
+      for (int i = 0; i < 8; ++i) {
+        const int b = __ffs(group) - 1;
+        if (b < 0) break;
+        if (i == g) col = base + b;
+        if (i == 2 * q) c_even = base + b;
+        if (i == 2 * q + 1) c_odd = base + b;
+        group &= group - 1;
+        left &= ~(1u << b);
+      }
+      float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      const __nv_bfloat16 *bp = f.lora_b + (static_cast<int64_t>(ad) * f.lora_n + n0 + row0 + g) * f.rank + q * 8;
+      const float *tp = f.lora_t + static_cast<int64_t>(c0 + max(col, 0)) * f.rank + q * 8;
+#pragma unroll 2
+      for (int r = 0; r < f.rank; r += 32) {
+        const bool in = r + q * 8 < f.rank;
+        uint4 bv[4] = {};
+        float4 t0 = make_float4(0.f, 0.f, 0.f, 0.f), t1 = t0;
+        if (in) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bv[i] = *reinterpret_cast<const uint4 *>(bp + static_cast<int64_t>(8 * i) * f.rank + r);
+          if (col >= 0) {
+            t0 = *reinterpret_cast<const float4 *>(tp + r);
+            t1 = *reinterpret_cast<const float4 *>(tp + r + 4);
+          }
+        }
+        const uint32_t hi[4] = {pack2(t0.x, t0.y), pack2(t0.z, t0.w), pack2(t1.x, t1.y), pack2(t1.z, t1.w)};
+        const float2 h0 = unpack2(hi[0]), h1 = unpack2(hi[1]), h2 = unpack2(hi[2]), h3 = unpack2(hi[3]);
+        const uint32_t lo[4] = {pack2(t0.x - h0.x, t0.y - h0.y), pack2(t0.z - h1.x, t0.w - h1.y),
+                                pack2(t1.x - h2.x, t1.y - h2.y), pack2(t1.z - h3.x, t1.w - h3.y)};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // rows row0 + 16 i + g and + 8
+          const uint4 &u = bv[2 * i], &v = bv[2 * i + 1];
+          lora_mma(acc[i], u.x, v.x, u.y, v.y, hi[0], hi[1]);
+          lora_mma(acc[i], u.z, v.z, u.w, v.w, hi[2], hi[3]);
+          lora_mma(acc[i], u.x, v.x, u.y, v.y, lo[0], lo[1]);
+          lora_mma(acc[i], u.z, v.z, u.w, v.w, lo[2], lo[3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float *o = out + row0 + 16 * i + g;
+        if (c_even >= 0) {
+          o[c_even * kLnRows] = acc[i][0];
+          o[c_even * kLnRows + 8] = acc[i][2];
+        }
+        if (c_odd >= 0) {
+          o[c_odd * kLnRows] = acc[i][1];
+          o[c_odd * kLnRows + 8] = acc[i][3];
+        }
+      }
     }
   }
 }
 
+// The adapters take four warps more.
+template <int EPI>
+constexpr int ln_threads() { return EPI == kEpiLora ? 2 * kLnThreads : kLnThreads; }
+
 template <int MP, bool NORM_IN, int EPI>
-__global__ void __launch_bounds__(kLnThreads)
+__global__ void __launch_bounds__(ln_threads<EPI>())
     linear_small_kernel(const __grid_constant__ CUtensorMap tm_w,
                         const __grid_constant__ CUtensorMap tm_x, const LinearArgs a,
                         const __grid_constant__ LinearFuse f) {
@@ -540,6 +609,11 @@ __global__ void __launch_bounds__(kLnThreads)
   }
 
   // Every thread: its TMEM lane = weight row (w*32 + lane) of the tile -> partial[.][row].
+  float *lora_part = reinterpret_cast<float *>(tmem_slot + 4);  // [cols][128], of kEpiLora only
+  if (EPI == kEpiLora && warp >= 4) {
+    pdl_wait();  // t and the rows' adapters come from earlier kernels
+    lora_columns(lora_part, f, a.m, kz * cols, cols, tile * kLnRows);
+  }
   __syncwarp();  // the producer / MMA lanes rejoin their warps (tcgen05.ld is warp-aligned)
   // While the MMAs run: the epilogue operands of this warp's first rows (inputs written by
   // earlier kernels; the wait returns at once, x or h was already waited for).
@@ -562,7 +636,7 @@ __global__ void __launch_bounds__(kLnThreads)
   const bool have = __all_sync(0xffffffffu, mbar_wait(done, 0, a.error_flag, &abort_flag));
   const uint32_t red_base = smem_addr(red), bar_base = smem_addr(recv_bar);
   float *colmaj = reinterpret_cast<float *>(stages);  // [MP][128]
-  {
+  if (EPI != kEpiLora || warp < 4) {
     tc_fence_after();
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
 #pragma unroll
@@ -583,6 +657,7 @@ __global__ void __launch_bounds__(kLnThreads)
   if (ks > 1) cluster_wait();  // every peer's receive barrier is initialised
 #pragma unroll
   for (int i = 0; i < MP * (kLnRows / 4) / kLnThreads; ++i) {
+    if (EPI == kEpiLora && warp >= 4) break;
     const int id = i * kLnThreads + tid;  // (column, 4-row group): warps write 512 B runs
     const int col = id / (kLnRows / 4), q = id % (kLnRows / 4);
     const int r = col >> cols_log2, cl = col & (cols - 1);  // cols: a power of two
@@ -601,7 +676,7 @@ __global__ void __launch_bounds__(kLnThreads)
 
   pdl_wait();  // (returns at once: the producer's wait has passed) orders the writes below
   // Warp w takes local columns w, w + 4, ...; each lane 4 consecutive tile rows.
-  for (int cl = warp, i = 0; cl < cols; cl += 4, ++i) {
+  for (int cl = warp, i = 0; cl < cols && (EPI != kEpiLora || warp < 4); cl += 4, ++i) {
     const int c = kz * cols + cl;
     if (c >= a.m) break;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);  // sources in rank order
@@ -655,11 +730,9 @@ __global__ void __launch_bounds__(kLnThreads)
       else epi_fetch<EPI>(cur, f, a, c, tile, lane);
       qk_rope_store4(f, a, c, tile, lane, v4, cur, qk_nw);
     } else if (EPI == kEpiLora) {
-      float y[4] = {acc.x, acc.y, acc.z, acc.w};
-      const int ad = f.row_adapter[c];
-      if (ad >= 0 && ad < f.num_adapters) lora_up4(y, f, c, ad, tile * kLnRows + lane * 4);
+      const float4 l = *reinterpret_cast<const float4 *>(&lora_part[cl * kLnRows + lane * 4]);
       __nv_bfloat16 *dst = a.y + c * a.y_stride + tile * kLnRows + lane * 4;
-      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc.x + l.x, acc.y + l.y), pack2(acc.z + l.z, acc.w + l.w));
     } else {
       __nv_bfloat16 *dst = a.y + c * a.y_stride + tile * kLnRows + lane * 4;
       *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc.x, acc.y), pack2(acc.z, acc.w));
@@ -950,10 +1023,12 @@ int launch_linear(const void *x, int64_t x_stride, int m, int k, const void *w, 
                   cudaStream_t stream) {
   using C = Ln<MP, NORM_IN>;
   auto kfn = linear_small_kernel<MP, NORM_IN, EPI>;
+  // (the adapters' part: [columns of a CTA][128] fp32)
+  constexpr size_t extra = EPI == kEpiLora ? MP * kLnRows * 4 : 0;
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(C::SMEM));
+                                         static_cast<int>(C::SMEM + extra + 16));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kfn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) {
       set_error("linear_small: kernel configuration failed: %s", cudaGetErrorString(e));
@@ -980,8 +1055,8 @@ int launch_linear(const void *x, int64_t x_stride, int m, int k, const void *w, 
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kLnThreads, 1, 1);
-  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.blockDim = dim3(ln_threads<EPI>(), 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM + extra;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -1010,7 +1085,9 @@ int launch_linear(const void *x, int64_t x_stride, int m, int k, const void *w, 
   a.steps = k / kLnBK / a.k_split;
   cfg.gridDim = dim3(tiles * a.k_split, 1, 1);
   attr[0].val.clusterDim.x = a.k_split;
-  if (pdl_enabled()) {
+  if (EPI == kEpiLora) cfg.dynamicSmemBytes = C::SMEM + extra / a.k_split + 16;
+  // The adapters' product always follows lora_down, whose time its weight loads hide.
+  if (EPI == kEpiLora || pdl_enabled()) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;

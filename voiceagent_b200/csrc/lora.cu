@@ -38,15 +38,27 @@ __global__ void __launch_bounds__(128) lora_down_kernel(
   const __nv_bfloat16 *xr = x + row * x_stride;
   const __nv_bfloat16 *ar = a + (static_cast<int64_t>(ad) * rank + r0) * k;
   float acc[kLdRanks] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = lane * 8; i < k; i += 256) {
-    float xv[8], av[8];
-    unpack8(*reinterpret_cast<const uint4 *>(xr + i), xv);
+  constexpr int AHEAD = 4;  // blocks of 256 k on their way at a time
+  for (int i0 = lane * 8; i0 < k; i0 += AHEAD * 256) {
+    uint4 xu[AHEAD], au[AHEAD][kLdRanks];
 #pragma unroll
-    for (int r = 0; r < kLdRanks; ++r) {
-      unpack8(*reinterpret_cast<const uint4 *>(ar + static_cast<int64_t>(r) * k + i), av);
+    for (int s = 0; s < AHEAD; ++s) {  // (past the end of K: the last 8 again, not used)
+      const int i = min(i0 + s * 256, k - 8);
+      xu[s] = *reinterpret_cast<const uint4 *>(xr + i);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[r] = fmaf(xv[e], av[e], acc[r]);
+      for (int r = 0; r < kLdRanks; ++r) au[s][r] = *reinterpret_cast<const uint4 *>(ar + static_cast<int64_t>(r) * k + i);
+    }
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      if (i0 + s * 256 >= k) break;
+      float xv[8], av[8];
+      unpack8(xu[s], xv);
+#pragma unroll
+      for (int r = 0; r < kLdRanks; ++r) {
+        unpack8(au[s][r], av);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[r] = fmaf(xv[e], av[e], acc[r]);
+      }
     }
   }
 #pragma unroll
@@ -124,8 +136,8 @@ __device__ __forceinline__ void lora_plan(const LoraDownArgs &p, int tile) {
 template <int NT>
 __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs p) {
   __shared__ float part[2][kLtRows][8 * NT + 1];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // after the wait: the product reads x before its own
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int tiles = (p.rows + kLtRows - 1) / kLtRows;
   if (static_cast<int>(blockIdx.x) >= tiles) {
@@ -149,25 +161,29 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-#pragma unroll 2
-      for (int k0 = warp * 32; k0 < p.k; k0 += 128) {
-        const int kk = k0 + q * 8;
+      // Rows of other adapters, past the last row and past the rank are read as well, from valid
+      // places, and their sums are not kept: loads without conditions, so that four blocks of k are
+      // in flight. Only the end of K is masked.
+      const __nv_bfloat16 *xp[2][2], *ap[NT];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+          xp[m][hh] = p.x + min(row0 + m * 16 + hh * 8 + g, static_cast<int64_t>(p.rows) - 1) * p.x_stride + q * 8;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        ap[j] = am + static_cast<int64_t>(min(r0 + j * 8 + g, p.rank - 1)) * p.k + q * 8;
+      auto block = [&](int k0, bool whole) {
         uint4 xv[2][2], av[NT];
+        const bool in = whole || k0 + q * 8 < p.k;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const int r = m * 16 + hh * 8 + g;
-            xv[m][hh] = make_uint4(0, 0, 0, 0);
-            if (kk < p.k && (rows >> r & 1))
-              xv[m][hh] = *reinterpret_cast<const uint4 *>(p.x + (row0 + r) * p.x_stride + kk);
-          }
+          for (int hh = 0; hh < 2; ++hh)
+            xv[m][hh] = in ? *reinterpret_cast<const uint4 *>(xp[m][hh] + k0) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          av[j] = make_uint4(0, 0, 0, 0);
-          if (kk < p.k && r0 + j * 8 + g < p.rank)
-            av[j] = *reinterpret_cast<const uint4 *>(am + static_cast<int64_t>(r0 + j * 8 + g) * p.k + kk);
-        }
+        for (int j = 0; j < NT; ++j)
+          av[j] = in ? *reinterpret_cast<const uint4 *>(ap[j] + k0) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -175,7 +191,12 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
             mma_bf16_16816(acc[m][j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av[j].x, av[j].y);
             mma_bf16_16816(acc[m][j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av[j].z, av[j].w);
           }
-      }
+      };
+      const int whole = p.k / 32 * 32;
+      int k0 = warp * 32;
+#pragma unroll NT == 4 ? 4 : 2
+      for (; k0 < whole; k0 += 128) block(k0, true);
+      if (k0 < p.k) block(k0, false);
       // warps 0 and 1 lay their sums down, 2 and 3 add theirs
 #pragma unroll
       for (int turn = 0; turn < 2; ++turn) {
@@ -349,7 +370,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
   lg_cluster_sync();  // both CTAs' barriers are initialised
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
 
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tiles = a.tiles_m * a.tiles_n;
@@ -360,6 +380,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
 
   if (warp == 8) {
     // ---------------------------------------------------------------------- loads
+    // x and W do not wait for lora_down_rows: it lets this launch begin once it has itself waited
+    // for x. The plan and t do, here and below.
     if (lane == 0) {
       uint32_t it = 0, lt = 0;
       bool ok = true;
@@ -374,6 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
           lg_load_2d(ring + st * kLgStage, &tm_x, s * kLgBK, m0, bar);
           lg_load_2d(ring + st * kLgStage + kLgHalf, &tm_w, s * kLgBK, n0, bar);
         }
+        pdl_wait();
         const int steps = lora_steps(t);
         for (int s = 0; s < steps && ok; ++s, ++lt) {
           ok = lg_wait(l_empty, (lt & 1) ^ 1, a.error_flag, &abort_flag);
@@ -409,6 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
                    (s > 0 || kk > 0) ? 1u : 0u);
           lg_commit(&empty[st]);
         }
+        pdl_wait();
         const int steps = ok ? lora_steps(t) : 0;
         for (int s = 0; s < steps; ++s, ++lt) {
           ok = lg_wait(l_full, lt & 1, a.error_flag, &abort_flag);
@@ -426,6 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
   } else if (warp >= 4) {
     // ------------------------------------------------------- t rows of the adapters
     const int r = tid - 128;  // row of this CTA's half
+    pdl_wait();
     uint8_t *dst = lora + (r >> 3) * 1024 + (r & 7) * 128;
     uint32_t lt = 0;
     bool ok = true;
@@ -455,6 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------- epilogue
+    pdl_wait();  // y is written after whatever ran before
     int j = 0;
     for (int t = pair; t < tiles; t += pairs, ++j) {
       const int acc = j & 1;
@@ -610,8 +636,17 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
   auto kfn = rank <= 32 ? lora_down_rows_kernel<4> : lora_down_rows_kernel<8>;
   B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(down + g.tiles_m), dim3(128), 0, st, true, 1, p), "lora_rows (down)");
   const int pairs = std::min(g.tiles_m * g.tiles_n, num_sms() / 2);
-  B200_LAUNCH_CHECK_ERR(launch_kernel(lora_gemm_kernel, dim3(2 * pairs), dim3(kLgThreads), kLgSmem, st, true, 1, tx,
-                                      tw, tb, g),
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(kLgThreads);
+  cfg.dynamicSmemBytes = kLgSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  B200_LAUNCH_CHECK_ERR(cudaLaunchKernelEx(&cfg, lora_gemm_kernel, tx, tw, tb, g),
                         "lora_rows");
   return B200ASR_OK;
 }

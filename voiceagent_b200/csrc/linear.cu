@@ -35,7 +35,7 @@
 //        store of K and V happen on the reduced tile, with the rounding of the unfused
 //        kernels (bf16 projection, bf16 after the norm, after the weight, after RoPE).
 //      - low-rank adapter epilogue: a batch column is a request, whose adapter's up-projection of
-//        lora_down's t (lora.cu) is worked out by four more warps while the weights stream, and
+//        lora_down's t (lora.cu) is worked out by eight more warps while the weights stream, and
 //        added to the reduced sums in fp32 before their one rounding; the K split, which deals
 //        the columns to the CTAs of a cluster, spreads the adapters' rows over the GPU too.
 //    A decode layer is then qkv (norm + rope + store) -> attention -> o_proj (+residual)
@@ -393,7 +393,7 @@ __device__ __forceinline__ void qk_rope_store4(const LinearFuse &f, const Linear
 }
 
 // The low-rank adapters' part of this CTA's `cols` batch columns and 128 output rows, [col][row],
-// by four warps of 32 rows each while the others stream the weights: t B_a^T by mma m16n8k16 with
+// by warps of their own, 32 rows each, while the others stream the weights: t B_a^T by mma m16n8k16 with
 // B's rows as its rows (a lane's 8 consecutive ranks are its operands of two k-steps) and up to 8
 // columns of one adapter as its columns, so that requests sharing an adapter read it once. t, held
 // in 32 bits, goes in as the sum of two bf16 numbers. Columns without an adapter become zero.
@@ -406,77 +406,128 @@ __device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+constexpr int kLoraWarps = 8;  // 4 x 32 rows, every second group of columns each
+
+// One adapter's columns (up to 8), and 64 of its ranks.
+struct LoraStep {
+  int adapter, r;          // adapter < 0: none left
+  int col, even, odd;      // the group's column g, and 2q and 2q + 1 (-1: none)
+};
+
 __device__ __forceinline__ void lora_columns(float *out, const LinearFuse &f, int m, int c0, int cols, int n0) {
-  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int row0 = warp * 32;
+  const int warp = ((threadIdx.x >> 5) - 4) & (kLoraWarps - 1), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int row0 = (warp & 3) * 32;
   for (int base = 0; base < cols; base += 32) {
     const int c = c0 + base + lane;
     int mine = base + lane < cols && c < m ? f.row_adapter[c] : -1;
     if (mine >= f.num_adapters) mine = -1;  // (flagged by lora_down)
-    for (unsigned none = __ballot_sync(0xffffffffu, mine < 0 && base + lane < cols); none; none &= none - 1)
-      out[(base + __ffs(none) - 1) * kLnRows + row0 + lane] = 0.f;
-    for (unsigned left = __ballot_sync(0xffffffffu, mine >= 0); left;) {
-      const int ad = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
-      unsigned group = __ballot_sync(0xffffffffu, mine == ad) & left;
-      int col = -1, c_even = -1, c_odd = -1;  // the group's column g, and 2q and 2q + 1
+    if (warp < 4)
+      for (unsigned none = __ballot_sync(0xffffffffu, mine < 0 && base + lane < cols); none; none &= none - 1)
+        out[(base + __ffs(none) - 1) * kLnRows + row0 + lane] = 0.f;
+    unsigned left = __ballot_sync(0xffffffffu, mine >= 0);
+    int turn = warp >> 2;  // groups to leave to the other warps first
+    auto next_group = [&](LoraStep &s) {
+      s.adapter = -1;
+      while (left) {
+        const int ad = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
+        unsigned group = __ballot_sync(0xffffffffu, mine == ad) & left;
+        s.col = s.even = s.odd = -1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int b = __ffs(group) - 1;
-        if (b < 0) break;
-        if (i == g) col = base + b;
-        if (i == 2 * q) c_even = base + b;
-        if (i == 2 * q + 1) c_odd = base + b;
-        group &= group - 1;
-        left &= ~(1u << b);
-      }
-      float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      const __nv_bfloat16 *bp = f.lora_b + (static_cast<int64_t>(ad) * f.lora_n + n0 + row0 + g) * f.rank + q * 8;
-      const float *tp = f.lora_t + static_cast<int64_t>(c0 + max(col, 0)) * f.rank + q * 8;
-#pragma unroll 2
-      for (int r = 0; r < f.rank; r += 32) {
-        const bool in = r + q * 8 < f.rank;
-        uint4 bv[4] = {};
-        float4 t0 = make_float4(0.f, 0.f, 0.f, 0.f), t1 = t0;
-        if (in) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) bv[i] = *reinterpret_cast<const uint4 *>(bp + static_cast<int64_t>(8 * i) * f.rank + r);
-          if (col >= 0) {
-            t0 = *reinterpret_cast<const float4 *>(tp + r);
-            t1 = *reinterpret_cast<const float4 *>(tp + r + 4);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int b = __ffs(group) - 1;
+          if (b < 0) break;
+          if (i == g) s.col = base + b;
+          if (i == 2 * q) s.even = base + b;
+          if (i == 2 * q + 1) s.odd = base + b;
+          group &= group - 1;
+          left &= ~(1u << b);
         }
+        turn ^= 1;
+        if (turn) {  // mine
+          s.adapter = ad;
+          s.r = 0;
+          return;
+        }
+      }
+    };
+    uint4 bv[2][4];
+    float4 tv[2][2];
+    // B's rows row0 + g + 8 i and the group's t, ranks r + 8 q and up, + 32: no load waits for another
+    auto load = [&](const LoraStep &s) {
+      const __nv_bfloat16 *bp = f.lora_b + (static_cast<int64_t>(s.adapter) * f.lora_n + n0 + row0 + g) * f.rank;
+      const float *tp = f.lora_t + static_cast<int64_t>(c0 + max(s.col, 0)) * f.rank;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = min(s.r + 32 * h + q * 8, f.rank - 8);  // (past the rank: not used)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(bv[h][i].x), "=r"(bv[h][i].y), "=r"(bv[h][i].z), "=r"(bv[h][i].w)
+                       : "l"(bp + static_cast<int64_t>(8 * i) * f.rank + r));
+        tv[h][0] = *reinterpret_cast<const float4 *>(tp + r);
+        tv[h][1] = *reinterpret_cast<const float4 *>(tp + r + 4);
+      }
+    };
+    LoraStep s, n;
+    next_group(s);
+    if (s.adapter >= 0) load(s);
+    float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    while (s.adapter >= 0) {
+      uint4 b[2][4];
+      float4 t[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool in = s.r + 32 * h + q * 8 < f.rank;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[h][i] = in ? bv[h][i] : make_uint4(0, 0, 0, 0);
+        t[h][0] = in && s.col >= 0 ? tv[h][0] : make_float4(0.f, 0.f, 0.f, 0.f);
+        t[h][1] = in && s.col >= 0 ? tv[h][1] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      const bool last = s.r + 64 >= f.rank;
+      n = s;
+      if (last) next_group(n);
+      else n.r += 64;
+      if (n.adapter >= 0) load(n);  // under this step's products
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 t0 = t[h][0], t1 = t[h][1];
         const uint32_t hi[4] = {pack2(t0.x, t0.y), pack2(t0.z, t0.w), pack2(t1.x, t1.y), pack2(t1.z, t1.w)};
         const float2 h0 = unpack2(hi[0]), h1 = unpack2(hi[1]), h2 = unpack2(hi[2]), h3 = unpack2(hi[3]);
         const uint32_t lo[4] = {pack2(t0.x - h0.x, t0.y - h0.y), pack2(t0.z - h1.x, t0.w - h1.y),
                                 pack2(t1.x - h2.x, t1.y - h2.y), pack2(t1.z - h3.x, t1.w - h3.y)};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // rows row0 + 16 i + g and + 8
-          const uint4 &u = bv[2 * i], &v = bv[2 * i + 1];
+          const uint4 &u = b[h][2 * i], &v = b[h][2 * i + 1];
           lora_mma(acc[i], u.x, v.x, u.y, v.y, hi[0], hi[1]);
           lora_mma(acc[i], u.z, v.z, u.w, v.w, hi[2], hi[3]);
           lora_mma(acc[i], u.x, v.x, u.y, v.y, lo[0], lo[1]);
           lora_mma(acc[i], u.z, v.z, u.w, v.w, lo[2], lo[3]);
         }
       }
+      if (last) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float *o = out + row0 + 16 * i + g;
-        if (c_even >= 0) {
-          o[c_even * kLnRows] = acc[i][0];
-          o[c_even * kLnRows + 8] = acc[i][2];
-        }
-        if (c_odd >= 0) {
-          o[c_odd * kLnRows] = acc[i][1];
-          o[c_odd * kLnRows + 8] = acc[i][3];
+        for (int i = 0; i < 2; ++i) {
+          float *o = out + row0 + 16 * i + g;
+          if (s.even >= 0) {
+            o[s.even * kLnRows] = acc[i][0];
+            o[s.even * kLnRows + 8] = acc[i][2];
+          }
+          if (s.odd >= 0) {
+            o[s.odd * kLnRows] = acc[i][1];
+            o[s.odd * kLnRows + 8] = acc[i][3];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
         }
       }
+      s = n;
     }
   }
 }
 
-// The adapters take four warps more.
+// The adapters take more warps.
 template <int EPI>
-constexpr int ln_threads() { return EPI == kEpiLora ? 2 * kLnThreads : kLnThreads; }
+constexpr int ln_threads() { return kLnThreads + (EPI == kEpiLora ? kLoraWarps * 32 : 0); }
 
 template <int MP, bool NORM_IN, int EPI>
 __global__ void __launch_bounds__(ln_threads<EPI>())

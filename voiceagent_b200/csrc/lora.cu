@@ -17,6 +17,13 @@ __device__ __forceinline__ int row_adapter_of(const int32_t *rows, int64_t t, in
   return -1;
 }
 
+// A load that stays where it is written, so that many are in flight before the first is used.
+__device__ __forceinline__ uint4 load_now(const __nv_bfloat16 *p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // ------------------------------------------------------------------ down, few rows
 // One warp per (row, 4 ranks): every lane holds 8 consecutive k of x and of the four rows of A,
 // 16-byte loads all independent of each other. At decode sizes this is latency: enough warps
@@ -44,9 +51,9 @@ __global__ void __launch_bounds__(128) lora_down_kernel(
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) {  // (past the end of K: the last 8 again, not used)
       const int i = min(i0 + s * 256, k - 8);
-      xu[s] = *reinterpret_cast<const uint4 *>(xr + i);
+      xu[s] = load_now(xr + i);
 #pragma unroll
-      for (int r = 0; r < kLdRanks; ++r) au[s][r] = *reinterpret_cast<const uint4 *>(ar + static_cast<int64_t>(r) * k + i);
+      for (int r = 0; r < kLdRanks; ++r) au[s][r] = load_now(ar + static_cast<int64_t>(r) * k + i);
     }
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) {

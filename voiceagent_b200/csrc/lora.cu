@@ -78,17 +78,21 @@ __global__ void __launch_bounds__(128) lora_down_kernel(
 }
 
 // ------------------------------------------------------------------ down, any rows
-// A CTA takes 32 rows; its four warps split K, mma m16n8k16 straight from global memory (a
-// lane's 8 consecutive k are its operands of two k-steps, so x and A are read in 64-byte
-// runs), and their sums are joined in shared memory. The distinct adapters of the 32 rows are
-// taken in turn: a prefill batch's rows follow one another by request, so there are one or
-// two. t is rounded to bf16 once, as activations between projections are: it is the operand
-// of the second product. The last CTAs of the launch list each 256-row tile's distinct
-// adapters for that product.
+// A CTA takes 32 rows of x and streams them once, with the rows of A they need, through a ring of
+// cp.async stages of 64 k (128-byte swizzle, so that ldmatrix meets no bank twice); mma m16n8k16.
+// What the rows need is a list of rank tiles of 8, adapter after adapter: eight of them go through
+// a pass, a warp two, so that a prefill batch's tile, which has one or two adapters, is one pass
+// at ranks up to 32. Two CTAs per SM keep 120 KB on their way. t is rounded to bf16 once, as
+// activations between projections are: it is the operand of the second product. The last CTAs of
+// the launch list each 256-row tile's distinct adapters for that product.
+// (Operands straight from global memory, the warps splitting K: 34 us for 7829 rows of 2048.)
 constexpr int kLtRows = 32;
+constexpr int kLtBK = 64, kLtTiles = 8;  // k of a stage, rank tiles of a pass
+constexpr int kLtStages = 6;
+constexpr int kLtStage = (kLtRows + 8 * kLtTiles) * kLtBK * 2;
 constexpr int kLoraMaxRank = 128;
 constexpr int kLgTile = 256;            // rows and columns of a CTA pair's tile
-constexpr int kLgPlan = 1 + kLgTile;    // plan entry of a row tile: count, adapters ascending
+constexpr int kLgPlan = 1 + kLgTile;    // plan entry of a row tile: count, adapters
 
 struct LoraDownArgs {
   const __nv_bfloat16 *x;
@@ -112,37 +116,47 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t a0,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Distinct adapters of rows [256 tile, +256), ascending (128 threads, two rows each).
-__device__ __forceinline__ void lora_plan(const LoraDownArgs &p, int tile) {
-  __shared__ int ids[kLgTile], first[kLgTile];
-  int count = 0;
-  for (int i = threadIdx.x; i < kLgTile; i += 128) {
-    const int64_t r = static_cast<int64_t>(tile) * kLgTile + i;
-    ids[i] = r < p.rows ? row_adapter_of(p.row_adapter, r, p.num_adapters, nullptr) : -1;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kLgTile; i += 128) {
-    bool is_first = ids[i] >= 0;
-    for (int j = 0; j < i && is_first; ++j) is_first = ids[j] != ids[i];
-    first[i] = is_first;
-  }
-  __syncthreads();
-  int32_t *out = p.plan + static_cast<int64_t>(tile) * kLgPlan;
-  for (int i = threadIdx.x; i < kLgTile; i += 128) {
-    if (!first[i]) continue;
-    int place = 0;
-    for (int j = 0; j < kLgTile; ++j) place += first[j] && ids[j] < ids[i];
-    out[1 + place] = ids[i];
-    ++count;
-  }
-  count = __syncthreads_count(count & 1) + 2 * __syncthreads_count(count >> 1);
-  if (threadIdx.x == 0) out[0] = count;
+__device__ __forceinline__ void lt_copy16(uint32_t dst, const void *src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void lt_ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
-// NT: rank tiles of 8 per pass over x.
-template <int NT>
+// Distinct adapters of rows [256 tile, +256), in the order of their first rows (one warp).
+__device__ __forceinline__ void lora_plan(const LoraDownArgs &p, int tile) {
+  __shared__ int list[kLgTile];
+  if (threadIdx.x >= 32) return;
+  const int lane = threadIdx.x;
+  int mine[kLgTile / 32];
+#pragma unroll
+  for (int i = 0; i < kLgTile / 32; ++i) {
+    const int64_t r = static_cast<int64_t>(tile) * kLgTile + i * 32 + lane;
+    mine[i] = r < p.rows ? row_adapter_of(p.row_adapter, r, p.num_adapters, nullptr) : -1;
+  }
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < kLgTile / 32; ++i) {
+    const unsigned same = __match_any_sync(0xffffffffu, mine[i]);
+    bool is_new = mine[i] >= 0 && __ffs(same) - 1 == lane;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) is_new = is_new && list[j] != mine[i];
+    const unsigned news = __ballot_sync(0xffffffffu, is_new);
+    if (is_new) list[count + __popc(news & ((1u << lane) - 1))] = mine[i];
+    count += __popc(news);
+    __syncwarp();
+  }
+  int32_t *out = p.plan + static_cast<int64_t>(tile) * kLgPlan;
+  for (int j = lane; j < count; j += 32) out[1 + j] = list[j];
+  if (lane == 0) out[0] = count;
+}
+
 __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs p) {
-  __shared__ float part[2][kLtRows][8 * NT + 1];
+  extern __shared__ __align__(1024) uint8_t ring[];
+  __shared__ int list[kLtRows];
   pdl_wait();
   pdl_trigger();  // after the wait: the product reads x before its own
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -151,84 +165,102 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
     lora_plan(p, blockIdx.x - tiles);
     return;
   }
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kLtRows;
+  const int row0 = blockIdx.x * kLtRows;
   const int mine = row0 + lane < p.rows ? row_adapter_of(p.row_adapter, row0 + lane, p.num_adapters,
                                                          warp == 0 ? p.error_flag : nullptr)
                                         : -1;
-  for (unsigned left = __ballot_sync(0xffffffffu, mine >= 0); left;) {
+  int distinct = 0;
+  for (unsigned left = __ballot_sync(0xffffffffu, mine >= 0); left; ++distinct) {
     const int ad = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
-    const unsigned rows = __ballot_sync(0xffffffffu, mine == ad);
-    left &= ~rows;
-    const __nv_bfloat16 *am = p.a + static_cast<int64_t>(ad) * p.rank * p.k;
-    for (int r0 = 0; r0 < p.rank; r0 += 8 * NT) {
-      float acc[2][NT][4];
+    left &= ~__ballot_sync(0xffffffffu, mine == ad);
+    if (tid == 0) list[distinct] = ad;
+  }
+  __syncthreads();
+  const int per = p.rank / 8, all = distinct * per;  // rank tiles of an adapter, and in all
+  const int steps = (p.k + kLtBK - 1) / kLtBK;
+  const uint32_t ring_s = smem_addr(ring);
+  // This thread's pieces of a stage: 16 bytes of 2 rows of x and of 4 rows of A.
+  const int piece = tid & 7, prow = tid >> 3;
+  const __nv_bfloat16 *xp[2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+  for (int i = 0; i < 2; ++i)  // (past the last row: the last one again, not kept)
+    xp[i] = p.x + static_cast<int64_t>(min(row0 + prow + 16 * i, p.rows - 1)) * p.x_stride + piece * 8;
+  for (int first = 0; first < all; first += kLtTiles) {
+    const int used = min(kLtTiles, all - first);
+    const __nv_bfloat16 *ap[4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+    for (int i = 0; i < 4; ++i) {  // (past the last tile: the last one again, not kept)
+      const int r = prow + 16 * i, tile = min(first + (r >> 3), all - 1), at = tile / per;
+      ap[i] = p.a + (static_cast<int64_t>(list[at]) * p.rank + (tile - at * per) * 8 + (r & 7)) * p.k + piece * 8;
+    }
+    auto issue = [&](int s) {
+      if (s < steps) {
+        const uint32_t st = ring_s + s % kLtStages * kLtStage;
+        const int k0 = s * kLtBK;
+        const bool in = k0 + piece * 8 < p.k;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-      // Rows of other adapters, past the last row and past the rank are read as well, from valid
-      // places, and their sums are not kept: loads without conditions, so that four blocks of k are
-      // in flight. Only the end of K is masked.
-      const __nv_bfloat16 *xp[2][2], *ap[NT];
+        for (int i = 0; i < 2; ++i) {
+          const int r = prow + 16 * i;
+          lt_copy16(st + r * 128 + ((piece ^ (r & 7)) << 4), in ? xp[i] + k0 : p.x, in);
+        }
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+        for (int i = 0; i < 4; ++i) {
+          const int r = prow + 16 * i;
+          if (2 * i < used) lt_copy16(st + (kLtRows + r) * 128 + ((piece ^ (r & 7)) << 4), in ? ap[i] + k0 : p.a, in);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-          xp[m][hh] = p.x + min(row0 + m * 16 + hh * 8 + g, static_cast<int64_t>(p.rows) - 1) * p.x_stride + q * 8;
+    for (int s = 0; s < kLtStages - 1; ++s) issue(s);
+    float acc[2][2][4];  // 16 rows of x, rank tile
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        ap[j] = am + static_cast<int64_t>(min(r0 + j * 8 + g, p.rank - 1)) * p.k + q * 8;
-      auto block = [&](int k0, bool whole) {
-        uint4 xv[2][2], av[NT];
-        const bool in = whole || k0 + q * 8 < p.k;
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh)
-            xv[m][hh] = in ? *reinterpret_cast<const uint4 *>(xp[m][hh] + k0) : make_uint4(0, 0, 0, 0);
+        for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
+    const bool busy = 2 * warp < used;
+    // ldmatrix rows: x's of 16, and this warp's two rank tiles
+    const int lx = lane & 15, cx = lane >> 4, la = kLtRows + warp * 16 + (lane & 7) + ((lane >> 4) << 3), ca = (lane >> 3) & 1;
+    for (int s = 0; s < steps; ++s) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kLtStages - 2) : "memory");
+      __syncthreads();  // the stage is there, and the one before it has been read
+      issue(s + kLtStages - 1);
+      if (busy) {
+        const uint32_t st = ring_s + s % kLtStages * kLtStage;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          av[j] = in ? *reinterpret_cast<const uint4 *>(ap[j] + k0) : make_uint4(0, 0, 0, 0);
+        for (int kk = 0; kk < kLtBK / 16; ++kk) {
+          uint32_t xa[2][4], ab[4];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            mma_bf16_16816(acc[m][j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av[j].x, av[j].y);
-            mma_bf16_16816(acc[m][j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av[j].z, av[j].w);
-          }
-      };
-      const int whole = p.k / 32 * 32;
-      int k0 = warp * 32;
-#pragma unroll NT == 4 ? 4 : 2
-      for (; k0 < whole; k0 += 128) block(k0, true);
-      if (k0 < p.k) block(k0, false);
-      // warps 0 and 1 lay their sums down, 2 and 3 add theirs
-#pragma unroll
-      for (int turn = 0; turn < 2; ++turn) {
-        if (warp >> 1 == turn) {
+          for (int m = 0; m < 2; ++m)
+            lt_ldmatrix4(xa[m], st + (m * 16 + lx) * 128 + (((2 * kk + cx) ^ (lx & 7)) << 4));
+          lt_ldmatrix4(ab, st + la * 128 + (((2 * kk + ca) ^ (la & 7)) << 4));
 #pragma unroll
           for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float &to = part[warp & 1][m * 16 + g + (e >> 1) * 8][j * 8 + q * 2 + (e & 1)];
-                to = turn ? to + acc[m][j][e] : acc[m][j][e];
-              }
+            for (int j = 0; j < 2; ++j)
+              mma_bf16_16816(acc[m][j], xa[m][0], xa[m][1], xa[m][2], xa[m][3], ab[2 * j], ab[2 * j + 1]);
         }
-        __syncthreads();
       }
-      const float s = p.scales[ad];
-      for (int i = tid; i < kLtRows * 4 * NT; i += 128) {
-        const int r = i / (4 * NT), c = 2 * (i - r * (4 * NT));
-        if ((rows >> r & 1) && r0 + c < p.rank)
-          *reinterpret_cast<uint32_t *>(p.t + (row0 + r) * p.rank + r0 + c) =
-              pack2((part[0][r][c] + part[1][r][c]) * s, (part[0][r][c + 1] + part[1][r][c + 1]) * s);
-      }
-      __syncthreads();
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int tile = first + 2 * warp + j, at = min(tile, all - 1) / per, ad = list[at];
+      const float sc = p.scales[ad];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = m * 16 + h * 8 + g;
+          const bool keep = __shfl_sync(0xffffffffu, mine, r) == ad && tile < all;
+          if (keep)
+            *reinterpret_cast<uint32_t *>(p.t + static_cast<int64_t>(row0 + r) * p.rank + (tile - at * per) * 8 + 2 * q) =
+                pack2(acc[m][j][2 * h] * sc, acc[m][j][2 * h + 1] * sc);
+        }
+    }
+    __syncthreads();  // the ring may be filled anew
   }
 }
 
@@ -604,7 +636,7 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
   g.rank = rank;
   g.tiles_m = (rows + kLgTile - 1) / kLgTile;
   g.tiles_n = (n + kLgTile - 1) / kLgTile;
-  B200_REQUIRE(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 2, "lora_rows: too many tiles");
+  B200_REQUIRE(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 2 && rows <= 1 << 29, "lora_rows: too many tiles");
   LoraDownArgs p{};
   p.x = static_cast<const __nv_bfloat16 *>(x);
   p.x_stride = x_row_stride;
@@ -640,8 +672,12 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
       cudaFuncSetAttribute(lora_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmem),
       "lora_rows (configuration)");
   const int down = (rows + kLtRows - 1) / kLtRows;
-  auto kfn = rank <= 32 ? lora_down_rows_kernel<4> : lora_down_rows_kernel<8>;
-  B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(down + g.tiles_m), dim3(128), 0, st, true, 1, p), "lora_rows (down)");
+  B200_LAUNCH_CHECK_ERR(
+      cudaFuncSetAttribute(lora_down_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtStages * kLtStage),
+      "lora_rows (configuration)");
+  B200_LAUNCH_CHECK_ERR(launch_kernel(lora_down_rows_kernel, dim3(down + g.tiles_m), dim3(128), kLtStages * kLtStage,
+                                      st, true, 1, p),
+                        "lora_rows (down)");
   const int pairs = std::min(g.tiles_m * g.tiles_n, num_sms() / 2);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * pairs);

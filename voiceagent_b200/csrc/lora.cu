@@ -5,6 +5,8 @@
 // lora_down   rows of a decode step: t = s_a x A_a^T in 32 bits, which the projection's own
 //             epilogue expands (linear.cu, b200asr_linear_small_lora).
 // lora_rows   any number of rows: t as bf16, then x W^T and t B^T in one accumulator.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b200asr {
@@ -213,53 +215,59 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
     };
 #pragma unroll
     for (int s = 0; s < kLtStages - 1; ++s) issue(s);
-    float acc[2][2][4];  // 16 rows of x, rank tile
+    // A warp takes 16 of the rows and one or two pairs of rank tiles; all of a stage's operands are
+    // read before its products.
+    const int m = warp & 1, pair0 = warp >> 1;
+    float acc[2][2][4];  // pair pair0 or pair0 + 2, tile of it
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-    const bool busy = 2 * warp < used;
-    // ldmatrix rows: x's of 16, and this warp's two rank tiles
-    const int lx = lane & 15, cx = lane >> 4, la = kLtRows + warp * 16 + (lane & 7) + ((lane >> 4) << 3), ca = (lane >> 3) & 1;
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+    const int lx = m * 16 + (lane & 15), cx = lane >> 4;
+    const int la = kLtRows + pair0 * 16 + (lane & 7) + ((lane >> 4) << 3), ca = (lane >> 3) & 1;
+    auto stage = [&](uint32_t st, auto pairs) {
+      constexpr int PAIRS = decltype(pairs)::value;
+      uint32_t xa[kLtBK / 16][4], ab[PAIRS][kLtBK / 16][4];
+#pragma unroll
+      for (int kk = 0; kk < kLtBK / 16; ++kk) {
+        lt_ldmatrix4(xa[kk], st + lx * 128 + (((2 * kk + cx) ^ (lx & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i)
+          lt_ldmatrix4(ab[i][kk], st + (la + 32 * i) * 128 + (((2 * kk + ca) ^ (la & 7)) << 4));
+      }
+#pragma unroll
+      for (int kk = 0; kk < kLtBK / 16; ++kk)
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            mma_bf16_16816(acc[i][j], xa[kk][0], xa[kk][1], xa[kk][2], xa[kk][3], ab[i][kk][2 * j], ab[i][kk][2 * j + 1]);
+    };
     for (int s = 0; s < steps; ++s) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kLtStages - 2) : "memory");
       __syncthreads();  // the stage is there, and the one before it has been read
       issue(s + kLtStages - 1);
-      if (busy) {
-        const uint32_t st = ring_s + s % kLtStages * kLtStage;
-#pragma unroll
-        for (int kk = 0; kk < kLtBK / 16; ++kk) {
-          uint32_t xa[2][4], ab[4];
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-            lt_ldmatrix4(xa[m], st + (m * 16 + lx) * 128 + (((2 * kk + cx) ^ (lx & 7)) << 4));
-          lt_ldmatrix4(ab, st + la * 128 + (((2 * kk + ca) ^ (la & 7)) << 4));
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              mma_bf16_16816(acc[m][j], xa[m][0], xa[m][1], xa[m][2], xa[m][3], ab[2 * j], ab[2 * j + 1]);
-        }
-      }
+      const uint32_t st = ring_s + s % kLtStages * kLtStage;
+      if (used > 4) stage(st, std::integral_constant<int, 2>());
+      else if (2 * pair0 < used) stage(st, std::integral_constant<int, 1>());
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int tile = first + 2 * warp + j, at = min(tile, all - 1) / per, ad = list[at];
-      const float sc = p.scales[ad];
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int j = 0; j < 2; ++j) {
+        const int tile = first + 2 * (pair0 + 2 * i) + j, at = min(tile, all - 1) / per, ad = list[at];
+        const float sc = p.scales[ad];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = m * 16 + h * 8 + g;
-          const bool keep = __shfl_sync(0xffffffffu, mine, r) == ad && tile < all;
-          if (keep)
+          if (__shfl_sync(0xffffffffu, mine, r) == ad && tile < first + used)
             *reinterpret_cast<uint32_t *>(p.t + static_cast<int64_t>(row0 + r) * p.rank + (tile - at * per) * 8 + 2 * q) =
-                pack2(acc[m][j][2 * h] * sc, acc[m][j][2 * h + 1] * sc);
+                pack2(acc[i][j][2 * h] * sc, acc[i][j][2 * h + 1] * sc);
         }
-    }
+      }
     __syncthreads();  // the ring may be filled anew
   }
 }
@@ -272,15 +280,15 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
 // is written out while the next one's products run.
 // The adapters are more K steps at the end of a tile, one per distinct adapter of its 256 rows
 // (and 64 ranks): the weight side is 256 rows of B_a, the row side t with zeros in the rows of
-// other adapters, which four warps write in the layout the MMA reads. They have a buffer and
-// barriers of their own, so the ring of x and W runs on.
+// other adapters, which four warps write in the layout the MMA reads. They go through the same
+// ring, a barrier beside its slot's counting the t rows.
 //   warps 0-3 epilogue | 4-7 t rows | 8 TMA | 9 TMEM and MMA (of the pair's first CTA)
 constexpr int kLgThreads = 320;
 constexpr int kLgBK = 64;
-constexpr int kLgStages = 6;
+constexpr int kLgStages = 7;
 constexpr int kLgHalf = 128 * kLgBK * 2;          // 16 KB: 128 rows of x or of W
 constexpr int kLgStage = 2 * kLgHalf;
-constexpr int kLgSmem = 1024 + (kLgStages + 1) * kLgStage + 256;
+constexpr int kLgSmem = 1024 + kLgStages * kLgStage + 512;
 static_assert(kLgSmem <= 232448, "shared memory of a CTA");
 
 struct LoraGemmArgs {
@@ -370,16 +378,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
                      const __grid_constant__ CUtensorMap tm_b, const LoraGemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *ring = smem;                                   // [stage] x half | W half
-  uint8_t *lora = smem + kLgStages * kLgStage;            // t half | B half
-  uint64_t *bars = reinterpret_cast<uint64_t *>(lora + kLgStage);
+  uint8_t *ring = smem;                        // [stage] x half | W half, or t half | B half
+  uint64_t *bars = reinterpret_cast<uint64_t *>(ring + kLgStages * kLgStage);
   uint64_t *full = bars;                       // first CTA's: both CTAs' loads of the stage
   uint64_t *empty = full + kLgStages;          // each CTA's: the stage's MMAs are done
   uint64_t *acc_full = empty + kLgStages;      // [2] each CTA's: the tile's MMAs are done
   uint64_t *acc_empty = acc_full + 2;          // [2] first CTA's: both CTAs' warps have read it
-  uint64_t *l_full = acc_empty + 2;            // first CTA's: B of both CTAs and every t row
-  uint64_t *l_empty = l_full + 1;              // each CTA's
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(l_empty + 1);
+  uint64_t *t_full = acc_empty + 2;            // first CTA's: every t row of the stage is written
+  // Each CTA's: the stage may take t rows. The writers do not follow every stage, so the TMA thread,
+  // which does, tells them: waiting for `empty` themselves they could be two phases off.
+  uint64_t *t_go = t_full + kLgStages;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(t_go + kLgStages);
   __shared__ int abort_flag;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -390,13 +399,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
     for (int s = 0; s < kLgStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&t_full[s], 8);
+      mbar_init(&t_go[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 8);
     }
-    mbar_init(l_full, 1 + 8);
-    mbar_init(l_empty, 1);
     fence_barrier_init();
   }
   if (warp == 9) {
@@ -422,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
     // x and W do not wait for lora_down_rows: it lets this launch begin once it has itself waited
     // for x. The plan and t do, here and below.
     if (lane == 0) {
-      uint32_t it = 0, lt = 0;
+      uint32_t it = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs) {
         const int m0 = tile_m(t) * kLgTile + rank * 128, n0 = tile_n(t) * kLgTile + rank * 128;
@@ -437,12 +446,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
         }
         pdl_wait();
         const int steps = lora_steps(t);
-        for (int s = 0; s < steps && ok; ++s, ++lt) {
-          ok = lg_wait(l_empty, (lt & 1) ^ 1, a.error_flag, &abort_flag);
+        for (int s = 0; s < steps && ok; ++s, ++it) {
+          const int st = it % kLgStages;
+          ok = lg_wait(&empty[st], ((it / kLgStages) & 1) ^ 1, a.error_flag, &abort_flag);
           if (!ok) break;
-          if (rank == 0) mbar_arrive_expect_tx(l_full, 2 * kLgHalf);
+          mbar_arrive(&t_go[st]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * kLgHalf);
           const int ad = a.plan[static_cast<int64_t>(tile_m(t)) * kLgPlan + 1 + s / chunks];
-          lg_load_3d(lora + kLgHalf, &tm_b, (s % chunks) * kLgBK, n0, ad, lg_first(smem_addr(l_full)));
+          lg_load_3d(ring + st * kLgStage + kLgHalf, &tm_b, (s % chunks) * kLgBK, n0, ad,
+                     lg_first(smem_addr(&full[st])));
         }
       }
     }
@@ -450,7 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
     // ---------------------------------------------------------------------- MMAs
     if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc = idesc_bf16_f32(256, 256, false, false);
-      uint32_t it = 0, lt = 0;
+      uint32_t it = 0, t_phase = 0;  // t_phase: bit st is the parity of t_full[st]'s next phase
       int j = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs, ++j) {
@@ -473,15 +485,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
         }
         pdl_wait();
         const int steps = ok ? lora_steps(t) : 0;
-        for (int s = 0; s < steps; ++s, ++lt) {
-          ok = lg_wait(l_full, lt & 1, a.error_flag, &abort_flag);
+        for (int s = 0; s < steps; ++s, ++it) {
+          const int st = it % kLgStages;
+          ok = lg_wait(&full[st], (it / kLgStages) & 1, a.error_flag, &abort_flag) &&
+               lg_wait(&t_full[st], (t_phase >> st) & 1, a.error_flag, &abort_flag);
           if (!ok) break;
+          t_phase ^= 1u << st;
           tc_fence_after();
-          const uint32_t tb = smem_addr(lora), bb = tb + kLgHalf;
+          const uint32_t tb = smem_addr(ring + st * kLgStage), bb = tb + kLgHalf;
           const int kmax = (min(kLgBK, a.rank - (s % chunks) * kLgBK) + 15) / 16;
           for (int kk = 0; kk < kmax; ++kk)
             lg_mma(d, smem_desc_sw128(tb + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024), idesc, 1u);
-          lg_commit(l_empty);
+          lg_commit(&empty[st]);
         }
         if (ok) lg_commit(&acc_full[acc]);
       }
@@ -490,15 +505,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
     // ------------------------------------------------------- t rows of the adapters
     const int r = tid - 128;  // row of this CTA's half
     pdl_wait();
-    uint8_t *dst = lora + (r >> 3) * 1024 + (r & 7) * 128;
-    uint32_t lt = 0;
+    uint8_t *dst = ring + (r >> 3) * 1024 + (r & 7) * 128;
+    uint32_t it = 0, go_phase = 0;  // go_phase: bit st is the parity of t_go[st]'s next phase
     bool ok = true;
     for (int t = pair; t < tiles && ok; t += pairs) {
       const int64_t row = static_cast<int64_t>(tile_m(t)) * kLgTile + rank * 128 + r;
       const int mine = row < a.rows ? a.row_adapter[row] : -1;
       const int32_t *plan = a.plan + static_cast<int64_t>(tile_m(t)) * kLgPlan;
       const int steps = plan[0] * chunks;
-      for (int s = 0; s < steps; ++s, ++lt) {
+      it += a.k_steps;
+      for (int s = 0; s < steps; ++s, ++it) {
+        const int st = it % kLgStages;
         const int c0 = (s % chunks) * kLgBK;
         const bool own_row = mine == plan[1 + s / chunks];
         uint4 v[8];
@@ -508,13 +525,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
           if (own_row && c0 + c * 8 < a.rank)
             v[c] = *reinterpret_cast<const uint4 *>(a.t + row * a.rank + c0 + c * 8);
         }
-        ok = __all_sync(0xffffffffu, lg_wait(l_empty, (lt & 1) ^ 1, a.error_flag, &abort_flag));
+        ok = __all_sync(0xffffffffu, lg_wait(&t_go[st], (go_phase >> st) & 1, a.error_flag, &abort_flag));
         if (!ok) break;
+        go_phase ^= 1u << st;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4 *>(dst + ((c ^ (r & 7)) << 4)) = v[c];
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4 *>(dst + st * kLgStage + ((c ^ (r & 7)) << 4)) = v[c];
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) lg_arrive_first(l_full);
+        if (lane == 0) lg_arrive_first(&t_full[st]);
       }
     }
   } else {

@@ -81,17 +81,19 @@ __global__ void __launch_bounds__(128) lora_down_kernel(
 
 // ------------------------------------------------------------------ down, any rows
 // A CTA takes 32 rows of x and streams them once, with the rows of A they need, through a ring of
-// cp.async stages of 64 k (128-byte swizzle, so that ldmatrix meets no bank twice); mma m16n8k16.
-// What the rows need is a list of rank tiles of 8, adapter after adapter: eight of them go through
-// a pass, a warp two, so that a prefill batch's tile, which has one or two adapters, is one pass
-// at ranks up to 32. Two CTAs per SM keep 120 KB on their way. t is rounded to bf16 once, as
-// activations between projections are: it is the operand of the second product. The last CTAs of
-// the launch list each 256-row tile's distinct adapters for that product.
-// (Operands straight from global memory, the warps splitting K: 34 us for 7829 rows of 2048.)
+// TMA stages of 64 k (128-byte swizzle, so that ldmatrix meets no bank twice); mma m16n8k16 by four
+// warps, the fifth loads. What the rows need is a list of rank tiles of 8, adapter after adapter:
+// eight of them go through a pass, so that a prefill batch's tile, which has one or two adapters, is
+// one pass at ranks up to 32. A stage's products take ~250 cycles, so loads by the same warps (six
+// cp.async and their addresses a thread, ~600 cycles a stage) took 12 us a pass of K = 2048. t is
+// rounded to bf16 once, as activations between projections are: it is the operand of the second
+// product. The last CTAs of the launch list each 256-row tile's distinct adapters for that product.
 constexpr int kLtRows = 32;
 constexpr int kLtBK = 64, kLtTiles = 8;  // k of a stage, rank tiles of a pass
-constexpr int kLtStages = 6;
+constexpr int kLtStages = 8;
+constexpr int kLtThreads = 160;
 constexpr int kLtStage = (kLtRows + 8 * kLtTiles) * kLtBK * 2;
+constexpr int kLtSmem = 1024 + kLtStages * kLtStage + 256;
 constexpr int kLoraMaxRank = 128;
 constexpr int kLgTile = 256;            // rows and columns of a CTA pair's tile
 constexpr int kLgPlan = 1 + kLgTile;    // plan entry of a row tile: count, adapters
@@ -118,8 +120,12 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t a0,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void lt_copy16(uint32_t dst, const void *src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void lt_load_2d(void *dst, const CUtensorMap *map, int c0, int c1, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_addr(bar))
+      : "memory");
 }
 __device__ __forceinline__ void lt_ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -156,13 +162,31 @@ __device__ __forceinline__ void lora_plan(const LoraDownArgs &p, int tile) {
   if (lane == 0) out[0] = count;
 }
 
-__global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs p) {
-  extern __shared__ __align__(1024) uint8_t ring[];
-  __shared__ int list[kLtRows];
-  pdl_wait();
-  pdl_trigger();  // after the wait: the product reads x before its own
+// Rank tiles a copy of A brings: the more the fewer copies; a whole number of them makes an adapter
+// and a pass.
+__host__ __device__ __forceinline__ int lt_box(int rank) {
+  return rank % 64 == 0 ? 8 : rank % 32 == 0 ? 4 : rank % 16 == 0 ? 2 : 1;
+}
+
+__global__ void __launch_bounds__(kLtThreads) lora_down_rows_kernel(const __grid_constant__ CUtensorMap tm_x,
+                                                                    const __grid_constant__ CUtensorMap tm_a,
+                                                                    const LoraDownArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *full = reinterpret_cast<uint64_t *>(ring + kLtStages * kLtStage), *empty = full + kLtStages;
+  __shared__ int list[kLtRows], abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int tiles = (p.rows + kLtRows - 1) / kLtRows;
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kLtStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    fence_barrier_init();
+  }
+  pdl_wait();
+  pdl_trigger();  // after the wait: the product reads x before its own
   if (static_cast<int>(blockIdx.x) >= tiles) {
     lora_plan(p, blockIdx.x - tiles);
     return;
@@ -179,42 +203,35 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
   }
   __syncthreads();
   const int per = p.rank / 8, all = distinct * per;  // rank tiles of an adapter, and in all
-  const int steps = (p.k + kLtBK - 1) / kLtBK;
-  const uint32_t ring_s = smem_addr(ring);
-  // This thread's pieces of a stage: 16 bytes of 2 rows of x and of 4 rows of A.
-  const int piece = tid & 7, prow = tid >> 3;
-  const __nv_bfloat16 *xp[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)  // (past the last row: the last one again, not kept)
-    xp[i] = p.x + static_cast<int64_t>(min(row0 + prow + 16 * i, p.rows - 1)) * p.x_stride + piece * 8;
-  for (int first = 0; first < all; first += kLtTiles) {
-    const int used = min(kLtTiles, all - first);
-    const __nv_bfloat16 *ap[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // (past the last tile: the last one again, not kept)
-      const int r = prow + 16 * i, tile = min(first + (r >> 3), all - 1), at = tile / per;
-      ap[i] = p.a + (static_cast<int64_t>(list[at]) * p.rank + (tile - at * per) * 8 + (r & 7)) * p.k + piece * 8;
-    }
-    auto issue = [&](int s) {
-      if (s < steps) {
-        const uint32_t st = ring_s + s % kLtStages * kLtStage;
-        const int k0 = s * kLtBK;
-        const bool in = k0 + piece * 8 < p.k;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = prow + 16 * i;
-          lt_copy16(st + r * 128 + ((piece ^ (r & 7)) << 4), in ? xp[i] + k0 : p.x, in);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = prow + 16 * i;
-          if (2 * i < used) lt_copy16(st + (kLtRows + r) * 128 + ((piece ^ (r & 7)) << 4), in ? ap[i] + k0 : p.a, in);
+  const int steps = (p.k + kLtBK - 1) / kLtBK, box = lt_box(p.rank);
+  if (warp == 4) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int first = 0; first < all && ok; first += kLtTiles) {
+        const int used = min(kLtTiles, all - first);
+        for (int s = 0; s < steps; ++s, ++it) {
+          const int st = it % kLtStages;
+          ok = mbar_wait(&empty[st], ((it / kLtStages) & 1) ^ 1, p.error_flag, &abort_flag);
+          if (!ok) break;
+          uint8_t *to = ring + st * kLtStage;
+          mbar_arrive_expect_tx(&full[st], (kLtRows + 8 * used) * kLtBK * 2);
+          lt_load_2d(to, &tm_x, s * kLtBK, row0, &full[st]);
+          for (int i = 0; i < used; i += box) {
+            const int at = (first + i) / per;
+            tma_load_3d(to + (kLtRows + 8 * i) * 128, &tm_a, s * kLtBK, (first + i - at * per) * 8, list[at], &full[st]);
+          }
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int s = 0; s < kLtStages - 1; ++s) issue(s);
+      if (abort_flag)  // let the copies already issued land before the CTA exits
+        for (uint32_t i = it > kLtStages ? it - kLtStages : 0; i < it; ++i)
+          mbar_drain(&full[i % kLtStages], (i / kLtStages) & 1);
+    }
+    return;
+  }
+  uint32_t it = 0;
+  for (int first = 0; first < all; first += kLtTiles) {
+    const int used = min(kLtTiles, all - first);
     // A warp takes 16 of the rows and one or two pairs of rank tiles; all of a stage's operands are
     // read before its products.
     const int m = warp & 1, pair0 = warp >> 1;
@@ -245,15 +262,15 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
           for (int j = 0; j < 2; ++j)
             mma_bf16_16816(acc[i][j], xa[kk][0], xa[kk][1], xa[kk][2], xa[kk][3], ab[i][kk][2 * j], ab[i][kk][2 * j + 1]);
     };
-    for (int s = 0; s < steps; ++s) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kLtStages - 2) : "memory");
-      __syncthreads();  // the stage is there, and the one before it has been read
-      issue(s + kLtStages - 1);
-      const uint32_t st = ring_s + s % kLtStages * kLtStage;
-      if (used > 4) stage(st, std::integral_constant<int, 2>());
-      else if (2 * pair0 < used) stage(st, std::integral_constant<int, 1>());
+    for (int s = 0; s < steps; ++s, ++it) {
+      const int st = it % kLtStages;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (it / kLtStages) & 1, p.error_flag, &abort_flag))) return;
+      const uint32_t at = smem_addr(ring + st * kLtStage);
+      if (used > 4) stage(at, std::integral_constant<int, 2>());
+      else if (2 * pair0 < used) stage(at, std::integral_constant<int, 1>());
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -268,7 +285,6 @@ __global__ void __launch_bounds__(128) lora_down_rows_kernel(const LoraDownArgs 
                 pack2(acc[i][j][2 * h] * sc, acc[i][j][2 * h + 1] * sc);
         }
       }
-    __syncthreads();  // the ring may be filled anew
   }
 }
 
@@ -690,11 +706,17 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
       cudaFuncSetAttribute(lora_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmem),
       "lora_rows (configuration)");
   const int down = (rows + kLtRows - 1) / kLtRows;
+  CUtensorMap dx, da;
+  const uint32_t dx_box[2] = {kLtBK, kLtRows}, da_box[3] = {kLtBK, 8u * lt_box(rank), 1};
+  const uint64_t ad[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rank), static_cast<uint64_t>(num_adapters)};
+  const uint64_t as[2] = {static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(k) * rank * 2};
+  if (!make_tmap_bf16(&dx, x, 2, xd, xs, dx_box) || !make_tmap_bf16(&da, lora_a, 3, ad, as, da_box))
+    return B200ASR_ERR_CUDA;
   B200_LAUNCH_CHECK_ERR(
-      cudaFuncSetAttribute(lora_down_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtStages * kLtStage),
+      cudaFuncSetAttribute(lora_down_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtSmem),
       "lora_rows (configuration)");
-  B200_LAUNCH_CHECK_ERR(launch_kernel(lora_down_rows_kernel, dim3(down + g.tiles_m), dim3(128), kLtStages * kLtStage,
-                                      st, true, 1, p),
+  B200_LAUNCH_CHECK_ERR(launch_kernel(lora_down_rows_kernel, dim3(down + g.tiles_m), dim3(kLtThreads), kLtSmem, st,
+                                      true, 1, dx, da, p),
                         "lora_rows (down)");
   const int pairs = std::min(g.tiles_m * g.tiles_n, num_sms() / 2);
   cudaLaunchConfig_t cfg = {};

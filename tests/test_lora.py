@@ -97,6 +97,31 @@ def test_strided_rows_given_out_and_nan_of_other_adapters(kx, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [40, 300])
+def test_values_that_are_not_finite_in_b_reach_their_adapter_alone(kx, rows):
+    """Rows of several adapters share a tile of the product: 0 * inf must not join them."""
+    x, w, a, b, s = inputs(rows, 128, 256, 16, 4, 9)
+    ids = torch.arange(rows, device="cuda").remainder(5).sub(1).int()
+    want = plain(x, w, a, b, s, ids)
+    b[2, 7, 3], b[2, 200, 0] = float("inf"), float("nan")
+    b[3, 40:80] = float("nan")
+    got = kx.lora_linear(x, w, a, b, s, ids)
+    wild = torch.zeros(rows, 256, dtype=torch.bool, device="cuda")
+    wild[ids == 2, 7] = wild[ids == 2, 200] = True
+    wild[(ids == 3)[:, None] & (torch.arange(256, device="cuda") // 40 == 1)] = True
+    assert not got[wild].isfinite().any()
+    got[wild] = torch.from_numpy(want[0]).cuda()[wild].to(BF16)
+    check(got, want)
+    w[5, 9] = float("nan")  # the shared weights reach every row
+    x[1] = float("inf")     # and a row of x its own
+    got = kx.lora_linear(x, w, a, b, s, ids)
+    wild[:, 5] = wild[1] = True
+    assert not got[wild].isfinite().any()
+    got[wild] = torch.from_numpy(want[0]).cuda()[wild].to(BF16)
+    check(got, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [5, 70])
 def test_bad_indices_are_flagged_and_count_as_none(kx, rows):
     args = inputs(rows, 128, 128, 8, 2)

@@ -20,9 +20,9 @@
 //  * A word of 8 codes gives the pairs (i, i + 4), so dims are permuted within groups of 8;
 //    q is laid out alike, and the output is put back in order as it is written.
 //  * Values are zero + code * scale in one rounding, and q, K, V and P go through the tensor
-//    cores as fp16, 11 bits where bf16 keeps 8 (error of the output against 64 bits, relative:
-//    0.0042 with bf16, of which the output's own rounding is 0.0017). q is brought to fp16's
-//    range by a power of two per row, K by one per 32 tokens, both undone in the factor of the
+//    cores as fp16, 11 bits where bf16 keeps 8 (root mean square error of the output against 64
+//    bits, relative to its own: 0.0042 with bf16, of which the output's rounding is 0.0017). q is
+//    brought to fp16's range by a power of two per row, K by one per 32 tokens, both undone in the factor of the
 //    scores. V carries no such factor, so 32 tokens whose V rows do not lie within
 //    [2^-10, 2^15] (or are zero) go through as bf16, with their P.
 //  * A V row that is not finite is written as zeros and its K row as NaN: the rows that may
@@ -207,16 +207,20 @@ __device__ __forceinline__ uint32_t p4_f16x2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
-// 8 codes as four pairs of values zero + code * scale, dims (i, i + 4); bf16 from 128 + code.
+// 8 codes as four pairs of values zero + code * scale, dims (i, i + 4); bf16 from 128 + code. The
+// top codes of a row that ends at the largest bf16 may round past it: held there, since an infinity
+// would reach the rows that do not see it (0 * inf).
 __device__ __forceinline__ uint4 p4_values_bf16(uint32_t w, uint32_t scale2, uint32_t zero2) {
   uint32_t out[4];
   const uint32_t k = 0xc300c300u;  // -128, -128
+  const uint32_t most = 0x7f7f7f7fu;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t p = p4_and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
     __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&p);
     x = __hadd2(x, *reinterpret_cast<const __nv_bfloat162 *>(&k));  // code, exact
     x = __hfma2(x, *reinterpret_cast<const __nv_bfloat162 *>(&scale2), *reinterpret_cast<const __nv_bfloat162 *>(&zero2));
+    x = __hmin2(x, *reinterpret_cast<const __nv_bfloat162 *>(&most));
     out[i] = *reinterpret_cast<uint32_t *>(&x);
   }
   return make_uint4(out[0], out[1], out[2], out[3]);

@@ -316,7 +316,45 @@ struct LoraGemmArgs {
   __nv_bfloat16 *y;
   int64_t y_stride;
   int32_t *error_flag;
+  // for lora_put_right alone
+  const __nv_bfloat16 *x, *w, *b;
+  int64_t x_stride;
+  int k, num_adapters;
 };
+
+// A row has zeros for t in the steps of other adapters, which leaves it alone while their B is
+// finite: 0 * inf would reach it. So where 32 columns just written hold an infinity or a NaN, those
+// that come from a row of B of another adapter than the row's own are worked out anew without it,
+// a warp per element.
+__device__ __noinline__ void lora_put_right(const LoraGemmArgs &a, int64_t row, const int32_t *plan, int n0) {
+  const int lane = threadIdx.x & 31;
+  auto wild = [](__nv_bfloat16 v) { return !(fabsf(bf2f(v)) < INFINITY); };
+  int mine = row < a.rows ? a.row_adapter[row] : -1;
+  if (mine < 0 || mine >= a.num_adapters) mine = -1;
+  for (int n = n0; n < min(n0 + 32, a.n); ++n) {
+    const bool bad = row < a.rows && wild(a.y[row * a.y_stride + n]);
+    if (!__any_sync(0xffffffffu, bad)) continue;
+    bool others = false;
+    for (int i = 0; i < plan[0]; ++i) {
+      const int ad = plan[1 + i];
+      bool inf = false;
+      for (int r = lane; r < a.rank; r += 32) inf = inf || wild(a.b[(static_cast<int64_t>(ad) * a.n + n) * a.rank + r]);
+      const bool any = __any_sync(0xffffffffu, inf);  // (by every lane, whatever `others` is)
+      others = others || (any && ad != mine);
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, bad && others); left; left &= left - 1) {
+      const int src = __ffs(left) - 1, ad = __shfl_sync(0xffffffffu, mine, src);
+      const int64_t t = row - lane + src;  // a warp's rows follow one another
+      float sum = 0.f;
+      for (int i = lane; i < a.k; i += 32)
+        sum = fmaf(bf2f(a.x[t * a.x_stride + i]), bf2f(a.w[static_cast<int64_t>(n) * a.k + i]), sum);
+      for (int r = lane; ad >= 0 && r < a.rank; r += 32)
+        sum = fmaf(bf2f(a.t[t * a.rank + r]), bf2f(a.b[(static_cast<int64_t>(ad) * a.n + n) * a.rank + r]), sum);
+      sum = warp_sum(sum);
+      if (lane == src) a.y[t * a.y_stride + n] = f2bf(sum);
+    }
+  }
+}
 
 __device__ __forceinline__ uint32_t lg_rank() {
   uint32_t r;
@@ -391,7 +429,7 @@ __device__ __forceinline__ void lg_commit(uint64_t *bar) {
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                     const __grid_constant__ CUtensorMap tm_b, const LoraGemmArgs a) {
+                     const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ LoraGemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *ring = smem;                        // [stage] x half | W half, or t half | B half
@@ -577,6 +615,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1)
                   make_uint4(pack2(v[8 * i], v[8 * i + 1]), pack2(v[8 * i + 2], v[8 * i + 3]),
                              pack2(v[8 * i + 4], v[8 * i + 5]), pack2(v[8 * i + 6], v[8 * i + 7]));
         }
+        float wild[4] = {0.f, 0.f, 0.f, 0.f};  // NaN once a value is not finite
+#pragma unroll
+        for (int i = 0; i < 32; ++i) wild[i & 3] = fmaf(v[i], 0.f, wild[i & 3]);
+        if (__any_sync(0xffffffffu, !((wild[0] + wild[1]) + (wild[2] + wild[3]) == 0.f)))
+          lora_put_right(a, row, a.plan + static_cast<int64_t>(tile_m(t)) * kLgPlan, n0 + c);
       }
       tc_fence_before();
       __syncwarp();
@@ -671,6 +714,12 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
   g.tiles_m = (rows + kLgTile - 1) / kLgTile;
   g.tiles_n = (n + kLgTile - 1) / kLgTile;
   B200_REQUIRE(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 2 && rows <= 1 << 29, "lora_rows: too many tiles");
+  g.x = static_cast<const __nv_bfloat16 *>(x);
+  g.x_stride = x_row_stride;
+  g.w = static_cast<const __nv_bfloat16 *>(w);
+  g.b = static_cast<const __nv_bfloat16 *>(lora_b);
+  g.k = k;
+  g.num_adapters = num_adapters;
   LoraDownArgs p{};
   p.x = static_cast<const __nv_bfloat16 *>(x);
   p.x_stride = x_row_stride;

@@ -7,7 +7,7 @@
 // 128 (the MMA's M) that share every K and V tile of 128 tokens:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, thread = row = TMEM lane
 //   warps 8-11      codes to bf16: K and V tiles into shared memory, 128-byte swizzled
-//   warp 12         TMEM and tcgen05.mma
+//   warps 12, 13    tcgen05.mma of tile 0 / 1 (12: TMEM)
 // What bounds it: per 128 tokens of one KV head (D = 128) the tensor cores need 2048 cycles for
 // both row tiles, the 32768 exponentials 2048 cycles of the special-function units, and the
 // codes of K and V ~600 instructions per converting thread, a quarter of what two row
@@ -35,7 +35,7 @@
 
 namespace b200asr {
 
-constexpr int kP4Threads = 16 * 32;  // warps 13 to 15 only give their registers away
+constexpr int kP4Threads = 16 * 32;  // warps 14 and 15 only give their registers away
 constexpr int kP4Rows = 256, kP4Keys = 128;
 constexpr float kP4Lazy = 8.f;
 
@@ -164,6 +164,16 @@ __device__ __forceinline__ void p4_tmem_st16(uint32_t taddr, const uint32_t *v) 
       : "memory");
 }
 
+__device__ __forceinline__ void p4_tmem_ld16(uint32_t taddr, float *v) {
+  uint32_t *u = reinterpret_cast<uint32_t *>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(taddr)
+      : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void p4_more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -255,10 +265,11 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   uint64_t *bars = reinterpret_cast<uint64_t *>(sV + 2 * C::TILE);
   uint64_t *q_full = bars;            // [2] rows of the item laid out
   uint64_t *k_full = bars + 2, *k_empty = bars + 4, *v_full = bars + 6, *v_empty = bars + 8;  // [2] each
-  uint64_t *s_full = bars + 10;       // [2] scores of the row tile (and its earlier P V) done
-  uint64_t *p_full = bars + 12;       // [2] P written, O rescaled
-  uint64_t *o_full = bars + 14;       // [2] the item's last P V done
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
+  uint64_t *s_full = bars + 10;       // [2][2] scores of the row tile and half done
+  uint64_t *p_full = bars + 14;       // [2][2] P written, O rescaled
+  uint64_t *pv_done = bars + 18;      // [2] a P V of the row tile done
+  uint64_t *o_full = bars + 20;       // [2] the item's last P V done
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
   __shared__ int abort_flag;
   __shared__ int lens[kP4Sorted];
   __shared__ uint16_t order[kP4Sorted];
@@ -274,11 +285,14 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
       mbar_init(&k_full[i], 4);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
       mbar_init(&v_full[i], 4);
-      mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&v_empty[i], 2);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s_full[2 * i + h], 1);
+        mbar_init(&p_full[2 * i + h], 4);
+      }
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
     }
     fence_barrier_init();
@@ -355,7 +369,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
       arrive(&q_full[w]);
       return a.scale_log2 * mine;
     };
-    uint32_t ps = 0, po = 0;  // phases of this row tile's scores and outputs
+    uint32_t ps = 0, po = 0, pv = 0;  // phases of this row tile's scores and outputs, its halves so far
     uint32_t jg = 0;          // K/V tiles of the items so far
     float next_factor = 0.f;
     bool more = walk.next(a, it);
@@ -373,36 +387,38 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
       const int all_seen = min(cur.offset + first_row / a.group, cur.n_kv - 1);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      // One tile: scores to P. MASKED where some row of the warp does not see all its keys.
-      auto softmax_tile = [&](auto masked, int j, const float *factors) {
+      // Half a tile: scores to P. MASKED where some row of the warp does not see all its keys.
+      auto softmax_half = [&](auto masked, int j, int h, const float *factors) {
         constexpr bool MASKED = decltype(masked)::value;
-        const int lim = last - j * kP4Keys;  // the last column this row sees
+        const int lim = last - j * kP4Keys - h * 64;  // the last column this row sees
+        const uint32_t at = s_base + h * 64;
         float mx = -INFINITY;
-        float s[2][32];  // 32 columns at hand and the next 32 on their way
-        tmem_ld32(s_base, s[0]);
+        float s[2][32];
+        tmem_ld32(at, s[0]);
+        tmem_ld32(at + 32, s[1]);
+        tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait_ld();
-          tmem_ld32(s_base + ((c + 1) & 3) * 32, s[(c + 1) & 1]);
-          const float *x = s[c & 1];
+        for (int c = 0; c < 2; ++c) {
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            top[i & 3] = fmaxf(top[i & 3], !MASKED || c * 32 + i <= lim ? x[i] : -INFINITY);
-          mx = fmaxf(mx, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (factor * fabsf(factors[c])));
+            top[i & 3] = fmaxf(top[i & 3], !MASKED || c * 32 + i <= lim ? s[c][i] : -INFINITY);
+          mx = fmaxf(mx, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (factor * fabsf(factors[2 * h + c])));
         }
         const bool move = mx > m + kP4Lazy || m == -INFINITY;
         const float m_new = move ? fmaxf(m, mx) : m;
         const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
-        if (j > 0 && __any_sync(0xffffffffu, move && alpha != 1.f)) {
+        if (j + h > 0 && __any_sync(0xffffffffu, move && alpha != 1.f)) {
+          if (!wait(&pv_done[w], pv - 1)) return false;  // O as the half before leaves it
+          tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            tmem_ld32(o_base + c, o);
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            p4_tmem_ld16(o_base + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(o_base + c, o);
+            for (int i = 0; i < 16; ++i) o[i] *= alpha;
+            p4_tmem_st16(o_base + c, reinterpret_cast<const uint32_t *>(o));
           }
         }
         m = m_new;
@@ -410,11 +426,9 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
         const float shift = m == -INFINITY ? 0.f : -m;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait_ld();  // (columns 0 to 31 again since the maxima)
-          if (c < 3) tmem_ld32(s_base + (c + 1) * 32, s[(c + 1) & 1]);
-          const float *x = s[c & 1];
-          const float fc = factors[c], f = factor * fabsf(fc);
+        for (int c = 0; c < 2; ++c) {
+          const float *x = s[c];
+          const float fc = factors[2 * h + c], f = factor * fabsf(fc);
           uint32_t p[16];
           float2 e[16];
 #pragma unroll
@@ -436,27 +450,30 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[i] = pack2(e[i].x, e[i].y);
           }
-          p4_tmem_st16(s_base + c * 16, p);  // over scores already read
+          p4_tmem_st16(at + c * 16, p);  // over scores already read
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
+        return true;
       };
       if (mine) {
-        for (int j = 0; j < cur.tiles; ++j, ++ps) {
-          if (!wait(&s_full[w], ps)) {
-            ok = false;
-            break;
+        for (int j = 0; j < cur.tiles && ok; ++j, ++ps) {
+          const float *factors = chunk_factor[(jg + j) & 3];
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h, ++pv) {
+            ok = wait(&s_full[2 * w + h], ps);
+            if (!ok) break;
+            tc_fence_after();
+            if (warp_rows) {
+              if (__all_sync(0xffffffffu, j * kP4Keys + h * 64 + 63 <= all_seen))
+                ok = softmax_half(std::false_type(), j, h, factors);
+              else
+                ok = softmax_half(std::true_type(), j, h, factors);
+              if (!ok) break;
+            }
+            tc_fence_before();
+            arrive(&p_full[2 * w + h]);
           }
-          tc_fence_after();
-          if (warp_rows) {
-            const float *factors = chunk_factor[(jg + j) & 3];
-            if (__all_sync(0xffffffffu, j * kP4Keys + kP4Keys - 1 <= all_seen))
-              softmax_tile(std::false_type(), j, factors);
-            else
-              softmax_tile(std::true_type(), j, factors);
-          }
-          tc_fence_before();
-          arrive(&p_full[w]);
         }
       }
       jg += cur.tiles;
@@ -664,73 +681,79 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   } else {
     // ---------------------------------------------------------------------- MMAs
     p4_fewer_registers<kP4RegMma>();
-    if (warp == 12) {
-    constexpr uint32_t idesc_s = p4_idesc_f16(128, kP4Keys, false);
-    constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true), idesc_o16 = p4_idesc_f16(128, D, true);
-    uint64_t q_desc[2], k_desc[2], v_desc[2];
+    if (warp < 14) {
+      // A warp per row tile: what lies between two products (waits, commits, descriptors; half of
+      // its time with one warp for both) passes under the other tile's.
+      const int w = warp - 12;
+      constexpr uint32_t idesc_s = p4_idesc_f16(128, kP4Keys / 2, false);
+      constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true), idesc_o16 = p4_idesc_f16(128, D, true);
+      const uint64_t q_desc = smem_desc_sw128(smem_addr(sQ + w * C::TILE), 16, 1024);
+      uint64_t k_desc[2], v_desc[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      q_desc[i] = smem_desc_sw128(smem_addr(sQ + i * C::TILE), 16, 1024);
-      k_desc[i] = smem_desc_sw128(smem_addr(sK + i * C::TILE), 16, 1024);
-      v_desc[i] = smem_desc_sw128(smem_addr(sV + i * C::TILE), C::BLOCK, 1024);
-    }
-    uint32_t jg = 0, items = 0, items1 = 0, tile0 = 0, tile1 = 0;
-    bool ok = true;
-    auto scores = [&](int w, uint32_t jj) {  // S_w = Q_w K^T of global tile jj
-      const uint64_t qd = w ? q_desc[1] : q_desc[0], kd = jj & 1 ? k_desc[1] : k_desc[0];
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint64_t off = ((k >> 2) * C::BLOCK + (k & 3) * 32) >> 4;
-        p4_mma_ss(tmem + w * 128, qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
+      for (int i = 0; i < 2; ++i) {
+        k_desc[i] = smem_desc_sw128(smem_addr(sK + i * C::TILE), 16, 1024);
+        v_desc[i] = smem_desc_sw128(smem_addr(sV + i * C::TILE), C::BLOCK, 1024);
       }
-      p4_commit(&s_full[w]);
-    };
-    while (ok && walk.next(a, it)) {
-      if (it.cut && lane == 0) raise_flag(a.error_flag, B200ASR_DEVERR_LENGTH);
-      if (it.tiles == 0) continue;
-      const int tiles_w = it.rows > 128 ? 2 : 1;
-      ok = wait(&q_full[0], items) && wait(&k_full[jg & 1], jg >> 1);
-      if (!ok) break;
-      tc_fence_after();
-      scores(0, jg);
-      if (tiles_w == 2) {
-        ok = wait(&q_full[1], items1);
+      const uint32_t s_at = tmem + w * 128, o_at = tmem + 256 + w * 128;
+      uint32_t jg = 0, items = 0, tile = 0;
+      bool ok = true;
+      auto scores = [&](uint32_t jj, int h) {  // S = Q K^T of half h of global tile jj
+        const uint64_t kd = (jj & 1 ? k_desc[1] : k_desc[0]) + ((h * 8192) >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = ((k >> 2) * C::BLOCK + (k & 3) * 32) >> 4;
+          p4_mma_ss(s_at + h * 64, q_desc + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
+        }
+        p4_commit(&s_full[2 * w + h]);
+      };
+      while (ok && walk.next(a, it)) {
+        if (it.cut && w == 0 && lane == 0) raise_flag(a.error_flag, B200ASR_DEVERR_LENGTH);
+        if (it.tiles == 0) continue;
+        if (w * 128 >= it.rows) {  // no row of this tile: it only gives K and V back
+          for (int j = 0; j < it.tiles && ok; ++j, ++jg) {
+            ok = wait(&k_full[jg & 1], jg >> 1);
+            if (!ok) break;
+            arrive(&k_empty[jg & 1]);
+            ok = wait(&v_full[jg & 1], jg >> 1);
+            if (!ok) break;
+            arrive(&v_empty[jg & 1]);
+          }
+          continue;
+        }
+        ok = wait(&q_full[w], items) && wait(&k_full[jg & 1], jg >> 1);
         if (!ok) break;
         tc_fence_after();
-        scores(1, jg);
-      }
-      p4_commit(&k_empty[jg & 1]);
-      for (int j = 0; j < it.tiles && ok; ++j, ++jg) {
-        for (int w = 0; w < tiles_w && ok; ++w) {
-          ok = wait(&p_full[w], w ? tile1 : tile0);
-          if (!ok) break;
-          if (w) ++tile1;
-          else ++tile0;
-          if (w == 0) ok = wait(&v_full[jg & 1], jg >> 1);
-          if (!ok) break;
-          tc_fence_after();
-          const float4 f = *reinterpret_cast<const float4 *>(chunk_factor[jg & 3]);
-          const uint32_t ids[4] = {f.x > 0.f ? idesc_o16 : idesc_o, f.y > 0.f ? idesc_o16 : idesc_o,
-                                   f.z > 0.f ? idesc_o16 : idesc_o, f.w > 0.f ? idesc_o16 : idesc_o};
+        scores(jg, 0);
+        scores(jg, 1);
+        p4_commit(&k_empty[jg & 1]);
+        for (int j = 0; j < it.tiles && ok; ++j, ++jg, ++tile) {
           const uint64_t vd = jg & 1 ? v_desc[1] : v_desc[0];
+          const bool next = j + 1 < it.tiles;
 #pragma unroll
-          for (int k = 0; k < kP4Keys / 16; ++k)
-            p4_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, vd + ((k * 2048) >> 4), ids[k >> 1],
-                      (j > 0 || k > 0) ? 1u : 0u);
-          if (w == tiles_w - 1) p4_commit(&v_empty[jg & 1]);
-          if (j == it.tiles - 1) p4_commit(&o_full[w]);
-          if (j + 1 < it.tiles) {
-            if (w == 0) ok = wait(&k_full[(jg + 1) & 1], (jg + 1) >> 1);
+          for (int h = 0; h < 2; ++h) {
+            ok = wait(&p_full[2 * w + h], tile) && (h > 0 || wait(&v_full[jg & 1], jg >> 1));
             if (!ok) break;
             tc_fence_after();
-            scores(w, jg + 1);
-            if (w == tiles_w - 1) p4_commit(&k_empty[(jg + 1) & 1]);
+            const float2 f = *reinterpret_cast<const float2 *>(&chunk_factor[jg & 3][2 * h]);
+            const uint32_t ids[2] = {f.x > 0.f ? idesc_o16 : idesc_o, f.y > 0.f ? idesc_o16 : idesc_o};
+#pragma unroll
+            for (int k = 0; k < kP4Keys / 32; ++k)
+              p4_mma_ts(o_at, s_at + h * 64 + k * 8, vd + (((h * 4 + k) * 2048) >> 4), ids[k >> 1],
+                        (j > 0 || h > 0 || k > 0) ? 1u : 0u);
+            p4_commit(&pv_done[w]);
+            if (h) p4_commit(&v_empty[jg & 1]);
+            if (h && !next) p4_commit(&o_full[w]);
+            if (next) {
+              if (h == 0) ok = wait(&k_full[(jg + 1) & 1], (jg + 1) >> 1);
+              if (!ok) break;
+              tc_fence_after();
+              scores(jg + 1, h);
+              if (h) p4_commit(&k_empty[(jg + 1) & 1]);
+            }
           }
         }
+        ++items;
       }
-      ++items;
-      if (tiles_w == 2) ++items1;
-    }
     }
   }
 

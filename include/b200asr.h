@@ -555,12 +555,17 @@ B200ASR_API int b200asr_qk_norm_mrope_store(
  * the projections of models/qwen3.py:20-69. lora_a bf16 [num_adapters, rank, k], lora_b bf16
  * [num_adapters, n, rank], both contiguous; scales fp32; row_adapter int32; rank a multiple
  * of 8, at most 128 (smaller adapters are padded with zeros). x rows 16-byte aligned.
+ * lora_rows: y bf16 [rows, n], both products in one fp32 accumulator and one rounding; k and n
+ *   multiples of 8. Up to 64 rows (k a multiple of 64, n of 128) it is lora_down and
+ *   linear_small_lora, which needs 4 * rows * rank bytes of workspace; beyond, t is rounded to
+ *   bf16 and the workspace is b200asr_lora_rows_workspace_size bytes (enough for both). It is
+ *   16-byte aligned, needs no initial value, keeps nothing between calls and serves one call at
+ *   a time. A value of lora_b that is not finite reaches only the rows of its own adapter.
  * lora_down: t fp32 [rows, rank] = scales[a] x A_a^T; rows without an adapter are not written.
  * linear_small_lora: linear_small (no SiLU) whose epilogue adds t B_a^T before the one
- *   rounding to bf16, from lora_down's t; m <= 64.
- * lora_rows: y bf16 [rows, n], both products in one accumulator, t rounded to bf16; k and n
- *   multiples of 8. The workspace (b200asr_lora_rows_workspace_size bytes, 16-byte aligned)
- *   needs no initial value, keeps nothing between calls and serves one call at a time. */
+ *   rounding to bf16, from lora_down's t, on the same stream after it; m <= 64. It is always
+ *   a dependent launch that reads w while lora_down still runs: with PDL on, the contract of
+ *   b200asr_set_pdl holds for w. */
 B200ASR_API int b200asr_lora_down(const void *x, int64_t x_row_stride, int32_t rows, int32_t k,
                                   const void *lora_a, int32_t num_adapters, int32_t rank,
                                   const float *scales, const int32_t *row_adapter, float *t,

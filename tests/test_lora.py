@@ -79,6 +79,20 @@ def test_no_adapter_one_adapter_and_runs(kx, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [512, 513, 700])
+@pytest.mark.parametrize("k,n,rank,adapters", [(1024, 256, 16, 8), (320, 136, 64, 40), (72, 40, 24, 5), (264, 128, 128, 2)])
+def test_many_rows_against_64_bits(kx, rows, k, n, rank, adapters):
+    """The down product that streams 32 rows of x: runs of rows, and every row another adapter."""
+    args = inputs(rows, k, n, rank, adapters, rows + 1)
+    rng = np.random.default_rng(rows)
+    for ids in (np.sort(rng.integers(-1, adapters, rows)), rng.integers(-1, adapters, rows), np.full(rows, -1)):
+        ids = torch.from_numpy(ids.astype(np.int32)).cuda()
+        wide = torch.full((rows, args[0].shape[1] + 8), float("nan"), dtype=BF16, device="cuda")
+        wide[:, :args[0].shape[1]] = args[0]
+        check(kx.lora_linear(wide[:, :args[0].shape[1]], *args[1:], ids), plain(*args, ids))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [9, 90])
 def test_strided_rows_given_out_and_nan_of_other_adapters(kx, rows):
     x, w, a, b, s = inputs(rows, 256, 128, 16, 4, 7)
@@ -97,7 +111,7 @@ def test_strided_rows_given_out_and_nan_of_other_adapters(kx, rows):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [40, 300])
+@pytest.mark.parametrize("rows", [40, 300, 600])
 def test_values_that_are_not_finite_in_b_reach_their_adapter_alone(kx, rows):
     """Rows of several adapters share a tile of the product: 0 * inf must not join them."""
     x, w, a, b, s = inputs(rows, 128, 256, 16, 4, 9)

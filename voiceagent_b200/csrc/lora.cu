@@ -4,7 +4,10 @@
 //
 // lora_down   rows of a decode step: t = s_a x A_a^T in 32 bits, which the projection's own
 //             epilogue expands (linear.cu, b200asr_linear_small_lora).
-// lora_rows   any number of rows: t as bf16, then x W^T and t B^T in one accumulator.
+// lora_rows   any number of rows: decode batches by the two launches above; beyond, t as bf16, then
+//             x W^T and t B^T in one accumulator.
+// K = 2048, N = 4096: 64 rows with 48 adapters of rank 64 20 us, 7829 rows with 16 of rank 32
+// 118-139 us as the power limit lets it (x W^T alone 98-100 us, 1.34 PFLOP/s).
 #include <type_traits>
 
 #include "common.cuh"
@@ -26,75 +29,8 @@ __device__ __forceinline__ uint4 load_now(const __nv_bfloat16 *p) {
   return v;
 }
 
-// ------------------------------------------------------------------ down, few rows
-// One warp per (row, 4 ranks): every lane holds 8 consecutive k of x and of the four rows of A,
-// 16-byte loads all independent of each other. At decode sizes this is latency: enough warps
-// that each streams a few KB, no shared memory, no second pass.
-constexpr int kLdRanks = 4;
-
-__global__ void __launch_bounds__(128) lora_down_kernel(
-    const __nv_bfloat16 *__restrict__ x, int64_t x_stride, int rows, int k,
-    const __nv_bfloat16 *__restrict__ a, int num_adapters, int rank, const float *__restrict__ scales,
-    const int32_t *__restrict__ row_adapter, float *__restrict__ t, int32_t *error_flag) {
-  pdl_trigger();
-  pdl_wait();
-  const int per_row = rank / kLdRanks;
-  const int w = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int row = w / per_row, r0 = (w - row * per_row) * kLdRanks;
-  if (row >= rows) return;
-  const int ad = row_adapter_of(row_adapter, row, num_adapters, lane == 0 ? error_flag : nullptr);
-  if (ad < 0) return;  // the expansion does not read this row
-  const __nv_bfloat16 *xr = x + row * x_stride;
-  const __nv_bfloat16 *ar = a + (static_cast<int64_t>(ad) * rank + r0) * k;
-  float acc[kLdRanks] = {0.f, 0.f, 0.f, 0.f};
-  constexpr int AHEAD = 4;  // blocks of 256 k on their way at a time
-  for (int i0 = lane * 8; i0 < k; i0 += AHEAD * 256) {
-    uint4 xu[AHEAD], au[AHEAD][kLdRanks];
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) {  // (past the end of K: the last 8 again, not used)
-      const int i = min(i0 + s * 256, k - 8);
-      xu[s] = load_now(xr + i);
-#pragma unroll
-      for (int r = 0; r < kLdRanks; ++r) au[s][r] = load_now(ar + static_cast<int64_t>(r) * k + i);
-    }
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) {
-      if (i0 + s * 256 >= k) break;
-      float xv[8], av[8];
-      unpack8(xu[s], xv);
-#pragma unroll
-      for (int r = 0; r < kLdRanks; ++r) {
-        unpack8(au[s][r], av);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[r] = fmaf(xv[e], av[e], acc[r]);
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < kLdRanks; ++r) acc[r] = warp_sum(acc[r]);
-  if (lane == 0) {
-    const float s = scales[ad];
-    *reinterpret_cast<float4 *>(t + static_cast<int64_t>(row) * rank + r0) =
-        make_float4(acc[0] * s, acc[1] * s, acc[2] * s, acc[3] * s);
-  }
-}
-
-// ------------------------------------------------------------------ down, any rows
-// A CTA takes 32 rows of x and streams them once, with the rows of A they need, through a ring of
-// TMA stages of 64 k (128-byte swizzle, so that ldmatrix meets no bank twice); mma m16n8k16 by four
-// warps, the fifth loads. What the rows need is a list of rank tiles of 8, adapter after adapter:
-// eight of them go through a pass, so that a prefill batch's tile, which has one or two adapters, is
-// one pass at ranks up to 32. A stage's products take ~250 cycles, so loads by the same warps (six
-// cp.async and their addresses a thread, ~600 cycles a stage) took 12 us a pass of K = 2048. t is
-// rounded to bf16 once, as activations between projections are: it is the operand of the second
-// product. The last CTAs of the launch list each 256-row tile's distinct adapters for that product.
-constexpr int kLtRows = 32;
-constexpr int kLtBK = 64, kLtTiles = 8;  // k of a stage, rank tiles of a pass
-constexpr int kLtStages = 8;
-constexpr int kLtThreads = 160;
-constexpr int kLtStage = (kLtRows + 8 * kLtTiles) * kLtBK * 2;
-constexpr int kLtSmem = 1024 + kLtStages * kLtStage + 256;
 constexpr int kLoraMaxRank = 128;
+constexpr int kLoraSmallRows = 64;      // linear_small_lora's; must match LINEAR_SMALL_MAX_ROWS in kernels.py
 constexpr int kLgTile = 256;            // rows and columns of a CTA pair's tile
 constexpr int kLgPlan = 1 + kLgTile;    // plan entry of a row tile: count, adapters
 
@@ -105,34 +41,10 @@ struct LoraDownArgs {
   const __nv_bfloat16 *a;
   const float *scales;
   const int32_t *row_adapter;
-  __nv_bfloat16 *t;   // [rows, rank]
-  int32_t *plan;      // [row tiles][kLgPlan]
+  void *t;            // [rows, rank], fp32 (lora_down) or bf16 (lora_rows)
+  int32_t *plan;      // [row tiles][kLgPlan], lora_rows alone
   int32_t *error_flag;
 };
-
-__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t a0, const uint32_t a1,
-                                               const uint32_t a2, const uint32_t a3,
-                                               const uint32_t b0, const uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void lt_load_2d(void *dst, const CUtensorMap *map, int c0, int c1, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_addr(bar))
-      : "memory");
-}
-__device__ __forceinline__ void lt_ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
 
 // Distinct adapters of rows [256 tile, +256), in the order of their first rows (one warp).
 __device__ __forceinline__ void lora_plan(const LoraDownArgs &p, int tile) {
@@ -160,6 +72,114 @@ __device__ __forceinline__ void lora_plan(const LoraDownArgs &p, int tile) {
   int32_t *out = p.plan + static_cast<int64_t>(tile) * kLgPlan;
   for (int j = lane; j < count; j += 32) out[1 + j] = list[j];
   if (lane == 0) out[0] = count;
+}
+
+// ------------------------------------------------------------------ down, few rows
+// One warp per (row, 4 ranks): every lane holds 8 consecutive k of x and of the four rows of A,
+// 16-byte loads all independent of each other. At decode sizes this is latency: enough warps
+// that each streams a few KB, no shared memory, no second pass.
+constexpr int kLdRanks = 4;
+// Rows up to which lora_rows uses it too. lora_rows in all, K = 2048, N = 4096, this kernel / the
+// one below, us, rank 64: 65 rows of one adapter 20 / 17, of two 20 / 27, each row the next of 48
+// adapters 67 / 361; 512 rows 29 / 19, 30 / 29, 80 / 371; 2048 rows 69 / 41, 69 / 42, 178 / 439.
+// Rank 16, 8 adapters: 512 rows 22 / 19, 22 / 22, 28 / 54.
+constexpr int kLdMostRows = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(128) lora_down_kernel(const LoraDownArgs p) {
+  constexpr bool ROWS = sizeof(T) == 2;  // for lora_rows, whose product reads x before its own wait
+  if (!ROWS) pdl_trigger();
+  pdl_wait();
+  if (ROWS) pdl_trigger();
+  const int per_row = p.rank / kLdRanks, k = p.k;
+  if (ROWS) {  // the last CTAs
+    const int first = (p.rows * per_row + 3) / 4;
+    if (static_cast<int>(blockIdx.x) >= first) {
+      lora_plan(p, blockIdx.x - first);
+      return;
+    }
+  }
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = w / per_row, r0 = (w - row * per_row) * kLdRanks;
+  if (row >= p.rows) return;
+  const int ad = row_adapter_of(p.row_adapter, row, p.num_adapters, lane == 0 ? p.error_flag : nullptr);
+  if (ad < 0) return;  // the expansion does not read this row
+  const __nv_bfloat16 *xr = p.x + row * p.x_stride;
+  const __nv_bfloat16 *ar = p.a + (static_cast<int64_t>(ad) * p.rank + r0) * k;
+  float acc[kLdRanks] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int AHEAD = 4;  // blocks of 256 k on their way at a time
+  for (int i0 = lane * 8; i0 < k; i0 += AHEAD * 256) {
+    uint4 xu[AHEAD], au[AHEAD][kLdRanks];
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {  // (past the end of K: the last 8 again, not used)
+      const int i = min(i0 + s * 256, k - 8);
+      xu[s] = load_now(xr + i);
+#pragma unroll
+      for (int r = 0; r < kLdRanks; ++r) au[s][r] = load_now(ar + static_cast<int64_t>(r) * k + i);
+    }
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      if (i0 + s * 256 >= k) break;
+      float xv[8], av[8];
+      unpack8(xu[s], xv);
+#pragma unroll
+      for (int r = 0; r < kLdRanks; ++r) {
+        unpack8(au[s][r], av);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[r] = fmaf(xv[e], av[e], acc[r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kLdRanks; ++r) acc[r] = warp_sum(acc[r]);
+  if (lane == 0) {
+    const float s = p.scales[ad];
+    T *t = static_cast<T *>(p.t) + static_cast<int64_t>(row) * p.rank + r0;
+    if constexpr (ROWS)
+      *reinterpret_cast<uint2 *>(t) = make_uint2(pack2(acc[0] * s, acc[1] * s), pack2(acc[2] * s, acc[3] * s));
+    else
+      *reinterpret_cast<float4 *>(t) = make_float4(acc[0] * s, acc[1] * s, acc[2] * s, acc[3] * s);
+  }
+}
+
+// ------------------------------------------------------------------ down, many rows
+// A CTA takes 32 rows of x and streams them once, with the rows of A they need, through a ring of
+// TMA stages of 64 k (128-byte swizzle, so that ldmatrix meets no bank twice); mma m16n8k16 by four
+// warps, the fifth loads. What the rows need is a list of rank tiles of 8, adapter after adapter:
+// eight of them go through a pass, so that a prefill batch's tile, which has one or two adapters, is
+// one pass at ranks up to 32. A stage's products take ~250 cycles, so loads by the same warps (six
+// cp.async and their addresses a thread, ~600 cycles a stage) took 12 us a pass of K = 2048. t is
+// rounded to bf16 once, as activations between projections are: it is the operand of the second
+// product. The last CTAs of the launch list each 256-row tile's distinct adapters for that product.
+constexpr int kLtRows = 32;
+constexpr int kLtBK = 64, kLtTiles = 8;  // k of a stage, rank tiles of a pass
+constexpr int kLtStages = 8;
+constexpr int kLtThreads = 160;
+constexpr int kLtStage = (kLtRows + 8 * kLtTiles) * kLtBK * 2;
+constexpr int kLtSmem = 1024 + kLtStages * kLtStage + 256;
+
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t a0, const uint32_t a1,
+                                               const uint32_t a2, const uint32_t a3,
+                                               const uint32_t b0, const uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void lt_load_2d(void *dst, const CUtensorMap *map, int c0, int c1, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void lt_ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
 // Rank tiles a copy of A brings: the more the fewer copies; a whole number of them makes an adapter
@@ -281,7 +301,7 @@ __global__ void __launch_bounds__(kLtThreads) lora_down_rows_kernel(const __grid
         for (int h = 0; h < 2; ++h) {
           const int r = m * 16 + h * 8 + g;
           if (__shfl_sync(0xffffffffu, mine, r) == ad && tile < first + used)
-            *reinterpret_cast<uint32_t *>(p.t + static_cast<int64_t>(row0 + r) * p.rank + (tile - at * per) * 8 + 2 * q) =
+            *reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(p.t) + static_cast<int64_t>(row0 + r) * p.rank + (tile - at * per) * 8 + 2 * q) =
                 pack2(acc[i][j][2 * h] * sc, acc[i][j][2 * h + 1] * sc);
         }
       }
@@ -671,11 +691,21 @@ extern "C" int b200asr_lora_down(const void *x, int64_t x_row_stride, int32_t ro
                "lora_down: rows must be 16-byte aligned");
   const int64_t warps = static_cast<int64_t>(rows) * (rank / kLdRanks);
   B200_REQUIRE(warps <= 0x7fffffff, "lora_down: too many rows");
+  LoraDownArgs p{};
+  p.x = static_cast<const __nv_bfloat16 *>(x);
+  p.x_stride = x_row_stride;
+  p.rows = rows;
+  p.k = k;
+  p.rank = rank;
+  p.num_adapters = num_adapters;
+  p.a = static_cast<const __nv_bfloat16 *>(lora_a);
+  p.scales = scales;
+  p.row_adapter = row_adapter;
+  p.t = t;
+  p.error_flag = error_flag;
   B200_LAUNCH_CHECK_ERR(
-      launch_kernel(lora_down_kernel, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, stream,
-                    true, 1, static_cast<const __nv_bfloat16 *>(x), x_row_stride, static_cast<int>(rows),
-                    static_cast<int>(k), static_cast<const __nv_bfloat16 *>(lora_a),
-                    static_cast<int>(num_adapters), static_cast<int>(rank), scales, row_adapter, t, error_flag),
+      launch_kernel(lora_down_kernel<float>, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0,
+                    static_cast<cudaStream_t>(stream), true, 1, p),
       "lora_down");
   return B200ASR_OK;
 }
@@ -683,7 +713,8 @@ extern "C" int b200asr_lora_down(const void *x, int64_t x_row_stride, int32_t ro
 extern "C" size_t b200asr_lora_rows_workspace_size(int32_t rows, int32_t rank) {
   if (rows < 0 || rank < 0) return 0;
   const size_t tiles = (static_cast<size_t>(rows) + kLgTile - 1) / kLgTile;
-  return (static_cast<size_t>(rows) * rank * 2 + 15) / 16 * 16 + tiles * kLgPlan * 4;
+  const size_t many = (static_cast<size_t>(rows) * rank * 2 + 15) / 16 * 16 + tiles * kLgPlan * 4;
+  return rows <= kLoraSmallRows ? std::max(many, static_cast<size_t>(rows) * rank * 4) : many;
 }
 
 extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t rows, int32_t k,
@@ -700,10 +731,20 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
   B200_REQUIRE(aligned16(x) && x_row_stride >= k && x_row_stride % 8 == 0 && aligned16(w) && aligned16(lora_a) &&
                    aligned16(lora_b) && aligned16(y) && y_row_stride % 8 == 0 && aligned16(workspace),
                "lora_rows: rows must be 16-byte aligned");
-  const size_t need = b200asr_lora_rows_workspace_size(rows, rank);
+  B200_REQUIRE(y_row_stride >= n, "lora_rows: rows of y overlap");
+  const bool small = rows <= kLoraSmallRows && k % 64 == 0 && n % 128 == 0;
+  const size_t need = small ? static_cast<size_t>(rows) * rank * 4 : b200asr_lora_rows_workspace_size(rows, rank);
   if (workspace_bytes < need) {
     set_error("lora_rows: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return B200ASR_ERR_WORKSPACE;
+  }
+  if (small) {
+    float *t = static_cast<float *>(workspace);
+    const int down = b200asr_lora_down(x, x_row_stride, rows, k, lora_a, num_adapters, rank, scales, row_adapter, t,
+                                       error_flag, stream);
+    return down != B200ASR_OK ? down
+                              : b200asr_linear_small_lora(x, x_row_stride, rows, k, w, n, t, lora_b, num_adapters,
+                                                          rank, row_adapter, y, y_row_stride, error_flag, stream);
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LoraGemmArgs g{};
@@ -730,11 +771,11 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
   p.a = static_cast<const __nv_bfloat16 *>(lora_a);
   p.scales = scales;
   p.row_adapter = row_adapter;
-  p.t = static_cast<__nv_bfloat16 *>(workspace);
+  p.t = workspace;
   p.plan = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(workspace) +
                                        (static_cast<size_t>(rows) * rank * 2 + 15) / 16 * 16);
   p.error_flag = error_flag;
-  g.t = p.t;
+  g.t = static_cast<const __nv_bfloat16 *>(workspace);
   g.plan = p.plan;
   g.row_adapter = row_adapter;
   g.y = static_cast<__nv_bfloat16 *>(y);
@@ -754,19 +795,26 @@ extern "C" int b200asr_lora_rows(const void *x, int64_t x_row_stride, int32_t ro
   B200_LAUNCH_CHECK_ERR(
       cudaFuncSetAttribute(lora_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmem),
       "lora_rows (configuration)");
-  const int down = (rows + kLtRows - 1) / kLtRows;
-  CUtensorMap dx, da;
-  const uint32_t dx_box[2] = {kLtBK, kLtRows}, da_box[3] = {kLtBK, 8u * lt_box(rank), 1};
-  const uint64_t ad[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rank), static_cast<uint64_t>(num_adapters)};
-  const uint64_t as[2] = {static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(k) * rank * 2};
-  if (!make_tmap_bf16(&dx, x, 2, xd, xs, dx_box) || !make_tmap_bf16(&da, lora_a, 3, ad, as, da_box))
-    return B200ASR_ERR_CUDA;
-  B200_LAUNCH_CHECK_ERR(
-      cudaFuncSetAttribute(lora_down_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtSmem),
-      "lora_rows (configuration)");
-  B200_LAUNCH_CHECK_ERR(launch_kernel(lora_down_rows_kernel, dim3(down + g.tiles_m), dim3(kLtThreads), kLtSmem, st,
-                                      true, 1, dx, da, p),
-                        "lora_rows (down)");
+  if (rows <= kLdMostRows) {
+    const int down = (rows * (rank / kLdRanks) + 3) / 4;
+    B200_LAUNCH_CHECK_ERR(launch_kernel(lora_down_kernel<__nv_bfloat16>, dim3(down + g.tiles_m), dim3(128), 0, st,
+                                        true, 1, p),
+                          "lora_rows (down)");
+  } else {
+    const int down = (rows + kLtRows - 1) / kLtRows;
+    CUtensorMap dx, da;
+    const uint32_t dx_box[2] = {kLtBK, kLtRows}, da_box[3] = {kLtBK, 8u * lt_box(rank), 1};
+    const uint64_t ad[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rank), static_cast<uint64_t>(num_adapters)};
+    const uint64_t as[2] = {static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(k) * rank * 2};
+    if (!make_tmap_bf16(&dx, x, 2, xd, xs, dx_box) || !make_tmap_bf16(&da, lora_a, 3, ad, as, da_box))
+      return B200ASR_ERR_CUDA;
+    B200_LAUNCH_CHECK_ERR(
+        cudaFuncSetAttribute(lora_down_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtSmem),
+        "lora_rows (configuration)");
+    B200_LAUNCH_CHECK_ERR(launch_kernel(lora_down_rows_kernel, dim3(down + g.tiles_m), dim3(kLtThreads), kLtSmem, st,
+                                        true, 1, dx, da, p),
+                          "lora_rows (down)");
+  }
   const int pairs = std::min(g.tiles_m * g.tiles_n, num_sms() / 2);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * pairs);

@@ -740,23 +740,16 @@ def lora_linear(x, weight, lora_a, lora_b, scales, row_adapter, *, out=None,
     _here(what, x, weight, lora_a, lora_b, scales, row_adapter, out, error_flag)
     if m == 0:
         return out
-    err, stream = _p(error_flag), _stream()
-    _count(2)
     if m <= LINEAR_SMALL_MAX_ROWS and k % 64 == 0 and n % 128 == 0:
-        t = torch.empty(m, rank, dtype=torch.float32, device=x.device)
-        x_p, t_p, row_p = x.data_ptr(), t.data_ptr(), row_adapter.data_ptr()
-        check(lib.b200asr_lora_down(x_p, xs[0], m, k, lora_a.data_ptr(), adapters, rank,
-                                    scales.data_ptr(), row_p, t_p, err, stream), what)
-        check(lib.b200asr_linear_small_lora(x_p, xs[0], m, k, weight.data_ptr(), n, t_p,
-                                            lora_b.data_ptr(), adapters, rank, row_p, out.data_ptr(),
-                                            os[0], err, stream), what)
-        return out
-    size = lib.b200asr_lora_rows_workspace_size(m, rank)
+        size = 4 * m * rank  # t alone
+    else:
+        size = lib.b200asr_lora_rows_workspace_size(m, rank)
     workspace = torch.empty(size, dtype=_U8, device=x.device)
+    _count(2)
     check(lib.b200asr_lora_rows(x.data_ptr(), xs[0], m, k, weight.data_ptr(), n, lora_a.data_ptr(),
                                 lora_b.data_ptr(), adapters, rank, scales.data_ptr(),
                                 row_adapter.data_ptr(), out.data_ptr(), os[0], workspace.data_ptr(),
-                                size, err, stream), what)
+                                size, _p(error_flag), _stream()), what)
     return out
 
 

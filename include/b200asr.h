@@ -58,7 +58,8 @@ B200ASR_API const char *b200asr_last_error(void);
 
 /* Programmatic dependent launch (no reference counterpart; default off). When on,
  * the decode-path kernels (rmsnorm, qk_norm_rope_store, paged_decode, linear_small,
- * silu_mul, store_kvcache, greedy_argmax) are launched so that each may begin its
+ * silu_mul, store_kvcache, greedy_argmax, and those of the 4-bit cache, the rotary axes
+ * and the adapters below) are launched so that each may begin its
  * prologue -- shared-memory and TMEM set-up, tensor-map and weight loads -- while the
  * previous kernel in the stream finishes; each waits for that kernel's results before
  * reading them or writing global memory. A CUDA graph captured with it on keeps the
@@ -483,7 +484,8 @@ typedef struct {
 
 /* key/value bf16 [num_tokens, num_kv_heads, D] (token and head strides in elements,
  * multiples of 8) quantised into their slots; slot -1 is skipped (store_kvcache,
- * layers/attention.py:52-67). No slot may occur twice. Rows of other slots are untouched. */
+ * layers/attention.py:52-67). No slot may occur twice (which of the rows it would keep is not
+ * defined). Rows of other slots are untouched. */
 B200ASR_API int b200asr_store_kvcache4(const void *key, int64_t key_token_stride,
                                        int64_t key_head_stride, const void *value,
                                        int64_t value_token_stride, int64_t value_head_stride,
@@ -521,7 +523,8 @@ B200ASR_API int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64
  * num_heads, D], rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] of sequence b attending its
  * cu_seqlens_k[b + 1] - cu_seqlens_k[b] cached tokens, causal with the mask aligned
  * bottom-right; strides, tables, flags and group sizes as for paged_decode4. A row that sees
- * no key (no cached token, or more query than cached tokens) gives zeros. */
+ * no key (no cached token, or more query than cached tokens) gives zeros; rows of q past
+ * cu_seqlens_q[batch] are not read and theirs of out are left alone. */
 B200ASR_API int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
                                        const b200asr_kv4 *cache, int32_t num_heads,
                                        const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
@@ -539,8 +542,8 @@ B200ASR_API int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int6
  * [num_tokens, num_heads, head_dim]. Everything is computed in 32 bits and rounded to bf16
  * once. With slot_mapping (-1 skips), K and V go to a contiguous bf16 cache (k_cache,
  * v_cache, num_slots; cache4 NULL) or, quantised from the bf16 K and V, to a 4-bit one
- * (cache4; k_cache and v_cache NULL). A position or an axis out of range reads as position
- * 0 (B200ASR_DEVERR_POSITION). */
+ * (cache4; k_cache and v_cache NULL); no slot may occur twice. A position or an axis out of
+ * range reads as position 0 (B200ASR_DEVERR_POSITION). */
 B200ASR_API int b200asr_qk_norm_mrope_store(
     const void *qkv, int64_t qkv_row_stride, const int64_t *positions, int64_t position_stride,
     int32_t axes, const int32_t *freq_axis, int32_t num_tokens, int32_t num_heads,

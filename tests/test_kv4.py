@@ -546,6 +546,33 @@ def test_prefill_not_finite_keys_reach_only_the_rows_that_see_them(kx):
 
 
 @pytest.mark.gpu
+def test_prefill_largest_values_reach_only_the_rows_that_see_them(kx):
+    """A V row whose top code lies past the largest bf16 is no infinity to rows behind the mask."""
+    table, blocks = paged(2, [100, 100], 16)
+    cache = filled(3, blocks, 16, 2, 128)
+    q = torch.randn(200, 4, 128, device="cuda").bfloat16()
+    call = lambda: kx.paged_prefill4(  # noqa: E731
+        q, *cache, starts([100, 100]), starts([100, 100]), table, max_seqlen_q=100, max_seqlen_k=100, scale=0.1,
+        out=torch.empty_like(q))
+    clean = call()
+    most = torch.finfo(BF16).max
+    row = cache[2][table[1, 4].long(), 6, 1]  # key 70 of the second sequence
+    row[2:] = torch.tensor([most / 15 * (1 + 2 ** -7), 0.0], device="cuda").bfloat16()
+    assert 15 * row[2].double().item() > most * (1 + 2 ** -9)
+    got = call()
+    hit = torch.zeros(200, 4, dtype=torch.bool, device="cuda")
+    hit[170:, 2:] = True
+    # rows that do not see the key, in the 32 keys whose P is now rounded to bf16 (2^-8 of values
+    # up to 15 steps past the zero): those of keys 64 to 69
+    near = torch.zeros_like(hit)
+    near[164:170, 2:] = True
+    assert torch.equal(got[~hit & ~near], clean[~hit & ~near])
+    top = (cache[2][..., 2].abs() * 15 + cache[2][..., 3].abs()).view(-1, 2)
+    top = top[top < 1e30].max().item()
+    assert (got[near].float() - clean[near].float()).abs().max().item() <= 4 * 2 ** -8 * top
+
+
+@pytest.mark.gpu
 def test_prefill_flags_and_capture(kx):
     q_lens, k_lens = [30, 40], [60, 300]
     table, blocks = paged(7, k_lens, 16)

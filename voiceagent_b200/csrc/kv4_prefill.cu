@@ -6,7 +6,7 @@
 // the group) pair, token-major, so any group size fills the tile. The rows are two tiles of
 // 128 (the MMA's M) that share every K and V tile of 128 tokens:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, thread = row = TMEM lane
-//   warps 8-11      codes to bf16: K and V tiles into shared memory, 128-byte swizzled
+//   warps 8-11      codes to values: K and V tiles into shared memory, 128-byte swizzled
 //   warps 12, 13    tcgen05.mma of tile 0 / 1 (12: TMEM)
 // What bounds it: per 128 tokens of one KV head (D = 128) the tensor cores need 2048 cycles for
 // both row tiles at their full rate, the 32768 exponentials 2048 cycles of the special-function
@@ -30,10 +30,10 @@
 //    q is laid out alike, and the output is put back in order as it is written.
 //  * Values are zero + code * scale in one rounding, and q, K, V and P go through the tensor
 //    cores as fp16, 11 bits where bf16 keeps 8 (root mean square error of the output against 64
-//    bits, relative to its own: 0.0042 with bf16, of which the output's rounding is 0.0017). q is
-//    brought to fp16's range by a power of two per row, K by one per 32 tokens, both undone in the factor of the
-//    scores. V carries no such factor, so 32 tokens whose V rows do not lie within
-//    [2^-10, 2^15] (or are zero) go through as bf16, with their P.
+//    bits, relative: 0.0042 with bf16, 0.0017 so, which is the output's own rounding). q is
+//    brought to fp16's range by a power of two per row, K by one per 32 tokens, both undone in
+//    the factor of the scores. V carries no such factor, so 32 tokens whose V rows do not lie
+//    within [2^-10, 2^15] (or are zero) go through as bf16, with their P.
 //  * A V row that is not finite is written as zeros and its K row as NaN: the rows that may
 //    attend it become NaN, those that may not keep their values (0 * NaN would reach them).
 #include <cuda_fp16.h>

@@ -524,14 +524,21 @@ B200ASR_API int b200asr_paged_decode4(const void *q, int64_t q_row_stride, int64
  * cu_seqlens_k[b + 1] - cu_seqlens_k[b] cached tokens, causal with the mask aligned
  * bottom-right; strides, tables, flags and group sizes as for paged_decode4. A row that sees
  * no key (no cached token, or more query than cached tokens) gives zeros; rows of q past
- * cu_seqlens_q[batch] are not read and theirs of out are left alone. */
+ * cu_seqlens_q[batch] are not read and theirs of out are left alone. With a workspace (16-byte
+ * aligned, no initial value, nothing kept, one call at a time) long contexts of few rows are
+ * split over CTAs; b200asr_paged_prefill4_workspace_size gives 0 where that cannot help, and
+ * with NULL or fewer bytes contexts are split less or not at all. */
+B200ASR_API size_t b200asr_paged_prefill4_workspace_size(int32_t total_q, int32_t batch,
+                                                         int32_t max_seqlen_k, int32_t num_heads,
+                                                         int32_t num_kv_heads, int32_t head_dim);
 B200ASR_API int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
                                        const b200asr_kv4 *cache, int32_t num_heads,
                                        const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
                                        const int32_t *block_tables, int64_t bt_stride,
                                        int32_t bt_width, int32_t batch, int32_t total_q,
                                        float scale, void *out, int64_t out_row_stride,
-                                       int64_t out_head_stride, int32_t *error_flag,
+                                       int64_t out_head_stride, void *workspace,
+                                       size_t workspace_bytes, int32_t *error_flag,
                                        b200asr_stream_t stream);
 
 /* ------------------------------------------- rotary positions with several axes ----

@@ -219,7 +219,10 @@ def test_c_entries_refuse_bad_calls():
     assert dec(batch=0) == 0
     pre = lambda **k: lib.b200asr_paged_prefill4(  # noqa: E731
         p, 2048, 128, c, k.get("heads", 16), p, p, p, 4, 4, k.get("batch", 2), k.get("rows", 9), 1.0, p,
-        k.get("os", 2048), 128, None, None)
+        k.get("os", 2048), 128, k.get("ws"), 1 << 20, None, None)
+    assert pre(ws=ctypes.c_void_p(264)) == 1 and "workspace" in err()
+    size = lib.b200asr_paged_prefill4_workspace_size
+    assert size(200, 1, 1024, 16, 8, 128) == size(0, 1, 5000, 16, 8, 128) == size(10**6, 1, 5000, 16, 8, 128) == 0
     assert pre(heads=12) == 1 and "multiple" in err()
     assert pre(os=2044) == 1 and "aligned" in err()
     assert pre(rows=-1) == 1 and "sizes" in err()
@@ -475,6 +478,51 @@ def test_prefill_against_64_bits(kx, heads, hkv, d, bs, layout):
     ([200], [200]), ([128], [128]), ([129], [1000]), ([1], [0]), ([3, 4], [0, 2]), ([300, 7], [290, 3]), ([1], [2500])])
 def test_prefill_lengths(kx, q_lens, k_lens):
     check_prefill(kx, q_lens, k_lens, 4, 2, 128, 16, seed=4)
+
+
+SPLIT = [([200], [5000]), ([1, 300, 0, 17, 4], [4000, 1300, 2000, 0, 3]), ([40, 40, 40, 1], [3000, 1500, 1025, 9]),
+         ([500, 3], [1400, 5]), ([600], [100])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,k_lens", SPLIT)
+@pytest.mark.parametrize("heads,hkv,d,bs", [(4, 2, 128, 256), (7, 1, 64, 16)])
+def test_prefill_contexts_split_over_ctas(kx, q_lens, k_lens, heads, hkv, d, bs):
+    assert kx.paged_prefill4_workspace_size(sum(q_lens) + 3, len(q_lens), max(max(k_lens), 1025), heads, hkv, d) > 0
+    check_prefill(kx, q_lens, k_lens, heads, hkv, d, bs)
+
+
+@pytest.mark.gpu
+def test_prefill_split_any_workspace_the_same_every_time_and_under_capture(kx):
+    q_lens, k_lens = SPLIT[1]
+    table, blocks = paged(3, k_lens, 32)
+    cache = filled(4, blocks, 32, 2, 128)
+    poison_unused(cache, table, k_lens)
+    q = torch.randn(sum(q_lens), 8, 128, device="cuda").bfloat16()
+    slot = 256 * 132 * 4
+
+    def call(ws, out=None):
+        return kx.paged_prefill4(q, *cache, starts(q_lens), starts(k_lens), table, max_seqlen_q=300, max_seqlen_k=4000,
+                                 scale=0.09, out=torch.empty_like(q) if out is None else out, workspace=ws)
+
+    want = call(None)
+    for slots in (0, 1, 2, 9, 50, 400):  # split less, or not at all
+        ws = torch.full((slots * slot + 16,), 255, dtype=torch.uint8, device="cuda")  # (NaN)
+        got = call(ws)
+        assert torch.equal(got, call(ws))
+        at = 0
+        for b, (m, n) in enumerate(zip(q_lens, k_lens)):
+            check_close(got[at:at + m], *plain_attention(q[at:at + m], cache, table[b], n, 0.09, prefill=True),
+                        f"{slots} slots, sequence {b}")
+            at += m
+    cq, ck, out = starts(q_lens), starts(k_lens), torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kx.paged_prefill4(q, *cache, cq, ck, table, max_seqlen_q=300, max_seqlen_k=4000, scale=0.09, out=out)
+    for _ in range(2):
+        out.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, want)
 
 
 @pytest.mark.gpu

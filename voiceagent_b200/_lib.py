@@ -106,7 +106,10 @@ SIGNATURES: dict[str, tuple] = {
     "b200asr_lora_rows": (c_int32, [P, c_int64, c_int32, c_int32, P, c_int32, P, P, c_int32, c_int32,
                                     P, P, P, c_int64, P, c_size_t, P, P]),
     "b200asr_paged_prefill4": (c_int32, [P, c_int64, c_int64, P, c_int32, P, P, P, c_int64, c_int32,
-                                         c_int32, c_int32, c_float, P, c_int64, c_int64, P, P]),
+                                         c_int32, c_int32, c_float, P, c_int64, c_int64, P,
+                                         c_size_t, P, P]),
+    "b200asr_paged_prefill4_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32,
+                                                         c_int32]),
 }
 
 

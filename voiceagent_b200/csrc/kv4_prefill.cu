@@ -59,6 +59,8 @@ struct Prefill4Args {
   uint32_t flip;     // sign bit to exchange in q
   __nv_bfloat16 *out;
   int64_t out_row, out_head;
+  float *ws;      // partials of split contexts: [slots][256 rows][D + 4] (maximum, sum, -, -, O), or null
+  int max_slots, ctas;
   int32_t *error_flag;
 };
 
@@ -73,7 +75,8 @@ struct Pre4 {
 // One sequence's part of the item list, and where an item lies.
 struct Item4 {
   int b, h, rows, row0;  // rows of this item, the first one's index in the sequence
-  int q0, offset, n_kv, tiles;
+  int q0, offset, n_kv, t0, tiles;  // keys in all; first K/V tile of this part of them, and its tiles
+  int slot;  // where a part of a split context leaves its partials; -1: not split
   bool cut;  // the table row is too short for the sequence
 };
 
@@ -82,14 +85,91 @@ struct Item4 {
 // rows first -- and is dealt back and forth, c, 2 G - 1 - c, 2 G + c, ... to CTA c of G: with 496
 // items of 2 to 64 tiles the fullest CTA has 148 tiles, 172 when dealt in order, 135 on average.
 // Every warp walks alone and sees the same items.
-constexpr int kP4Sorted = 256;  // sequences up to which they are sorted
-struct Walk4 {
-  // query tokens of a sequence, held to the rows that q has
-  static __device__ __forceinline__ int q_len_of(const Prefill4Args &a, int b) {
-    return max(0, min(a.cu_q[b + 1], a.total_q) - max(0, a.cu_q[b]));
+// Where that leaves SMs idle, contexts are split into parts of about `seg_tiles` K/V tiles, every
+// row tile of a sequence into as many, whose partials a second kernel joins in order: 200 tokens of
+// 16 query heads on 8 behind a cached prefix of 8k tokens 54 us, 183 unsplit.
+constexpr int kP4Sorted = 256;   // sequences up to which they are sorted, and split
+constexpr int kP4MinSeg = 4;     // K/V tiles of a part, at least
+// K/V tiles that the longest context gets shorter by, at least: a part's first loads, its partials
+// and the join cost about as much (two requests of 400 rows on 1400 and 778 keys, 6 fewer: 58 us
+// split, 44 not; one of 200 on 2200, 14 fewer: 38 and 60).
+constexpr int kP4MinSaved = 8;
+struct Plan4 {
+  int lens[kP4Sorted];
+  uint16_t order[kP4Sorted];  // sequences by falling length
+  unsigned long long sum[3];
+  int seg_tiles;
+};
+
+// query tokens of a sequence, held to the rows that q has
+__device__ __forceinline__ int p4_q_len(const Prefill4Args &a, int b) {
+  return max(0, min(a.cu_q[b + 1], a.total_q) - max(0, a.cu_q[b]));
+}
+__device__ __forceinline__ int p4_row_tiles(const Prefill4Args &a, int b) {
+  return (p4_q_len(a, b) * a.group + kP4Rows - 1) / kP4Rows;
+}
+__device__ __forceinline__ int p4_room(const Prefill4Args &a) {
+  return static_cast<int>(min(static_cast<int64_t>(0x7fffffff), static_cast<int64_t>(a.bt_width) * a.c.block_size));
+}
+// Parts of a sequence's contexts: by the K/V tiles of its last row.
+__device__ __forceinline__ int p4_segs(const Prefill4Args &a, int b, int seg_tiles) {
+  if (seg_tiles == kP4Whole) return 1;
+  const int keys = min(max(0, a.cu_k[b + 1] - a.cu_k[b]), p4_room(a));
+  return max(1, ((keys + kP4Keys - 1) / kP4Keys + seg_tiles - 1) / seg_tiles);
+}
+
+// The order of the sequences, and how long the parts of split contexts are: an even share of all
+// K/V tiles, or as much longer as it takes for every CTA to have one part at most and for the
+// partials to fit. The same in every CTA and in the join.
+__device__ __forceinline__ void p4_plan(const Prefill4Args &a, Plan4 &plan) {
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    plan.seg_tiles = kP4Whole;
+    plan.sum[0] = plan.sum[1] = plan.sum[2] = 0;
   }
-  int i, scan, carry;      // turn of the CTA; the sequences before `scan` hold `carry` row tiles
-  const uint16_t *order;   // sequences by falling length, or null
+  if (a.batch <= kP4Sorted) {
+    for (int b = tid; b < a.batch; b += blockDim.x) plan.lens[b] = a.cu_k[b + 1] - a.cu_k[b];
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += blockDim.x) {
+      const int len = plan.lens[b];
+      int rank = 0;
+      for (int o = 0; o < a.batch; ++o) rank += plan.lens[o] > len || (plan.lens[o] == len && o < b);
+      plan.order[rank] = static_cast<uint16_t>(b);
+      if (a.ws != nullptr)
+        atomicAdd(&plan.sum[0], static_cast<unsigned long long>(p4_row_tiles(a, b)) * p4_segs(a, b, 1));
+    }
+    __syncthreads();
+    if (a.ws != nullptr) {
+      int seg = static_cast<int>(min(static_cast<unsigned long long>(1 << 29),
+                                     (plan.sum[0] * a.c.num_kv_heads + a.ctas - 1) / a.ctas));
+      seg = max(seg, kP4MinSeg);
+      while (true) {  // ends: a part as long as the longest context splits nothing
+        for (int b = tid; b < a.batch; b += blockDim.x) {
+          const int n = p4_segs(a, b, seg), tiles = p4_row_tiles(a, b);
+          if (n > 1) atomicAdd(&plan.sum[1], static_cast<unsigned long long>(tiles) * n);
+          else atomicAdd(&plan.sum[2], static_cast<unsigned long long>(tiles));
+        }
+        __syncthreads();
+        const unsigned long long parts = plan.sum[1] * a.c.num_kv_heads, whole = plan.sum[2] * a.c.num_kv_heads;
+        __syncthreads();
+        if (tid == 0) plan.sum[1] = plan.sum[2] = 0;
+        if (parts == 0 || (parts <= static_cast<unsigned long long>(a.max_slots) &&
+                           parts + whole <= static_cast<unsigned long long>(a.ctas)))
+          break;
+        seg += seg / 8 + 1;
+        __syncthreads();
+      }
+      if (tid == 0 && p4_segs(a, plan.order[0], 1) - seg >= kP4MinSaved) plan.seg_tiles = seg;
+    }
+  }
+  __syncthreads();
+}
+
+template <bool SPLIT>
+struct Walk4 {
+  int i, scan, carry, split;  // turn of the CTA; the sequences before `scan` hold `carry` units, `split` of them parts
+  const uint16_t *order;      // sequences by falling length, or null
+  int seg_tiles;
   __device__ __forceinline__ bool next(const Prefill4Args &a, Item4 &it) {
     const int lane = threadIdx.x & 31, heads = a.c.num_kv_heads;
     while (true) {
@@ -97,38 +177,60 @@ struct Walk4 {
       const int t = item / heads;
       it.h = item - t * heads;
       ++i;
+      int seg = 0, segs = 1;
       while (true) {
         if (scan >= a.batch) return false;
         const int bb = scan + lane < a.batch ? order ? order[scan + lane] : scan + lane : a.batch;
-        const int n = bb < a.batch ? (q_len_of(a, bb) * a.group + kP4Rows - 1) / kP4Rows : 0;
-        int incl = n;
+        const int tiles = bb < a.batch ? p4_row_tiles(a, bb) : 0;
+        const int parts = SPLIT && bb < a.batch ? p4_segs(a, bb, seg_tiles) : 1;
+        const int n = tiles * parts;
+        int incl = n, incl2 = parts > 1 ? n : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int y = __shfl_up_sync(0xffffffffu, incl, o);
           if (lane >= o) incl += y;
+          if constexpr (SPLIT) {
+            const int z = __shfl_up_sync(0xffffffffu, incl2, o);
+            if (lane >= o) incl2 += z;
+          }
         }
         const unsigned here = __ballot_sync(0xffffffffu, t < carry + incl);
         if (here) {
           const int src = __ffs(here) - 1;
           it.b = __shfl_sync(0xffffffffu, bb, src);
-          // the sequence's row tiles from the last to the first
-          it.row0 = (carry + __shfl_sync(0xffffffffu, incl, src) - 1 - t) * kP4Rows;
+          // the sequence's row tiles from the last to the first, each in parts
+          const int u = t - carry - __shfl_sync(0xffffffffu, incl - n, src);
+          int back = u;
+          it.slot = -1;
+          if constexpr (SPLIT) {
+            segs = __shfl_sync(0xffffffffu, parts, src);
+            back = u / segs;
+            seg = u - back * segs;
+            if (segs > 1) it.slot = (split + __shfl_sync(0xffffffffu, incl2 - n, src) + u) * heads + it.h;
+          }
+          it.row0 = (__shfl_sync(0xffffffffu, tiles, src) - 1 - back) * kP4Rows;
           break;
         }
         carry += __shfl_sync(0xffffffffu, incl, 31);
+        if constexpr (SPLIT) split += __shfl_sync(0xffffffffu, incl2, 31);
         scan += 32;
       }
       it.q0 = max(0, a.cu_q[it.b]);
-      const int q_len = q_len_of(a, it.b);
+      const int q_len = p4_q_len(a, it.b);
       const int k_len = max(0, a.cu_k[it.b + 1] - a.cu_k[it.b]);
-      const int room = static_cast<int>(min(static_cast<int64_t>(0x7fffffff),
-                                            static_cast<int64_t>(a.bt_width) * a.c.block_size));
+      const int room = p4_room(a);
       it.offset = k_len - q_len;
       it.cut = k_len > room;
       it.rows = min(kP4Rows, q_len * a.group - it.row0);
       const int last = it.offset + (it.row0 + it.rows - 1) / a.group;  // last key of the last row
       it.n_kv = max(0, min(last + 1, room));
-      it.tiles = (it.n_kv + kP4Keys - 1) / kP4Keys;
+      const int all = (it.n_kv + kP4Keys - 1) / kP4Keys;
+      it.t0 = 0;
+      it.tiles = all;
+      if constexpr (SPLIT) {
+        it.t0 = static_cast<int>(static_cast<int64_t>(all) * seg / segs);
+        it.tiles = static_cast<int>(static_cast<int64_t>(all) * (seg + 1) / segs) - it.t0;
+      }
       return true;
     }
   }
@@ -263,7 +365,7 @@ __host__ __device__ constexpr uint32_t p4_idesc_f16(int m, int n, bool b_mn_majo
   return idesc_bf16_f32(m, n, false, b_mn_major) & ~((1u << 7) | (1u << 10));
 }
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Prefill4Args a) {
   using C = Pre4<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -280,8 +382,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   uint64_t *o_full = bars + 20;       // [2] the item's last P V done
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
   __shared__ int abort_flag;
-  __shared__ int lens[kP4Sorted];
-  __shared__ uint16_t order[kP4Sorted];
+  __shared__ Plan4 plan;
   // Per K/V tile (global count, modulo 4) and 32 tokens of it: what undoes K's power of two,
   // negative where V and P are bf16. Four tiles deep: a tile's entry is written anew only after
   // the V tile three before has been waited for, so after both softmaxes of the tile itself.
@@ -315,18 +416,8 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // S0 | S1 | O0 | O1, 128 columns each
   pdl_wait();
-  if (a.batch <= kP4Sorted) {
-    for (int b = tid; b < a.batch; b += kP4Threads) lens[b] = a.cu_k[b + 1] - a.cu_k[b];
-    __syncthreads();
-    for (int b = tid; b < a.batch; b += kP4Threads) {
-      int rank = 0;
-      for (int o = 0; o < a.batch; ++o) rank += lens[o] > lens[b] || (lens[o] == lens[b] && o < b);
-      order[rank] = static_cast<uint16_t>(b);
-    }
-    __syncthreads();
-  }
-
-  Walk4 walk{0, 0, 0, a.batch <= kP4Sorted ? order : nullptr};
+  p4_plan(a, plan);
+  Walk4<SPLIT> walk{0, 0, 0, 0, a.batch <= kP4Sorted ? plan.order : nullptr, plan.seg_tiles};
   Item4 it;
   // Waits as a whole warp: every lane of a role sees the same outcome.
   auto wait = [&](uint64_t *bar, uint32_t phase) {
@@ -399,7 +490,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
       // Half a tile: scores to P. MASKED where some row of the warp does not see all its keys.
       auto softmax_half = [&](auto masked, int j, int h, const float *factors) {
         constexpr bool MASKED = decltype(masked)::value;
-        const int lim = last - j * kP4Keys - h * 64;  // the last column this row sees
+        const int lim = last - ((SPLIT ? cur.t0 : 0) + j) * kP4Keys - h * 64;  // the last column this row sees
         const uint32_t at = s_base + h * 64;
         float mx = -INFINITY;
         float s[2][32];
@@ -474,7 +565,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
             if (!ok) break;
             tc_fence_after();
             if (warp_rows) {
-              if (__all_sync(0xffffffffu, j * kP4Keys + h * 64 + 63 <= all_seen))
+              if (__all_sync(0xffffffffu, ((SPLIT ? cur.t0 : 0) + j) * kP4Keys + h * 64 + 63 <= all_seen))
                 ok = softmax_half(std::false_type(), j, h, factors);
               else
                 ok = softmax_half(std::true_type(), j, h, factors);
@@ -495,7 +586,28 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
         ++po;
         tc_fence_after();
       }
-      if (cur.tiles == 0 ? warp_rows : mine && warp_rows) {
+      if (SPLIT && cur.slot >= 0) {  // a part: its maximum, sum and unscaled O
+        if (warp_rows) {
+          float *part = a.ws + (static_cast<int64_t>(cur.slot) * kP4Rows + row) * (D + 4);
+          const bool in = row < cur.rows;
+          if (in) *reinterpret_cast<float2 *>(part) = make_float2(m, l);
+          if (mine) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              tmem_ld32(o_base + c, o);
+              tmem_wait_ld();
+              if (in) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)  // (in the order of the columns; the join puts the dims back)
+                  *reinterpret_cast<float4 *>(part + 4 + c + 4 * i) =
+                      make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              }
+            }
+          }
+          tc_fence_before();
+        }
+      } else if (cur.tiles == 0 ? warp_rows : mine && warp_rows) {
         const bool in = row < cur.rows;
         const int head = (cur.row0 + row) - tok * a.group;
         const float inv = last >= 0 ? 1.f / l : 0.f;
@@ -547,7 +659,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
       uint4 kr[N], vr[N];
       uint2 pr[N];
       auto entry = [&](int j) -> int {  // the block of the warp's rows of tile j
-        const int key = j * kP4Keys + (warp - 8) * 32;
+        const int key = ((SPLIT ? it.t0 : 0) + j) * kP4Keys + (warp - 8) * 32;
         return even_blocks && key < it.n_kv ? table[key >> a.bs_shift] : 0;
       };
       auto usable = [&](int block) -> int {
@@ -556,7 +668,7 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
         return 0;
       };
       auto fetch = [&](int j, int block) {
-        const int first = j * kP4Keys + row0;
+        const int first = ((SPLIT ? it.t0 : 0) + j) * kP4Keys + row0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
@@ -780,17 +892,111 @@ __global__ void __launch_bounds__(kP4Threads, 1) paged_prefill4_kernel(const Pre
   }
 }
 
+// Joins the parts of split contexts: a CTA per row tile, KV head and 8 rows, a warp per row. Lanes
+// work out the parts' weights side by side, and no load waits for another (a part after the other,
+// 4 rows a warp: 48 us for 144 parts). Parts in order, so the sums do not depend on timing.
+constexpr int kP4JoinWarps = 8;
 template <int D>
-int launch_prefill4(const Prefill4Args &a, int64_t total_q, cudaStream_t stream) {
+__global__ void __launch_bounds__(kP4JoinWarps * 32) paged_prefill4_join_kernel(const Prefill4Args a) {
+  __shared__ Plan4 plan;
+  pdl_trigger();
+  pdl_wait();
+  p4_plan(a, plan);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.c.num_kv_heads;
+  const int t = blockIdx.x / heads, h = blockIdx.x - t * heads;
+  int b = -1, back = 0, segs = 1, tiles = 0, first = 0;  // first: the row tile's first part
+  for (int scan = 0, carry = 0, split = 0; scan < a.batch; scan += 32) {
+    const int bb = scan + lane < a.batch ? plan.order[scan + lane] : a.batch;
+    const int parts = bb < a.batch ? p4_segs(a, bb, plan.seg_tiles) : 1;
+    const int n = parts > 1 ? p4_row_tiles(a, bb) : 0;
+    int incl = n, incl2 = n * parts;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o), z = __shfl_up_sync(0xffffffffu, incl2, o);
+      if (lane >= o) {
+        incl += y;
+        incl2 += z;
+      }
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, t < carry + incl);
+    if (here) {
+      const int src = __ffs(here) - 1;
+      b = __shfl_sync(0xffffffffu, bb, src);
+      segs = __shfl_sync(0xffffffffu, parts, src);
+      tiles = __shfl_sync(0xffffffffu, n, src);
+      back = t - carry - __shfl_sync(0xffffffffu, incl - n, src);
+      first = split + __shfl_sync(0xffffffffu, incl2 - n * parts, src) + back * segs;
+      break;
+    }
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+    split += __shfl_sync(0xffffffffu, incl2, 31);
+  }
+  if (b < 0) return;
+  const int row0 = (tiles - 1 - back) * kP4Rows, rows = min(kP4Rows, p4_q_len(a, b) * a.group - row0);
+  const int q0 = max(0, a.cu_q[b]);
+  constexpr int PER = D / 32;  // columns of a lane
+  const int r = blockIdx.y * kP4JoinWarps + warp;
+  if (r >= rows) return;
+  const int64_t step = static_cast<int64_t>(heads) * kP4Rows * (D + 4);  // between parts
+  const float *x = a.ws + ((static_cast<int64_t>(first) * heads + h) * kP4Rows + r) * (D + 4);
+  float m = -INFINITY;
+  for (int i = lane; i < segs; i += 32) m = fmaxf(m, x[i * step]);
+  m = warp_max(m);
+  float den = 0.f, o[PER] = {};
+  for (int i0 = 0; i0 < segs; i0 += 32) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (i0 + lane < segs) ml = *reinterpret_cast<const float2 *>(x + (i0 + lane) * step);
+    // a part of which the row sees no key has written no O
+    const unsigned seen = __ballot_sync(0xffffffffu, !(ml.x == -INFINITY && ml.y == 0.f));
+    const float by = ml.x == -INFINITY ? 1.f : exp2f(ml.x - m);
+    den += warp_sum((seen >> lane) & 1 ? by * ml.y : 0.f);
+#pragma unroll 8
+    for (int i = 0; i < min(32, segs - i0); ++i) {
+      const float w = __shfl_sync(0xffffffffu, by, i);
+      const bool in = (seen >> i) & 1;
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        o[e] = fmaf(in ? w : 0.f, in ? x[(i0 + i) * step + 4 + e * 32 + lane] : 0.f, o[e]);
+    }
+  }
+  const int tok = (row0 + r) / a.group, head = (row0 + r) - tok * a.group;
+  __nv_bfloat16 *dst = a.out + (q0 + tok) * a.out_row + (static_cast<int64_t>(h) * a.group + head) * a.out_head;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  // columns of a group of 8 hold dims 0, 4, 1, 5, 2, 6, 3, 7
+  const int dim = (lane & ~7) + ((lane & 7) >> 1) + (lane & 1) * 4;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) dst[e * 32 + dim] = f2bf(o[e] * inv);
+}
+
+// Upper bound of the items, and whether contexts are split at all: a part costs what ~4 tiles do
+// (its first loads, its partials and the join), so only where at least half of the SMs would be
+// idle (a mixed batch of ~130 items on 148 SMs: 112 us split, 69 not).
+inline int64_t prefill4_items(int64_t total_q, int batch, int group, int heads) {
+  return ((total_q * group + kP4Rows - 1) / kP4Rows + batch) * heads;
+}
+inline bool prefill4_splits(int64_t items, int batch) { return batch <= kP4Sorted && items <= num_sms() / 2; }
+
+template <int D>
+int launch_prefill4(Prefill4Args a, size_t ws_bytes, cudaStream_t stream) {
   using C = Pre4<D>;
-  const int64_t most = ((total_q * a.group + kP4Rows - 1) / kP4Rows + a.batch) * a.c.num_kv_heads;
-  B200_REQUIRE(most <= 0x3fffffff && total_q * a.group <= 0x3fffffff, "paged_prefill4: too many rows");
-  auto kfn = paged_prefill4_kernel<D>;
+  const int64_t most = prefill4_items(a.total_q, a.batch, a.group, a.c.num_kv_heads);
+  B200_REQUIRE(most <= 0x3fffffff && static_cast<int64_t>(a.total_q) * a.group <= 0x3fffffff,
+               "paged_prefill4: too many rows");
+  a.max_slots = static_cast<int>(std::min<size_t>(2 * num_sms(), ws_bytes / (kP4Rows * (D + 4) * 4)));
+  if (!prefill4_splits(most, a.batch) || a.max_slots < 2) a.ws = nullptr;
+  auto kfn = a.ws != nullptr ? paged_prefill4_kernel<D, true> : paged_prefill4_kernel<D, false>;
   B200_LAUNCH_CHECK_ERR(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
                         "paged_prefill4 (configuration)");
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(most, num_sms()));
+  const unsigned grid = static_cast<unsigned>(a.ws != nullptr ? num_sms() : std::min<int64_t>(most, num_sms()));
+  a.ctas = static_cast<int>(grid);
   B200_LAUNCH_CHECK_ERR(launch_kernel(kfn, dim3(grid), dim3(kP4Threads), C::SMEM, stream, true, 1, a),
                         "paged_prefill4");
+  if (a.ws != nullptr)
+    B200_LAUNCH_CHECK_ERR(launch_kernel(paged_prefill4_join_kernel<D>,
+                                        dim3(static_cast<unsigned>(std::min<int64_t>(most, a.max_slots / 2)),
+                                             kP4Rows / kP4JoinWarps),
+                                        dim3(kP4JoinWarps * 32), 0, stream, true, 1, a),
+                          "paged_prefill4 (join)");
   return B200ASR_OK;
 }
 
@@ -798,13 +1004,25 @@ int launch_prefill4(const Prefill4Args &a, int64_t total_q, cudaStream_t stream)
 
 using namespace b200asr;
 
+extern "C" size_t b200asr_paged_prefill4_workspace_size(int32_t total_q, int32_t batch, int32_t max_seqlen_k,
+                                                        int32_t num_heads, int32_t num_kv_heads,
+                                                        int32_t head_dim) {
+  if (total_q < 1 || batch < 1 || max_seqlen_k <= 2 * kP4MinSeg * kP4Keys || num_kv_heads < 1 ||
+      num_heads < num_kv_heads || head_dim < 1)
+    return 0;
+  const int64_t items = prefill4_items(total_q, batch, num_heads / num_kv_heads, num_kv_heads);
+  if (!prefill4_splits(items, batch)) return 0;
+  return static_cast<size_t>(2 * num_sms()) * kP4Rows * (head_dim + 4) * 4;
+}
+
 extern "C" int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64_t q_head_stride,
                                       const b200asr_kv4 *cache, int32_t num_heads,
                                       const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
                                       const int32_t *block_tables, int64_t bt_stride,
                                       int32_t bt_width, int32_t batch, int32_t total_q, float scale,
                                       void *out, int64_t out_row_stride, int64_t out_head_stride,
-                                      int32_t *error_flag, b200asr_stream_t stream) {
+                                      void *workspace, size_t workspace_bytes, int32_t *error_flag,
+                                      b200asr_stream_t stream) {
   B200_REQUIRE(cache != nullptr, "paged_prefill4: null cache");
   const int D = cache->head_dim;
   B200_REQUIRE(D == 64 || D == 128, "paged_prefill4: head_dim %d unsupported (64 or 128)", D);
@@ -820,6 +1038,7 @@ extern "C" int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64
   B200_REQUIRE(aligned16(q) && aligned16(out) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0 &&
                    out_row_stride % 8 == 0 && out_head_stride % 8 == 0,
                "paged_prefill4: q and out rows must be 16-byte aligned");
+  B200_REQUIRE(aligned16(workspace), "paged_prefill4: workspace alignment");
   Prefill4Args a{};
   a.q = static_cast<const __nv_bfloat16 *>(q);
   a.q_row = q_row_stride;
@@ -840,7 +1059,8 @@ extern "C" int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.out_row = out_row_stride;
   a.out_head = out_head_stride;
+  a.ws = static_cast<float *>(workspace);
   a.error_flag = error_flag;
-  return D == 128 ? launch_prefill4<128>(a, total_q, static_cast<cudaStream_t>(stream))
-                  : launch_prefill4<64>(a, total_q, static_cast<cudaStream_t>(stream));
+  return D == 128 ? launch_prefill4<128>(a, workspace_bytes, static_cast<cudaStream_t>(stream))
+                  : launch_prefill4<64>(a, workspace_bytes, static_cast<cudaStream_t>(stream));
 }

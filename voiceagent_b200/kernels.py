@@ -517,12 +517,24 @@ def paged_decode4(q, k_codes, v_codes, kv_params, cu_seqlens_k, block_tables, *,
     return out
 
 
+# max_seqlen_k at or below this is never split; must match kP4MinSeg and kP4Keys in
+# csrc/kv4_prefill.cu.
+PREFILL4_WHOLE_CTX = 1024
+
+
+def paged_prefill4_workspace_size(total_q: int, batch: int, max_seqlen_k: int, num_heads: int,
+                                  num_kv_heads: int, head_dim: int = 128) -> int:
+    return int(lib.b200asr_paged_prefill4_workspace_size(total_q, batch, max_seqlen_k, num_heads,
+                                                         num_kv_heads, head_dim))
+
+
 def paged_prefill4(q, k_codes, v_codes, kv_params, cu_seqlens_q, cu_seqlens_k, block_tables, *,
-                   max_seqlen_q: int, max_seqlen_k: int, scale: float, out,
+                   max_seqlen_q: int, max_seqlen_k: int, scale: float, out, workspace=None,
                    error_flag=None) -> torch.Tensor:
     """:func:`paged_prefill` over a 4-bit cache: varlen causal attention (the mask aligned
     bottom-right) of q [total_q, H, D], H any multiple of H_kv, D 64 or 128; a row that sees
-    no key gives zeros."""
+    no key gives zeros. ``workspace`` (uint8, :func:`paged_prefill4_workspace_size` bytes, any
+    contents, one call at a time) is taken from the caching allocator when not given."""
     what = "paged_prefill4"
     cache, heads, dim = _kv4(what, k_codes, v_codes, kv_params)
     qs, os, batch, bt_stride, bt_width = _attention4_args(what, q, out, cu_seqlens_k, block_tables,
@@ -531,13 +543,20 @@ def paged_prefill4(q, k_codes, v_codes, kv_params, cu_seqlens_q, cu_seqlens_k, b
             or not cu_seqlens_q.is_contiguous()):
         _bad(what, "cu_seqlens_q like cu_seqlens_k")
     rows, q_heads, _ = q.shape
+    ws, ws_bytes = None, 0
+    if workspace is None and max_seqlen_k > PREFILL4_WHOLE_CTX:
+        ws_bytes = lib.b200asr_paged_prefill4_workspace_size(rows, batch, max_seqlen_k, q_heads, heads, dim)
+        if ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=_U8, device=q.device)
+    if workspace is not None:
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     _here(what, k_codes, v_codes, kv_params, q, out, cu_seqlens_q, cu_seqlens_k, block_tables,
-          error_flag)
-    _count()
+          workspace, error_flag)
+    _count(2 if ws_bytes else 1)  # + the join of split contexts
     check(lib.b200asr_paged_prefill4(
         q.data_ptr(), qs[0], qs[1], cache, q_heads, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
         block_tables.data_ptr(), bt_stride, bt_width, batch, rows, scale, out.data_ptr(), os[0], os[1],
-        _p(error_flag), _stream()), what)
+        ws, ws_bytes, _p(error_flag), _stream()), what)
     return out
 
 

@@ -94,6 +94,7 @@ constexpr int kP4MinSeg = 4;     // K/V tiles of a part, at least
 // and the join cost about as much (two requests of 400 rows on 1400 and 778 keys, 6 fewer: 58 us
 // split, 44 not; one of 200 on 2200, 14 fewer: 38 and 60).
 constexpr int kP4MinSaved = 8;
+constexpr int kP4Whole = 0x7fffffff;
 struct Plan4 {
   int lens[kP4Sorted];
   uint16_t order[kP4Sorted];  // sequences by falling length

@@ -59,7 +59,8 @@ struct Prefill4Args {
   uint32_t flip;     // sign bit to exchange in q
   __nv_bfloat16 *out;
   int64_t out_row, out_head;
-  float *ws;      // partials of split contexts: [slots][256 rows][D + 4] (maximum, sum, -, -, O), or null
+  float *ws;      // partials of split contexts: [slots][256 rows][D + 4] (maximum, sum, -, -, O), or null;
+                  // the 16 bytes before them hold the parts' tiles
   int max_slots, ctas;
   int32_t *error_flag;
 };
@@ -87,13 +88,13 @@ struct Item4 {
 // Every warp walks alone and sees the same items.
 // Where that leaves SMs idle, contexts are split into parts of about `seg_tiles` K/V tiles, every
 // row tile of a sequence into as many, whose partials a second kernel joins in order: 200 tokens of
-// 16 query heads on 8 behind a cached prefix of 8k tokens 54 us, 183 unsplit.
+// 16 query heads on 8 behind a cached prefix of 8k tokens 54 us, 182 unsplit.
 constexpr int kP4Sorted = 256;   // sequences up to which they are sorted, and split
 constexpr int kP4MinSeg = 4;     // K/V tiles of a part, at least
 // K/V tiles that the longest context gets shorter by, at least: a part's first loads, its partials
-// and the join cost about as much (two requests of 400 rows on 1400 and 778 keys, 6 fewer: 58 us
-// split, 44 not; one of 200 on 2200, 14 fewer: 38 and 60).
-constexpr int kP4MinSaved = 8;
+// and the join cost about as much (one request of 200 tokens on 1200 keys, 6 fewer: 33 us split, 39
+// not; two of 400 on 1400 and 778, 6 fewer: 49 and 44).
+constexpr int kP4MinSaved = 5;
 constexpr int kP4Whole = 0x7fffffff;
 struct Plan4 {
   int lens[kP4Sorted];
@@ -119,9 +120,21 @@ __device__ __forceinline__ int p4_segs(const Prefill4Args &a, int b, int seg_til
   return max(1, ((keys + kP4Keys - 1) / kP4Keys + seg_tiles - 1) / seg_tiles);
 }
 
+__device__ __forceinline__ void p4_order(const Prefill4Args &a, Plan4 &plan) {
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x) plan.lens[b] = a.cu_k[b + 1] - a.cu_k[b];
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+    const int len = plan.lens[b];
+    int rank = 0;
+    for (int o = 0; o < a.batch; ++o) rank += plan.lens[o] > len || (plan.lens[o] == len && o < b);
+    plan.order[rank] = static_cast<uint16_t>(b);
+  }
+  __syncthreads();
+}
+
 // The order of the sequences, and how long the parts of split contexts are: an even share of all
 // K/V tiles, or as much longer as it takes for every CTA to have one part at most and for the
-// partials to fit. The same in every CTA and in the join.
+// partials to fit. The same in every CTA; the first leaves it before the partials, for the join.
 __device__ __forceinline__ void p4_plan(const Prefill4Args &a, Plan4 &plan) {
   const int tid = threadIdx.x;
   if (tid == 0) {
@@ -129,16 +142,10 @@ __device__ __forceinline__ void p4_plan(const Prefill4Args &a, Plan4 &plan) {
     plan.sum[0] = plan.sum[1] = plan.sum[2] = 0;
   }
   if (a.batch <= kP4Sorted) {
-    for (int b = tid; b < a.batch; b += blockDim.x) plan.lens[b] = a.cu_k[b + 1] - a.cu_k[b];
-    __syncthreads();
-    for (int b = tid; b < a.batch; b += blockDim.x) {
-      const int len = plan.lens[b];
-      int rank = 0;
-      for (int o = 0; o < a.batch; ++o) rank += plan.lens[o] > len || (plan.lens[o] == len && o < b);
-      plan.order[rank] = static_cast<uint16_t>(b);
-      if (a.ws != nullptr)
+    p4_order(a, plan);
+    if (a.ws != nullptr)
+      for (int b = tid; b < a.batch; b += blockDim.x)
         atomicAdd(&plan.sum[0], static_cast<unsigned long long>(p4_row_tiles(a, b)) * p4_segs(a, b, 1));
-    }
     __syncthreads();
     if (a.ws != nullptr) {
       int seg = static_cast<int>(min(static_cast<unsigned long long>(1 << 29),
@@ -164,6 +171,7 @@ __device__ __forceinline__ void p4_plan(const Prefill4Args &a, Plan4 &plan) {
     }
   }
   __syncthreads();
+  if (a.ws != nullptr && blockIdx.x == 0 && tid == 0) *reinterpret_cast<int *>(a.ws - 4) = plan.seg_tiles;
 }
 
 template <bool SPLIT>
@@ -902,13 +910,15 @@ __global__ void __launch_bounds__(kP4JoinWarps * 32) paged_prefill4_join_kernel(
   __shared__ Plan4 plan;
   pdl_trigger();
   pdl_wait();
-  p4_plan(a, plan);
+  const int seg_tiles = *reinterpret_cast<const int *>(a.ws - 4);
+  if (seg_tiles == kP4Whole) return;
+  p4_order(a, plan);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.c.num_kv_heads;
   const int t = blockIdx.x / heads, h = blockIdx.x - t * heads;
   int b = -1, back = 0, segs = 1, tiles = 0, first = 0;  // first: the row tile's first part
   for (int scan = 0, carry = 0, split = 0; scan < a.batch; scan += 32) {
     const int bb = scan + lane < a.batch ? plan.order[scan + lane] : a.batch;
-    const int parts = bb < a.batch ? p4_segs(a, bb, plan.seg_tiles) : 1;
+    const int parts = bb < a.batch ? p4_segs(a, bb, seg_tiles) : 1;
     const int n = parts > 1 ? p4_row_tiles(a, bb) : 0;
     int incl = n, incl2 = n * parts;
 #pragma unroll
@@ -983,8 +993,9 @@ int launch_prefill4(Prefill4Args a, size_t ws_bytes, cudaStream_t stream) {
   const int64_t most = prefill4_items(a.total_q, a.batch, a.group, a.c.num_kv_heads);
   B200_REQUIRE(most <= 0x3fffffff && static_cast<int64_t>(a.total_q) * a.group <= 0x3fffffff,
                "paged_prefill4: too many rows");
-  a.max_slots = static_cast<int>(std::min<size_t>(2 * num_sms(), ws_bytes / (kP4Rows * (D + 4) * 4)));
+  a.max_slots = static_cast<int>(std::min<size_t>(2 * num_sms(), (std::max<size_t>(ws_bytes, 16) - 16) / (kP4Rows * (D + 4) * 4)));
   if (!prefill4_splits(most, a.batch) || a.max_slots < 2) a.ws = nullptr;
+  if (a.ws != nullptr) a.ws += 4;
   auto kfn = a.ws != nullptr ? paged_prefill4_kernel<D, true> : paged_prefill4_kernel<D, false>;
   B200_LAUNCH_CHECK_ERR(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
                         "paged_prefill4 (configuration)");
@@ -1013,7 +1024,7 @@ extern "C" size_t b200asr_paged_prefill4_workspace_size(int32_t total_q, int32_t
     return 0;
   const int64_t items = prefill4_items(total_q, batch, num_heads / num_kv_heads, num_kv_heads);
   if (!prefill4_splits(items, batch)) return 0;
-  return static_cast<size_t>(2 * num_sms()) * kP4Rows * (head_dim + 4) * 4;
+  return 16 + static_cast<size_t>(2 * num_sms()) * kP4Rows * (head_dim + 4) * 4;
 }
 
 extern "C" int b200asr_paged_prefill4(const void *q, int64_t q_row_stride, int64_t q_head_stride,

@@ -243,6 +243,13 @@ def test_wrappers_refuse_cpu_tensors_and_wrong_types(kx):
         kx.load_kvcache4(kc, vc[:, :8], par, slots)
     with pytest.raises(ValueError, match="64 or 128"):
         kx.kv4_cache(2, 16, 2, 96, device="cpu")
+    table, starts = torch.zeros(3, 1, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    wide = torch.empty(1, dtype=torch.uint8).expand(1 << 26)
+    with pytest.raises(ValueError, match="contiguous workspace"):
+        kx.paged_decode4(x, kc, vc, par, starts, table, max_seqlen_k=2000, scale=1.0, out=x, workspace=wide)
+    with pytest.raises(ValueError, match="contiguous workspace"):
+        kx.paged_prefill4(x, kc, vc, par, starts, starts, table, max_seqlen_q=1, max_seqlen_k=2000, scale=1.0, out=x,
+                          workspace=wide)
 
 
 # ---------------------------------------------------------------------- rows in and out

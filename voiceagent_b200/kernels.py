@@ -476,6 +476,12 @@ def _attention4_args(what: str, q, out, cu_seqlens_k, block_tables, heads: int, 
     return qs, os, batch, bs[0], table[1]
 
 
+def _workspace(what: str, workspace):
+    if not workspace.is_contiguous():  # its bytes are counted by its elements
+        _bad(what, "a contiguous workspace")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 # max_seqlen_k at or below this is one launch without a workspace; must match kD4WholeMax in
 # csrc/kv4_decode.cu.
 DECODE4_WHOLE_CTX = 1024
@@ -503,7 +509,7 @@ def paged_decode4(q, k_codes, v_codes, kv_params, cu_seqlens_k, block_tables, *,
         _bad(what, "cu_seqlens_k longer than the batch")
     ws, ws_bytes = None, 0
     if workspace is not None:
-        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        ws, ws_bytes = _workspace(what, workspace)
     elif max_seqlen_k > DECODE4_WHOLE_CTX:
         ws_bytes = lib.b200asr_paged_decode4_workspace_size(max_seqlen_k, q_heads, heads, dim)
         workspace = torch.empty(ws_bytes, dtype=_U8, device=q.device)
@@ -549,7 +555,7 @@ def paged_prefill4(q, k_codes, v_codes, kv_params, cu_seqlens_q, cu_seqlens_k, b
         if ws_bytes:
             workspace = torch.empty(ws_bytes, dtype=_U8, device=q.device)
     if workspace is not None:
-        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        ws, ws_bytes = _workspace(what, workspace)
     _here(what, k_codes, v_codes, kv_params, q, out, cu_seqlens_q, cu_seqlens_k, block_tables,
           workspace, error_flag)
     _count(2 if ws_bytes else 1)  # + the join of split contexts

@@ -10,7 +10,7 @@
 //
 // What bounds it: at 136 bytes per cached (token, KV head) of D = 128 the bytes are a quarter
 // of the bf16 cache's, and turning codes into MMA operands costs ~240 instructions per 16
-// tokens, ~65 % of the SM's issue slots at the copy rate of HBM; so instructions are counted:
+// tokens, ~60 % of the SM's issue slots at the copy rate of HBM; so instructions are counted:
 //  * MMA m16n8k16 with cached tokens (scores) or dims (output) as its 16 rows and the group's
 //    query heads as its 8 columns. Scores in fp16: a word of 8 codes becomes four pairs by a mask
 //    and an or, each 1024 + code or, in place, 1024 + 16 code (its q is a sixteenth), so a word
